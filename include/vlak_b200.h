@@ -233,6 +233,69 @@ VLAK_API int vlak_attn_fwd(const void* q, const void* k, const void* v, void* o,
                            int64_t B, int64_t H, int64_t M, int64_t N, const void* mask,
                            double scale, void* stream);
 
+/* ------------------------------------------------------------------------
+ * Position rotation of query / key heads, alone or behind a per-head RMS
+ * norm in the same pass. No counterpart in the reference, which leaves both
+ * to the model's elementwise code.
+ *
+ * Per head of D entries, the first rotary_dim entries form pairs (a, b): half
+ * layout (i, i + rotary_dim / 2), interleaved (2i, 2i + 1). With
+ * t = position * inv_freq[i] and A = amplitude
+ *   y_a = A (u_a cos t - u_b sin t), y_b = A (u_b cos t + u_a sin t);
+ * the other entries pass through. u = x (vlak_rotary), or
+ * u = x * rsqrt(mean(x^2) + eps) * weight (vlak_qk_norm_rotary_fwd).
+ * Angles are taken in 64 bits, all other math in 32; one rounding per output.
+ *
+ *   t[0..n_tensors) : queries, and keys if there are any, of one token grid
+ *                     (B, M); heads H and strides of each its own
+ *   x, grad         : (B, M, H, D), element strides for (b, m, h), entries
+ *                     contiguous; strides of 0 broadcast
+ *   y               : contiguous (B, M, H, D); must not overlap x or grad
+ *   dtype           : VLAK_F32 / VLAK_F16 / VLAK_BF16 of x, grad and y
+ *   weight          : (D), weight_dtype VLAK_F32 or dtype
+ *   positions       : VLAK_I32 / VLAK_I64, element strides for (b, m); any
+ *                     sign, magnitudes up to 2^53
+ *   inv_freq        : rotary_dim / 2 doubles, radians per position
+ *   inverse         : turn the other way (the gradient of vlak_rotary)
+ * D even, 2 to 1024; rotary_dim even, 2 to D. B == 0 or M == 0 is a no-op
+ * (backward: zero weight gradients).
+ *
+ * vlak_qk_norm_rotary_bwd takes x (the forward's input) and grad (of its
+ * output), writes y = dL/dx and grad_weight = dL/dweight (weight_dtype). The
+ * weights' gradient is summed in a fixed order through `workspace` (device,
+ * 16-byte aligned, vlak_qk_norm_rotary_workspace_size bytes), which must stay
+ * unused by anything else until the work on `stream` has finished.
+ * ---------------------------------------------------------------------- */
+typedef struct {
+  const void* x;
+  const void* grad;    /* backward only */
+  void* y;
+  const void* weight;  /* norm only */
+  void* grad_weight;   /* backward only */
+  int64_t H;
+  int64_t x_stride[3];
+  int64_t grad_stride[3];
+} vlak_rotary_tensor;
+
+typedef struct {
+  vlak_rotary_tensor t[2];
+  const void* positions;
+  const double* inv_freq;
+  int64_t B, M, D, rotary_dim;
+  int64_t pos_stride[2];
+  double amplitude;
+  double eps;
+  int n_tensors;
+  int dtype, pos_dtype, weight_dtype;
+  int interleaved, inverse;
+} vlak_rotary_args;
+
+VLAK_API int vlak_rotary(const vlak_rotary_args* args, void* stream);
+VLAK_API int vlak_qk_norm_rotary_fwd(const vlak_rotary_args* args, void* stream);
+VLAK_API int vlak_qk_norm_rotary_workspace_size(const vlak_rotary_args* args, int64_t* bytes);
+VLAK_API int vlak_qk_norm_rotary_bwd(const vlak_rotary_args* args, void* workspace,
+                                     int64_t workspace_bytes, void* stream);
+
 /* Self-test of the bounded device waits. No counterpart in the reference:
  * a test hook for the failure path that replaces a hang. Launches, on
  * `stream`, one kernel that waits on a barrier nothing completes; after the

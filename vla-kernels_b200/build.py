@@ -19,20 +19,24 @@ import os
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 REPO = os.path.dirname(PKG_DIR)
 CSRC = os.path.join(PKG_DIR, "csrc")
 LIB_DIR = os.path.join(PKG_DIR, "lib")
+OBJ_DIR = os.path.join(LIB_DIR, "obj")  # object files, one per source
 INCLUDE = os.path.join(REPO, "include")
 
 CAPI_LIB = os.path.join(LIB_DIR, "libvlak_b200.so")
 TORCH_LIB = os.path.join(LIB_DIR, "libvlak_torch.so")
 CMP_LIB = os.path.join(LIB_DIR, "libvlak_comparators.so")
 
-CU_SOURCES = ["capi.cu", "softmax.cu", "attention_gqa.cu", "attention_simt.cu"]
+CU_SOURCES = ["capi.cu", "softmax.cu", "attention_gqa.cu", "attention_simt.cu",
+              "rotary.cu"]
 HEADERS = ["vlak_device.cuh", "vlak_internal.h"]
-SHIM_SOURCES = ["torch_ops.cpp"]
+SHIM_SOURCES = ["torch_ops.cpp", "torch_rotary.cpp"]
+SHIM_HEADERS = ["vlak_torch.h"]
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
@@ -61,19 +65,28 @@ def _run(cmd: list[str]) -> None:
                            f"{r.stdout}\n{r.stderr}")
 
 
+def _compile_all(jobs: list[tuple[list[str], str]]) -> None:
+    """Run compile commands, each (command, object), side by side."""
+    with ThreadPoolExecutor(max_workers=os.cpu_count() or 1) as pool:
+        list(pool.map(lambda job: _run(job[0] + ["-o", job[1]]), jobs))
+
+
 def build_capi(force: bool = False, verbose_ptxas: bool = False) -> str:
+    headers = [os.path.join(CSRC, h) for h in HEADERS] + [os.path.join(INCLUDE, "vlak_b200.h")]
     srcs = [os.path.join(CSRC, s) for s in CU_SOURCES]
-    deps = srcs + [os.path.join(CSRC, h) for h in HEADERS] + [os.path.join(INCLUDE, "vlak_b200.h")]
-    if not force and not _stale(CAPI_LIB, deps):
+    if not force and not _stale(CAPI_LIB, srcs + headers):
         return CAPI_LIB
     os.makedirs(LIB_DIR, exist_ok=True)
+    os.makedirs(OBJ_DIR, exist_ok=True)
     nvcc = os.path.join(_cuda_home(), "bin", "nvcc")
-    cmd = [nvcc, *ARCH_FLAGS, "-O3", "-lineinfo", "-std=c++17", "--shared",
-           "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",
-           "-I", INCLUDE, "-o", CAPI_LIB + ".tmp", *srcs]
+    flags = [*ARCH_FLAGS, "-O3", "-lineinfo", "-std=c++17",
+             "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden", "-I", INCLUDE]
     if verbose_ptxas:
-        cmd.insert(1, "-Xptxas=-v")
-    _run(cmd)
+        flags.insert(0, "-Xptxas=-v")
+    objs = [os.path.join(OBJ_DIR, os.path.basename(s) + ".o") for s in srcs]
+    _compile_all([([nvcc, *flags, "-c", s], o) for s, o in zip(srcs, objs)
+                  if force or _stale(o, [s, *headers])])
+    _run([nvcc, *ARCH_FLAGS, "--shared", "-o", CAPI_LIB + ".tmp", *objs])
     os.replace(CAPI_LIB + ".tmp", CAPI_LIB)
     return CAPI_LIB
 
@@ -82,19 +95,24 @@ def build_torch_shim(force: bool = False) -> str:
     import torch.utils.cpp_extension as cpp
 
     srcs = [os.path.join(CSRC, s) for s in SHIM_SOURCES]
-    deps = srcs + [os.path.join(INCLUDE, "vlak_b200.h"), CAPI_LIB]
+    deps = (srcs + [os.path.join(CSRC, h) for h in SHIM_HEADERS]
+            + [os.path.join(INCLUDE, "vlak_b200.h"), CAPI_LIB])
     if not force and not _stale(TORCH_LIB, deps):
         return TORCH_LIB
     os.makedirs(LIB_DIR, exist_ok=True)
     import torch
 
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
-    cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC",
+    os.makedirs(OBJ_DIR, exist_ok=True)
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-c",
            f"-D_GLIBCXX_USE_CXX11_ABI={abi}", "-DTORCH_API_INCLUDE_EXTENSION_H",
            "-I", INCLUDE, "-I", os.path.join(_cuda_home(), "include")]
     for inc in cpp.include_paths():
         cmd += ["-isystem", inc]
-    cmd += ["-o", TORCH_LIB + ".tmp", *srcs]
+    objs = [os.path.join(OBJ_DIR, os.path.basename(s) + ".o") for s in srcs]
+    _compile_all([(cmd + [s], o) for s, o in zip(srcs, objs)
+                  if force or _stale(o, [s, *deps[len(srcs):-1]])])
+    cmd = ["g++", "-shared", "-o", TORCH_LIB + ".tmp", *objs]
     for libdir in cpp.library_paths():
         cmd += ["-L", libdir, f"-Wl,-rpath,{libdir}"]
     cmd += ["-L", LIB_DIR, "-Wl,-rpath,$ORIGIN", "-lvlak_b200",

@@ -20,25 +20,13 @@
 #include <optional>
 
 #include "vlak_b200.h"
+#include "vlak_torch.h"
 
 namespace {
 
-void check_status(int status, const char* op) {
-  TORCH_CHECK(status == VLAK_OK, op, ": ", vlak_last_error_message(), " (",
-              vlak_status_string(status), ")");
-}
-
-// Every op first reads the host-mapped error word (no device
-// synchronization): a bounded wait that ran out in an attention kernel which
-// has finished since is raised here, on the caller's next op, instead of
-// going unnoticed. The word is cleared by the read, so the following call
-// runs normally.
-void raise_pending_device_error(const char* op) {
-  int code = VLAK_OK;
-  vlak_device_error_poll(&code);
-  TORCH_CHECK(code == VLAK_OK, op, ": an earlier vlak kernel gave up a bounded device wait (",
-              vlak_status_string(code), "); the output of that call is incomplete");
-}
+using vlak_torch::check_status;
+using vlak_torch::dtype_code;
+using vlak_torch::raise_pending_device_error;
 
 // vlak::device_error(): the synchronous check. Waits for the device, then
 // reads and clears the error words; returns the status found (0 = none).
@@ -47,16 +35,6 @@ int64_t device_error() {
   c10::cuda::device_synchronize();
   check_status(vlak_device_error_read(&code), "vlak::device_error");
   return code;
-}
-
-int dtype_code(at::ScalarType t) {
-  switch (t) {
-    case at::kFloat: return VLAK_F32;
-    case at::kHalf: return VLAK_F16;
-    case at::kBFloat16: return VLAK_BF16;
-    case at::kDouble: return VLAK_F64;
-    default: return -1;
-  }
 }
 
 // kernels/softmax/softmax_kernels.cu:255-297
