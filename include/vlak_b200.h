@@ -234,6 +234,55 @@ VLAK_API int vlak_attn_fwd(const void* q, const void* k, const void* v, void* o,
                            double scale, void* stream);
 
 /* ------------------------------------------------------------------------
+ * GQA attention for training: a forward pass that also stores each row's
+ * log-sum, and a backward pass that recomputes the probabilities from it. No
+ * counterpart in the reference, whose kernels are forward only.
+ *
+ *   attn     : q, k, v, o, sizes, strides, scale and analytic mask as in
+ *              vlak_attn_gqa_fwd (o is written by the forward and read by the
+ *              backward call)
+ *   lengths  : NULL, or per-sample lengths as in vlak_attn_gqa_varlen_fwd
+ *   mask     : NULL, or a bool mask as in vlak_attn_gqa_masked_fwd; at most one
+ *              of the two, and the analytic fields are ignored with either
+ *   lse      : contiguous (B, M, H) fp32: log2 of the sum of 2^(scale log2(e)
+ *              q.k) over the keys a row sees, -inf for a row that sees none;
+ *              written by the forward call and read by the backward call
+ *   grad_o   : gradient of o, bf16, strides as q (backward only)
+ *   dq       : contiguous (B, M, H, 64) bf16 (backward only)
+ *   dk, dv   : contiguous (B, N, Hkv, 64) bf16, summed over the G query heads
+ *              of each kv head (backward only); both NULL for dq alone
+ * Rows that see no key get dq = 0 and add nothing to dk and dv. Keys that no
+ * row sees by the analytic mask or the lengths may hold anything (NaN
+ * included), and so may rows past their sample's length; those get dk, dv or
+ * dq = 0. Behind a bool mask every value must be finite. A NaN or infinity
+ * that is seen spreads as in the formulas. Results repeat bit for bit.
+ *
+ * Workspaces: device, 256-byte aligned, owned by the caller and unused by
+ * anything else until the work on `stream` has finished. The forward one is
+ * optional and sized by vlak_attn_gqa_workspace_size (key splits of small
+ * batches); the backward one is required, vlak_attn_gqa_bwd_workspace_size.
+ * ---------------------------------------------------------------------- */
+typedef struct {
+  vlak_attn_gqa_args attn;
+  const void* lengths;
+  const void* mask;
+  int64_t mask_stride_b, mask_stride_m;
+  float* lse;
+  const void* grad_o;
+  int64_t grad_o_stride[3];
+  void* dq;
+  void* dk;
+  void* dv;
+  int lengths_dtype; /* VLAK_I32 or VLAK_I64 */
+} vlak_attn_train_args;
+
+VLAK_API int vlak_attn_gqa_train_fwd(const vlak_attn_train_args* args, void* workspace,
+                                     int64_t workspace_bytes, void* stream);
+VLAK_API int vlak_attn_gqa_bwd_workspace_size(const vlak_attn_train_args* args, int64_t* bytes);
+VLAK_API int vlak_attn_gqa_bwd(const vlak_attn_train_args* args, void* workspace,
+                               int64_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------
  * Position rotation of query / key heads, alone or behind a per-head RMS
  * norm in the same pass. No counterpart in the reference, which leaves both
  * to the model's elementwise code.

@@ -33,9 +33,9 @@ TORCH_LIB = os.path.join(LIB_DIR, "libvlak_torch.so")
 CMP_LIB = os.path.join(LIB_DIR, "libvlak_comparators.so")
 
 CU_SOURCES = ["capi.cu", "softmax.cu", "attention_gqa.cu", "attention_simt.cu",
-              "rotary.cu"]
-HEADERS = ["vlak_device.cuh", "vlak_internal.h"]
-SHIM_SOURCES = ["torch_ops.cpp", "torch_rotary.cpp"]
+              "attention_bwd.cu", "rotary.cu"]
+HEADERS = ["vlak_device.cuh", "vlak_internal.h", "attention_common.cuh"]
+SHIM_SOURCES = ["torch_ops.cpp", "torch_rotary.cpp", "torch_attention_train.cpp"]
 SHIM_HEADERS = ["vlak_torch.h"]
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]

@@ -59,6 +59,14 @@ int current_device_info(DeviceInfo* out) {
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return set_cuda_error("cudaGetDevice", e);
   if (dev < 0 || dev >= kMaxDev) return set_error(VLAK_ERR_CUDA, "device ordinal out of range");
+  // A thread that has made no runtime call on its device yet (an autograd
+  // worker) has no current context, which encoding a tensor map needs.
+  thread_local int bound = -1;
+  if (bound != dev) {
+    e = cudaSetDevice(dev);
+    if (e != cudaSuccess) return set_cuda_error("cudaSetDevice", e);
+    bound = dev;
+  }
   int status = VLAK_OK;
   std::call_once(once[dev], [&] {
     DeviceInfo d;

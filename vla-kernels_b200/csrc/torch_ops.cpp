@@ -22,37 +22,7 @@
 #include "vlak_b200.h"
 #include "vlak_torch.h"
 
-namespace {
-
-using vlak_torch::check_status;
-using vlak_torch::dtype_code;
-using vlak_torch::raise_pending_device_error;
-
-// vlak::device_error(): the synchronous check. Waits for the device, then
-// reads and clears the error words; returns the status found (0 = none).
-int64_t device_error() {
-  int code = VLAK_OK;
-  c10::cuda::device_synchronize();
-  check_status(vlak_device_error_read(&code), "vlak::device_error");
-  return code;
-}
-
-// kernels/softmax/softmax_kernels.cu:255-297
-at::Tensor softmax_lastdim(const at::Tensor& x_in, int64_t version) {
-  raise_pending_device_error("vlak::softmax");
-  TORCH_CHECK(x_in.is_cuda(), "input must be CUDA");
-  TORCH_CHECK(x_in.dim() == 2, "expected a 2D [rows, cols] tensor");
-  const int dt = dtype_code(x_in.scalar_type());
-  TORCH_CHECK(dt >= 0, "softmax_lastdim: unsupported dtype ", x_in.scalar_type());
-  c10::cuda::CUDAGuard guard(x_in.device());
-  at::Tensor x = x_in.contiguous();
-  at::Tensor y = at::empty_like(x, at::MemoryFormat::Contiguous);
-  const int st = vlak_softmax_fwd(x.data_ptr(), y.data_ptr(), x.size(0), x.size(1), dt,
-                                  static_cast<int>(version),
-                                  c10::cuda::getCurrentCUDAStream().stream());
-  check_status(st, "softmax kernel launch failed");
-  return y;
-}
+namespace vlak_torch {
 
 vlak_attn_gqa_args gqa_args(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
                             double scale, int64_t prefix_len, int64_t dead_start,
@@ -100,8 +70,47 @@ at::Tensor split_workspace(const vlak_attn_gqa_args& a, const at::Tensor& like) 
   if (bytes == 0) return at::Tensor();
   return at::empty({bytes}, like.options().dtype(at::kByte));
 }
+// workspace pointer and bytes as the C ABI wants them
 void* ws_ptr(const at::Tensor& ws) { return ws.defined() ? ws.data_ptr() : nullptr; }
 int64_t ws_bytes(const at::Tensor& ws) { return ws.defined() ? ws.numel() : 0; }
+
+}  // namespace vlak_torch
+
+namespace {
+
+using vlak_torch::check_status;
+using vlak_torch::dtype_code;
+using vlak_torch::gqa_args;
+using vlak_torch::raise_pending_device_error;
+using vlak_torch::split_workspace;
+using vlak_torch::ws_bytes;
+using vlak_torch::ws_ptr;
+
+// vlak::device_error(): the synchronous check. Waits for the device, then
+// reads and clears the error words; returns the status found (0 = none).
+int64_t device_error() {
+  int code = VLAK_OK;
+  c10::cuda::device_synchronize();
+  check_status(vlak_device_error_read(&code), "vlak::device_error");
+  return code;
+}
+
+// kernels/softmax/softmax_kernels.cu:255-297
+at::Tensor softmax_lastdim(const at::Tensor& x_in, int64_t version) {
+  raise_pending_device_error("vlak::softmax");
+  TORCH_CHECK(x_in.is_cuda(), "input must be CUDA");
+  TORCH_CHECK(x_in.dim() == 2, "expected a 2D [rows, cols] tensor");
+  const int dt = dtype_code(x_in.scalar_type());
+  TORCH_CHECK(dt >= 0, "softmax_lastdim: unsupported dtype ", x_in.scalar_type());
+  c10::cuda::CUDAGuard guard(x_in.device());
+  at::Tensor x = x_in.contiguous();
+  at::Tensor y = at::empty_like(x, at::MemoryFormat::Contiguous);
+  const int st = vlak_softmax_fwd(x.data_ptr(), y.data_ptr(), x.size(0), x.size(1), dt,
+                                  static_cast<int>(version),
+                                  c10::cuda::getCurrentCUDAStream().stream());
+  check_status(st, "softmax kernel launch failed");
+  return y;
+}
 
 at::Tensor run_gqa(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, double scale,
                    int64_t prefix_len, int64_t dead_start, int64_t dead_end, bool v4) {

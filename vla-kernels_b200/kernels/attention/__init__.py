@@ -7,6 +7,7 @@ implementations and register guards, so ``vla/variants.py`` routes to them
 unchanged and each call traces as one node under ``torch.compile``. One
 additive op has no counterpart there: ``fused_attention_gqa_varlen``
 (per-sample lengths, the prefix-attention site the reference leaves on SDPA).
+``fused_attention_gqa_train`` is the same attention with gradients.
 
 The bf16 ops run one tcgen05 kernel (vla-kernels_b200/csrc/attention_gqa.cu):
 QK^T and PV on the 5th-generation tensor cores with accumulators in tensor
@@ -49,8 +50,30 @@ def _ext_v4():
     return torch.ops.vlak
 
 
+@lru_cache(maxsize=1)
+def _ext_train():
+    _native.load_ops()
+
+    def o_like(q):
+        return torch.empty(q.shape, dtype=q.dtype, device=q.device)
+
+    torch.library.register_fake("vlak::fused_attention_gqa_train")(
+        lambda q, k, v, scale=-1.0, prefix_len=-1, dead_start=0, dead_end=0, lengths=None,
+        attn_mask=None: o_like(q))
+    torch.library.register_fake("vlak::fused_attention_gqa_fwd_lse")(
+        lambda q, k, v, scale=-1.0, prefix_len=-1, dead_start=0, dead_end=0, lengths=None,
+        attn_mask=None:
+            (o_like(q), torch.empty(q.shape[:3], dtype=torch.float32, device=q.device)))
+    torch.library.register_fake("vlak::fused_attention_gqa_bwd")(
+        lambda grad_o, q, k, v, o, lse, scale=-1.0, prefix_len=-1, dead_start=0, dead_end=0,
+        lengths=None, attn_mask=None, with_kv=True:
+            [o_like(t) for t in ((q, k, v) if with_kv else (q,))])
+    return torch.ops.vlak
+
+
 _registered = False
 _registered_v4 = False
+_registered_train = False
 
 
 def _ensure_registered():
@@ -65,6 +88,13 @@ def _ensure_registered_v4():
     if not _registered_v4:
         _ext_v4()
         _registered_v4 = True
+
+
+def _ensure_registered_train():
+    global _registered_train
+    if not _registered_train:
+        _ext_train()
+        _registered_train = True
 
 
 def fused_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
@@ -133,6 +163,38 @@ def fused_attention_gqa_v4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     return torch.ops.vlak.fused_attention_gqa_v4(
         q, k, v, -1.0 if scale is None else scale,
         -1 if prefix_len is None else prefix_len, dead_start, dead_end)
+
+
+def fused_attention_gqa_train(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                              scale: float | None = None,
+                              prefix_len: int | None = None,
+                              dead_start: int = 0,
+                              dead_end: int = 0,
+                              lengths: torch.Tensor | None = None,
+                              attn_mask: torch.Tensor | None = None) -> torch.Tensor:
+    """``fused_attention_gqa`` with gradients of q, k and v.
+
+    Shapes, layouts and the analytic mask are those of ``fused_attention_gqa``;
+    instead of it, ``lengths`` masks as in ``fused_attention_gqa_varlen`` or
+    ``attn_mask`` (B, M, N) bool, True to attend, over all heads. Head h's
+    gradient goes to kv head h // (H // H_kv), summed over its query heads.
+
+    The backward pass (vla-kernels_b200/csrc/attention_bwd.cu) recomputes the
+    probabilities; between the passes only q, k, v, the output and one float
+    per row are kept. Sums are 32-bit in a fixed order, so gradients repeat bit
+    for bit. A row that sees no key is zeros and has a zero gradient. Values
+    that no row may see (a dead band, positions past a sample's length) may be
+    anything, NaN included; behind ``attn_mask`` all values must be finite.
+    Differentiable once.
+
+    To capture a training step into a CUDA graph, let no eager autograd graph
+    of the same leaves live meanwhile (drop its loss and outputs first):
+    autograd would order the capture behind that graph's stream.
+    """
+    _ensure_registered_train()
+    return torch.ops.vlak.fused_attention_gqa_train(
+        q, k, v, -1.0 if scale is None else scale,
+        -1 if prefix_len is None else prefix_len, dead_start, dead_end, lengths, attn_mask)
 
 
 def device_error() -> int:
