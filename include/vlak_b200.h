@@ -306,7 +306,9 @@ VLAK_API int vlak_attn_gqa_bwd(const vlak_attn_train_args* args, void* workspace
  *                     sign, magnitudes up to 2^53
  *   inv_freq        : rotary_dim / 2 doubles, radians per position
  *   inverse         : turn the other way (the gradient of vlak_rotary)
- * D even, 2 to 1024; rotary_dim even, 2 to D. B == 0 or M == 0 is a no-op
+ * D even, 2 to 1024; rotary_dim even, 2 to D; at most 2^31 - 1 tokens. Rows
+ * whose strides, pointers and (rotated) widths keep 16-byte vectors whole run
+ * faster; any others are taken as they are. B == 0 or M == 0 is a no-op
  * (backward: zero weight gradients).
  *
  * vlak_qk_norm_rotary_bwd takes x (the forward's input) and grad (of its

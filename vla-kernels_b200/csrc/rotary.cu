@@ -59,6 +59,9 @@ struct RotParams {
   long long pos_sb, pos_sm;
   int pos_i64, M, D, half, interleaved, w_f32;
   float amp, sign, eps;
+  // 16-byte path: log2 of the lanes per head and of the heads side by side
+  int lg_units, lg_heads[2];
+  int blocks[2];       // blocks of each tensor
 };
 
 __device__ __forceinline__ double position_of(const RotParams& p, long long b, long long m) {
@@ -74,6 +77,11 @@ __device__ __forceinline__ float2 turn_of(const RotParams& p, double pos, double
   float s, c;
   sincospif(2.f * static_cast<float>(frac), &s, &c);
   return make_float2(p.amp * c, p.amp * p.sign * s);
+}
+
+// the pair turned; one that is not rotated passes through (whatever its mate)
+__device__ __forceinline__ float2 turned(float a, float b, float2 cs, bool rotated) {
+  return rotated ? make_float2(a * cs.x - b * cs.y, b * cs.x + a * cs.y) : make_float2(a, b);
 }
 
 template <typename T>
@@ -98,9 +106,9 @@ __global__ void __launch_bounds__(32 * kLaneWarps) rotary_lane(const RotParams p
 #pragma unroll
   for (int i = 0; i < K; ++i) {
     const int q = lane + 32 * i;
-    const bool turned = q < p.half, there = q < pairs;
-    ia[i] = !there ? -1 : turned && !p.interleaved ? q : 2 * q;
-    ib[i] = turned && !p.interleaved ? q + p.half : 2 * q + 1;
+    const bool there = q < pairs, halves = q < p.half && !p.interleaved;
+    ia[i] = !there ? -1 : halves ? q : 2 * q;
+    ib[i] = halves ? q + p.half : 2 * q + 1;
     wa[i] = wb[i] = dwa[i] = dwb[i] = 0.f;
     if (kMode != kRotate && there) {
       wa[i] = weight_at<T>(p, t.w, ia[i]);
@@ -138,7 +146,8 @@ __global__ void __launch_bounds__(32 * kLaneWarps) rotary_lane(const RotParams p
         for (int i = 0; i < K; ++i) {
           const float ga = ia[i] >= 0 ? Elem<T>::to_f(g[ia[i]]) : 0.f;
           const float gb = ia[i] >= 0 ? Elem<T>::to_f(g[ib[i]]) : 0.f;
-          const float ta = ga * cs[i].x - gb * cs[i].y, tb = gb * cs[i].x + ga * cs[i].y;
+          const float2 t = turned(ga, gb, cs[i], lane + 32 * i < p.half);
+          const float ta = t.x, tb = t.y;
           xa[i] *= r;
           xb[i] *= r;
           dwa[i] += ta * xa[i];
@@ -160,8 +169,9 @@ __global__ void __launch_bounds__(32 * kLaneWarps) rotary_lane(const RotParams p
           if (ia[i] >= 0) {
             const float ua = kMode == kNormFwd ? xa[i] * r * wa[i] : xa[i];
             const float ub = kMode == kNormFwd ? xb[i] * r * wb[i] : xb[i];
-            y[ia[i]] = Elem<T>::from_f(ua * cs[i].x - ub * cs[i].y);
-            y[ib[i]] = Elem<T>::from_f(ub * cs[i].x + ua * cs[i].y);
+            const float2 t = turned(ua, ub, cs[i], lane + 32 * i < p.half);
+            y[ia[i]] = Elem<T>::from_f(t.x);
+            y[ib[i]] = Elem<T>::from_f(t.y);
           }
       }
     }
@@ -184,8 +194,188 @@ __global__ void __launch_bounds__(32 * kLaneWarps) rotary_lane(const RotParams p
   }
 }
 
-// dw[d] = sum over the partial rows, in a fixed order: thread row y of a block
-// adds rows y, y + 8, ..., then the eight sums are added. blockIdx.y: tensor.
+// ---------------------------------------------------------------------------
+// 16-byte path: a thread holds a unit of two vectors of V entries, the two
+// halves of V pairs (half layout), or 2V neighbouring entries (interleaved, and
+// past rd). A head is D / 2V units on the next power of two of lanes, so a norm
+// is a few shuffles. The 256 threads of a block take `TB` tokens x `HS` heads
+// at a time and walk the remaining heads of those tokens, so the angles, which
+// the block first computes into shared memory, one sincospi per (token, pair),
+// serve every head from registers. Weight-gradient sums stay in registers over
+// all the rows a thread visits.
+constexpr int kVecThreads = 256;
+
+template <typename T, int kMode>
+__global__ void __launch_bounds__(kVecThreads, kMode == kNormBwd ? 2 : 3)
+    rotary_vec(const RotParams p) {
+  constexpr int V = Elem<T>::kVec;
+  constexpr int kRows = kMode == kRotate ? 2 : 1;   // heads in flight per thread
+  constexpr int kVecs = kMode == kNormBwd ? 4 : 2;  // vectors per head: x, and the gradient
+  // two tables in turn, so one barrier per step is enough: TB * half entries,
+  // at most (256 / units) * (units * V)
+  __shared__ __align__(16) float2 table[2][kVecThreads * V];
+  const int z = static_cast<int>(blockIdx.x) >= p.blocks[0] ? 1 : 0;
+  const RotTensor& t = p.t[z];
+  const int blk = blockIdx.x - (z ? p.blocks[0] : 0);
+  const int u = threadIdx.x & ((1 << p.lg_units) - 1), slot = threadIdx.x >> p.lg_units;
+  const int HS = 1 << p.lg_heads[z], h0 = slot & (HS - 1), tl = slot >> p.lg_heads[z];
+  const int TB = (kVecThreads >> p.lg_units) >> p.lg_heads[z];
+  const int turned_units = p.half / V;
+  const bool there = u < p.D / (2 * V), rot = u < turned_units;
+  const int e0 = rot ? (p.interleaved ? 2 * u * V : u * V) : 2 * u * V;
+  const int e1 = rot && !p.interleaved ? e0 + p.half : e0 + V;
+  const unsigned tokens = static_cast<unsigned>(p.tokens), M = p.M;
+
+  float w[2 * V], dw[2 * V];
+  if (kMode != kRotate) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      w[i] = there ? weight_at<T>(p, t.w, e0 + i) : 0.f;
+      w[V + i] = there ? weight_at<T>(p, t.w, e1 + i) : 0.f;
+      dw[i] = dw[V + i] = 0.f;
+    }
+  }
+  int buf = 0;
+  for (unsigned tok0 = blk * TB; tok0 < tokens; tok0 += p.blocks[z] * TB, buf ^= 1) {
+    const unsigned tok = tok0 + tl;
+    const bool here = there && tok < tokens;
+    const long long b = tok / M, m = tok - tok / M * M;
+    const T* x = static_cast<const T*>(t.x) + b * t.x_sb + m * t.x_sm;
+    const T* g = static_cast<const T*>(t.g) + b * t.g_sb + m * t.g_sm;
+    T* y = static_cast<T*>(t.y) + static_cast<long long>(tok) * t.H * p.D;
+    uint4 raw[kRows][kVecs];
+    auto load = [&](int h) {
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) {
+        const int hr = h + r * HS;
+        if (here && hr < t.H) {
+          raw[r][0] = ld_stream16(x + hr * t.x_sh + e0);
+          raw[r][1] = ld_stream16(x + hr * t.x_sh + e1);
+          if (kMode == kNormBwd) {
+            raw[r][kVecs - 2] = ld_stream16(g + hr * t.g_sh + e0);
+            raw[r][kVecs - 1] = ld_stream16(g + hr * t.g_sh + e1);
+          }
+        } else {
+#pragma unroll
+          for (int v = 0; v < kVecs; ++v) raw[r][v] = make_uint4(0, 0, 0, 0);
+        }
+      }
+    };
+    load(h0);  // in flight while the angles are computed
+    for (int e = threadIdx.x; e < TB * p.half; e += kVecThreads) {
+      const int tt = e / p.half, i = e - tt * p.half;
+      const unsigned at = tok0 + tt;
+      if (at < tokens)
+        table[buf][e] = turn_of(p, position_of(p, at / M, at - at / M * M), p.freq[i]);
+    }
+    __syncthreads();
+    float2 cs[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      cs[i] = rot && here ? table[buf][tl * p.half + u * V + i] : make_float2(1.f, 0.f);
+    // turn the unit's pairs (f[0..V) and f[V..2V) are its two vectors)
+    auto turn = [&](float (&f)[2 * V]) {
+      if (!rot) return;
+      if (p.interleaved) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const float2 r = turned(f[2 * i], f[2 * i + 1], cs[i], true);
+          f[2 * i] = r.x;
+          f[2 * i + 1] = r.y;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const float2 r = turned(f[i], f[V + i], cs[i], true);
+          f[i] = r.x;
+          f[V + i] = r.y;
+        }
+      }
+    };
+    // the sum over the lanes of a head
+    auto head_sum = [&](float v) {
+      for (int o = (1 << p.lg_units) >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(kFullMask, v, o);
+      return v;
+    };
+    // every lane of a warp makes the same trips (shuffles): up to the block's
+    // first head slot
+    for (int h = h0; h - h0 < t.H; h += kRows * HS) {
+      float f[kRows][2 * V], gr[kMode == kNormBwd ? 2 * V : 1];
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) {
+        Elem<T>::unpack(raw[r][0], f[r]);
+        Elem<T>::unpack(raw[r][1], f[r] + V);
+      }
+      if constexpr (kMode == kNormBwd) {
+        Elem<T>::unpack(raw[0][2], gr);
+        Elem<T>::unpack(raw[0][3], gr + V);
+      }
+      if (h - h0 + kRows * HS < t.H) load(h + kRows * HS);
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) {
+        const int hr = h + r * HS;
+        float inv = 1.f;
+        if (kMode != kRotate) {
+          float ss = 0.f;
+#pragma unroll
+          for (int i = 0; i < 2 * V; ++i) ss += f[r][i] * f[r][i];
+          inv = rsqrtf(head_sum(ss) / p.D + p.eps);
+        }
+        if constexpr (kMode == kNormBwd) {
+          turn(gr);
+          float dot = 0.f;
+          const bool row = here && hr < t.H;
+#pragma unroll
+          for (int i = 0; i < 2 * V; ++i) {
+            f[r][i] *= inv;
+            dw[i] += row ? gr[i] * f[r][i] : 0.f;
+            gr[i] *= w[i];
+            dot += gr[i] * f[r][i];
+          }
+          dot = head_sum(dot) / p.D;
+#pragma unroll
+          for (int i = 0; i < 2 * V; ++i) f[r][i] = inv * (gr[i] - f[r][i] * dot);
+        } else {
+          if (kMode == kNormFwd) {
+#pragma unroll
+            for (int i = 0; i < 2 * V; ++i) f[r][i] *= inv * w[i];
+          }
+          turn(f[r]);
+        }
+        if (here && hr < t.H) {
+          st_stream16(y + hr * p.D + e0, Elem<T>::pack(f[r]));
+          st_stream16(y + hr * p.D + e1, Elem<T>::pack(f[r] + V));
+        }
+      }
+    }
+  }
+  if constexpr (kMode == kNormBwd) {
+    // lanes of one unit within the warp, then the warps
+#pragma unroll
+    for (int i = 0; i < 2 * V; ++i)
+      for (int o = 16; o >= (1 << p.lg_units); o >>= 1) dw[i] += __shfl_xor_sync(kFullMask, dw[i], o);
+    float* part = reinterpret_cast<float*>(table);  // [warp][D]
+    __syncthreads();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (lane < (1 << p.lg_units) && there) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        part[warp * p.D + e0 + i] = dw[i];
+        part[warp * p.D + e1 + i] = dw[V + i];
+      }
+    }
+    __syncthreads();
+    for (int d = threadIdx.x; d < p.D; d += kVecThreads) {
+      float sum = 0.f;
+#pragma unroll
+      for (int k = 0; k < kVecThreads / 32; ++k) sum += part[k * p.D + d];
+      t.dw_part[static_cast<long long>(blk) * p.D + d] = sum;
+    }
+  }
+}
+
+// dw[d] = sum over the partial rows, in a fixed order: warp y of a block adds
+// rows y, y + 32, ..., then the 32 sums are added. blockIdx.y: tensor.
 struct DwParams {
   const float* part[2];
   void* dw[2];
@@ -193,36 +383,89 @@ struct DwParams {
   int D, w_f32;
 };
 template <typename T>
-__global__ void __launch_bounds__(256) reduce_dw(const DwParams p) {
-  __shared__ float acc[8][33];
+__global__ void __launch_bounds__(1024) reduce_dw(const DwParams p) {
+  __shared__ float acc[32][33];
   const int z = blockIdx.y, col = threadIdx.x & 31, row0 = threadIdx.x >> 5;
   const int d = blockIdx.x * 32 + col;
   float s = 0.f;
   if (d < p.D) {
 #pragma unroll 8
-    for (int r = row0; r < p.rows[z]; r += 8) s += p.part[z][static_cast<long long>(r) * p.D + d];
+    for (int r = row0; r < p.rows[z]; r += 32) s += p.part[z][static_cast<long long>(r) * p.D + d];
   }
   acc[row0][col] = s;
   __syncthreads();
-  if (row0 != 0 || d >= p.D) return;
-#pragma unroll
-  for (int r = 1; r < 8; ++r) s += acc[r][col];
+  s = warp_sum(acc[col][row0]);  // warp y now adds column y
+  const int dd = blockIdx.x * 32 + row0;
+  if (col != 0 || dd >= p.D) return;
   if (p.w_f32)
-    static_cast<float*>(p.dw[z])[d] = s;
+    static_cast<float*>(p.dw[z])[dd] = s;
   else
-    static_cast<T*>(p.dw[z])[d] = Elem<T>::from_f(s);
+    static_cast<T*>(p.dw[z])[dd] = Elem<T>::from_f(s);
 }
 
 // ---------------------------------------------------------------------------
 constexpr int kMaxHeadDim = 1024;
 
+// Grid of a launch: blocks[i] blocks for tensor i, and the 16-byte path's
+// shape if the layout allows it.
 struct Launch {
-  int blocks;  // grid.x
+  bool vec;
+  int lg_units, lg_heads[2], blocks[2];
 };
-// Blocks of a launch: one per token, at most sixteen per SM (the rest loop).
-Launch plan(const vlak_rotary_args* a, int sm_count) {
+int lg_ceil(int64_t n) {
+  int lg = 0;
+  while ((int64_t{1} << lg) < n) ++lg;
+  return lg;
+}
+// The 16-byte path wants whole units (two vectors) in the rotated part and in
+// the rest, a head on at most one warp, and vectors on 16-byte boundaries.
+bool vectors_fit(const vlak_rotary_args* a, int mode) {
+  const int V = a->dtype == VLAK_F32 ? 4 : 8;
+  if (a->D % (2 * V) != 0 || a->rotary_dim % (2 * V) != 0 || a->D > 64 * V) return false;
+  auto fits = [&](const void* ptr, const int64_t* stride) {
+    return reinterpret_cast<uintptr_t>(ptr) % 16 == 0 && stride[0] % V == 0 && stride[1] % V == 0 &&
+           stride[2] % V == 0;
+  };
+  for (int i = 0; i < a->n_tensors; ++i) {
+    const vlak_rotary_tensor& t = a->t[i];
+    if (!fits(t.x, t.x_stride) || reinterpret_cast<uintptr_t>(t.y) % 16 != 0) return false;
+    if (mode == kNormBwd && !fits(t.grad, t.grad_stride)) return false;
+  }
+  return true;
+}
+// Lane path: one block per token, at most sixteen per SM (the rest loop).
+int64_t lane_blocks(const vlak_rotary_args* a, int sm_count) {
+  return std::min<int64_t>(a->B * a->M, 16ll * sm_count);
+}
+Launch plan(const vlak_rotary_args* a, int mode, int sm_count) {
   const int64_t tokens = a->B * a->M;
-  return Launch{static_cast<int>(std::min<int64_t>(tokens, 16ll * sm_count))};
+  Launch l{};
+  l.vec = vectors_fit(a, mode);
+  if (!l.vec) {
+    for (int i = 0; i < a->n_tensors; ++i)
+      l.blocks[i] = static_cast<int>(lane_blocks(a, sm_count));
+    return l;
+  }
+  l.lg_units = lg_ceil(a->D / (a->dtype == VLAK_F32 ? 8 : 16));
+  const int lg_slots = 8 - l.lg_units;
+  int64_t heads = 0;
+  for (int i = 0; i < a->n_tensors; ++i) heads += a->t[i].H;
+  for (int i = 0; i < a->n_tensors; ++i) {
+    // four or more heads one after the other on a thread, to spread the angles'
+    // and the block's fixed work, but side by side when that leaves SMs idle
+    int lg = 0;
+    while (a->t[i].H >> (lg + 3) != 0) ++lg;
+    lg = std::min(lg, lg_slots);
+    auto tiles = [&](int lg_h) { return (tokens + (1 << (lg_slots - lg_h)) - 1) >> (lg_slots - lg_h); };
+    while (lg < lg_slots && (int64_t{1} << lg) < a->t[i].H && tiles(lg) < 2 * sm_count) ++lg;
+    l.lg_heads[i] = lg;
+    // the weights' gradient writes one partial row per block: fewer blocks,
+    // shared out by the tensors' heads
+    const int64_t most = mode == kNormBwd ? std::max<int64_t>(1, 4ll * sm_count * a->t[i].H / heads)
+                                          : 64ll * sm_count;
+    l.blocks[i] = static_cast<int>(std::min(tiles(lg), most));
+  }
+  return l;
 }
 
 int validate(const vlak_rotary_args* a, int mode, const char* op) {
@@ -247,6 +490,8 @@ int validate(const vlak_rotary_args* a, int mode, const char* op) {
     if (a->weight_dtype != VLAK_F32 && a->weight_dtype != a->dtype)
       return set_errorf(VLAK_ERR_UNSUPPORTED_DTYPE, "%s: weights must be fp32 or of the heads' dtype", op);
   }
+  if (a->B * a->M > INT32_MAX)
+    return set_errorf(VLAK_ERR_INVALID_ARGUMENT, "%s: at most 2^31 - 1 tokens", op);
   for (int i = 0; i < a->n_tensors; ++i)
     if (a->t[i].H <= 0 || a->t[i].H > INT32_MAX)
       return set_errorf(VLAK_ERR_INVALID_ARGUMENT, "%s: heads must be positive", op);
@@ -269,14 +514,18 @@ int validate(const vlak_rotary_args* a, int mode, const char* op) {
   return VLAK_OK;
 }
 
+// Partial weight gradients: what the lane path's grid writes, which is never
+// less than the 16-byte path's (so alignment does not enter).
 int64_t workspace_bytes(const vlak_rotary_args* a, int sm_count) {
-  return static_cast<int64_t>(a->n_tensors) * plan(a, sm_count).blocks * a->D * 4;
+  return a->n_tensors * lane_blocks(a, sm_count) * a->D * 4;
 }
 
 template <typename T, int kMode>
-cudaError_t launch(const RotParams& p, const Launch& l, int n, cudaStream_t cs) {
-  const dim3 grid(l.blocks, n);
-  if (p.D <= 64)
+cudaError_t launch(const RotParams& p, bool vec, int n, cudaStream_t cs) {
+  const dim3 grid(p.blocks[0], n);  // lane path: as many blocks for each tensor
+  if (vec)
+    rotary_vec<T, kMode><<<p.blocks[0] + p.blocks[1], kVecThreads, 0, cs>>>(p);
+  else if (p.D <= 64)
     rotary_lane<T, 1, kMode><<<grid, 32 * kLaneWarps, 0, cs>>>(p);
   else if (p.D <= 128)
     rotary_lane<T, 2, kMode><<<grid, 32 * kLaneWarps, 0, cs>>>(p);
@@ -311,7 +560,7 @@ int run(const vlak_rotary_args* a, void* workspace, int64_t ws_bytes, void* stre
   if (dev.cc_major != 10)
     return set_errorf(VLAK_ERR_UNSUPPORTED_DEVICE, "%s: needs an sm_100 device (found sm_%d%d)", op,
                       dev.cc_major, dev.cc_minor);
-  const Launch l = plan(a, dev.sm_count);
+  const Launch l = plan(a, kMode, dev.sm_count);
   RotParams p{};
   for (int i = 0; i < a->n_tensors; ++i) {
     const vlak_rotary_tensor& t = a->t[i];
@@ -320,7 +569,9 @@ int run(const vlak_rotary_args* a, void* workspace, int64_t ws_bytes, void* stre
                        t.grad_stride[0], t.grad_stride[1], t.grad_stride[2],
                        static_cast<int>(t.H)};
     if (kMode == kNormBwd)
-      p.t[i].dw_part = static_cast<float*>(workspace) + static_cast<int64_t>(i) * l.blocks * a->D;
+      p.t[i].dw_part = static_cast<float*>(workspace) + (i ? static_cast<int64_t>(l.blocks[0]) * a->D : 0);
+    p.lg_heads[i] = l.lg_heads[i];
+    p.blocks[i] = l.blocks[i];
   }
   if (kMode == kNormBwd) {
     if (!workspace || ws_bytes < workspace_bytes(a, dev.sm_count))
@@ -328,6 +579,7 @@ int run(const vlak_rotary_args* a, void* workspace, int64_t ws_bytes, void* stre
     if (reinterpret_cast<uintptr_t>(workspace) % 16 != 0)
       return set_errorf(VLAK_ERR_ALIGNMENT, "%s: workspace must be 16-byte aligned", op);
   }
+  p.lg_units = l.lg_units;
   p.pos = a->positions;
   p.pos_i64 = a->pos_dtype == VLAK_I64;
   p.pos_sb = a->pos_stride[0];
@@ -343,24 +595,24 @@ int run(const vlak_rotary_args* a, void* workspace, int64_t ws_bytes, void* stre
   p.sign = (kMode == kNormBwd) != (a->inverse != 0) ? -1.f : 1.f;
   p.eps = static_cast<float>(a->eps);
   p.w_f32 = a->weight_dtype == VLAK_F32;
-  cudaError_t e = a->dtype == VLAK_F32   ? launch<float, kMode>(p, l, a->n_tensors, cs)
-                  : a->dtype == VLAK_F16 ? launch<__half, kMode>(p, l, a->n_tensors, cs)
-                                         : launch<__nv_bfloat16, kMode>(p, l, a->n_tensors, cs);
+  cudaError_t e = a->dtype == VLAK_F32   ? launch<float, kMode>(p, l.vec, a->n_tensors, cs)
+                  : a->dtype == VLAK_F16 ? launch<__half, kMode>(p, l.vec, a->n_tensors, cs)
+                                         : launch<__nv_bfloat16, kMode>(p, l.vec, a->n_tensors, cs);
   if (e != cudaSuccess) return set_cuda_error(op, e);
   if (kMode == kNormBwd) {
     DwParams d{};
     for (int i = 0; i < a->n_tensors; ++i) {
       d.part[i] = p.t[i].dw_part;
       d.dw[i] = a->t[i].grad_weight;
-      d.rows[i] = l.blocks;
+      d.rows[i] = l.blocks[i];
     }
     d.D = p.D;
     d.w_f32 = p.w_f32;
     const dim3 grid((p.D + 31) / 32, a->n_tensors);
     if (a->dtype == VLAK_F16)
-      reduce_dw<__half><<<grid, 256, 0, cs>>>(d);
+      reduce_dw<__half><<<grid, 1024, 0, cs>>>(d);
     else
-      reduce_dw<__nv_bfloat16><<<grid, 256, 0, cs>>>(d);  // fp32 weights: the type is not used
+      reduce_dw<__nv_bfloat16><<<grid, 1024, 0, cs>>>(d);  // fp32 weights: the type is not used
     e = cudaGetLastError();
     if (e != cudaSuccess) return set_cuda_error(op, e);
   }
