@@ -293,7 +293,8 @@ VLAK_API int vlak_attn_gqa_bwd(const vlak_attn_train_args* args, void* workspace
  *   y_a = A (u_a cos t - u_b sin t), y_b = A (u_b cos t + u_a sin t);
  * the other entries pass through. u = x (vlak_rotary), or
  * u = x * rsqrt(mean(x^2) + eps) * weight (vlak_qk_norm_rotary_fwd).
- * Angles are taken in 64 bits, all other math in 32; one rounding per output.
+ * Angles are taken modulo whole turns in 64 bits, all other math in 32; one
+ * rounding per output.
  *
  *   t[0..n_tensors) : queries, and keys if there are any, of one token grid
  *                     (B, M); heads H and strides of each its own
@@ -302,8 +303,7 @@ VLAK_API int vlak_attn_gqa_bwd(const vlak_attn_train_args* args, void* workspace
  *   y               : contiguous (B, M, H, D); must not overlap x or grad
  *   dtype           : VLAK_F32 / VLAK_F16 / VLAK_BF16 of x, grad and y
  *   weight          : (D), weight_dtype VLAK_F32 or dtype
- *   positions       : VLAK_I32 / VLAK_I64, element strides for (b, m); any
- *                     sign, magnitudes up to 2^53
+ *   positions       : VLAK_I32 / VLAK_I64, element strides for (b, m); any sign
  *   inv_freq        : rotary_dim / 2 doubles, radians per position
  *   inverse         : turn the other way (the gradient of vlak_rotary)
  * D even, 2 to 1024; rotary_dim even, 2 to D; at most 2^31 - 1 tokens. Rows

@@ -12,10 +12,12 @@
 //   dw = sum over rows of g hat,  dx = r (g w - hat * mean(g w hat)).
 //
 // Angles. position * f_i reaches 10^5..10^9 radians in long contexts, where a
-// 32-bit product has lost the fraction of a turn. The product is taken in
-// turns (f_i / 2 pi) in 64 bits, its whole turns are removed there, and the
-// remaining fraction goes to sincospi in 32 bits. All else is 32-bit: norms,
-// dot products and the weight gradient's sums; outputs are rounded once.
+// 32-bit product has lost the fraction of a turn. Whole turns do not matter, so
+// f_i / 2 pi is held as a 64-bit binary fraction of a turn and the product with
+// the position wraps modulo 2^64, exactly: what is left, at 32 bits the
+// fraction of a turn to 2^-32, goes to sincospi in 32 bits. All else is 32-bit
+// too: norms, dot products and the weight gradient's sums; outputs are rounded
+// once.
 //
 // Bound: HBM. Each input is read once and each output written once; one angle
 // serves every head of its token.
@@ -51,6 +53,15 @@ struct RotTensor {
   int H;
 };
 
+// n / d for n < 2^31 by a multiplication: m = ceil(2^(32 + l) / d) - 2^32 with
+// l = ceil(log2 d); (n m >> 32) + n is below 2^32 for n < 2^31.
+struct FastDiv {
+  unsigned d, m, l;
+};
+__device__ __forceinline__ unsigned fast_div(unsigned n, const FastDiv& f) {
+  return (__umulhi(n, f.m) + n) >> f.l;
+}
+
 struct RotParams {
   RotTensor t[2];      // blockIdx.y selects
   const void* pos;
@@ -59,23 +70,36 @@ struct RotParams {
   long long pos_sb, pos_sm;
   int pos_i64, M, D, half, interleaved, w_f32;
   float amp, sign, eps;
-  // 16-byte path: log2 of the lanes per head and of the heads side by side
-  int lg_units, lg_heads[2];
-  int blocks[2];       // blocks of each tensor
+  // 16-byte path: log2 of the lanes per head, a block's tokens, the slots of
+  // each token that serve queries and keys, and the heads a slot takes in turn
+  int lg_units, block_tokens, q_slots, k_slots, trips;
+  FastDiv by_M;
 };
 
-__device__ __forceinline__ double position_of(const RotParams& p, long long b, long long m) {
+__device__ __forceinline__ unsigned long long position_of(const RotParams& p, long long b, long long m) {
   const long long i = b * p.pos_sb + m * p.pos_sm;
-  return p.pos_i64 ? static_cast<double>(static_cast<const long long*>(p.pos)[i])
-                   : static_cast<double>(static_cast<const int*>(p.pos)[i]);
+  return p.pos_i64 ? static_cast<const long long*>(p.pos)[i] : static_cast<const int*>(p.pos)[i];
 }
 
-// (A cos t, +-A sin t) of t = pos * f
-__device__ __forceinline__ float2 turn_of(const RotParams& p, double pos, double f) {
-  const double turns = f * 0.15915494309189533577;  // f / (2 pi)
-  const double frac = fma(pos, turns, -rint(pos * turns));
+// f radians as a fraction of a turn, modulo whole turns, in units of 2^-64
+__device__ __forceinline__ unsigned long long turns_of(double f) {
+  const double turns = f * 0.15915494309189533577;  // f / 2 pi
+  return __double2ull_rd((turns - floor(turns)) * 0x1p63) << 1;
+}
+// (A cos t, +-A sin t) of the turn position * turns. For 16-bit heads the
+// hardware's sine and cosine: within 2^-21 of the value on half a turn to each
+// side, 2^-10 of half a step of fp16; sincospi, four times the instructions,
+// for 32-bit ones.
+template <typename T>
+__device__ __forceinline__ float2 turn_of(const RotParams& p, unsigned long long pos,
+                                          unsigned long long turns) {
+  const int part = static_cast<int>((pos * turns) >> 32);  // of a turn, in 2^-32, -1/2 to 1/2
   float s, c;
-  sincospif(2.f * static_cast<float>(frac), &s, &c);
+  if constexpr (sizeof(T) == 2) {
+    __sincosf(static_cast<float>(part) * 1.4629180792671596e-9f, &s, &c);  // 2 pi 2^-32
+  } else {
+    sincospif(static_cast<float>(part) * 0x1p-31f, &s, &c);
+  }
   return make_float2(p.amp * c, p.amp * p.sign * s);
 }
 
@@ -117,12 +141,12 @@ __global__ void __launch_bounds__(32 * kLaneWarps) rotary_lane(const RotParams p
   }
   for (long long tok = blockIdx.x; tok < p.tokens; tok += gridDim.x) {
     const long long b = tok / p.M, m = tok - b * p.M;
-    const double pos = position_of(p, b, m);
+    const unsigned long long pos = position_of(p, b, m);
     float2 cs[K];
 #pragma unroll
     for (int i = 0; i < K; ++i) {
       const int q = lane + 32 * i;
-      cs[i] = q < p.half ? turn_of(p, pos, p.freq[q]) : make_float2(1.f, 0.f);
+      cs[i] = q < p.half ? turn_of<T>(p, pos, turns_of(p.freq[q])) : make_float2(1.f, 0.f);
     }
     for (int h = warp; h < t.H; h += kLaneWarps) {
       const T* x = static_cast<const T*>(t.x) + b * t.x_sb + m * t.x_sm + h * t.x_sh;
@@ -197,179 +221,282 @@ __global__ void __launch_bounds__(32 * kLaneWarps) rotary_lane(const RotParams p
 // ---------------------------------------------------------------------------
 // 16-byte path: a thread holds a unit of two vectors of V entries, the two
 // halves of V pairs (half layout), or 2V neighbouring entries (interleaved, and
-// past rd). A head is D / 2V units on the next power of two of lanes, so a norm
-// is a few shuffles. The 256 threads of a block take `TB` tokens x `HS` heads
-// at a time and walk the remaining heads of those tokens, so the angles, which
-// the block first computes into shared memory, one sincospi per (token, pair),
-// serve every head from registers. Weight-gradient sums stay in registers over
-// all the rows a thread visits.
-constexpr int kVecThreads = 256;
+// past rd). A head is D / 2V units on the next power of two of lanes, a slot,
+// so a norm is a few shuffles. A block takes TB tokens at a time with HS slots
+// each; some of the HS serve queries and the others keys, in turn over their
+// heads, so a thread stays with one tensor and its weight-gradient sums stay in
+// registers. The block first computes the tokens' angles into shared memory,
+// once for all heads of queries and keys.
+constexpr int kVecThreads = 128;
 
-template <typename T, int kMode>
-__global__ void __launch_bounds__(kVecThreads, kMode == kNormBwd ? 2 : 3)
-    rotary_vec(const RotParams p) {
+// Arithmetic is on pairs of fp32 (f32x2), which halves its issue slots; the
+// forward norm folds its weights into the angles' factors once per token:
+//   y_a = r (x_a c w_a - x_b s w_b),  y_b = r (x_b c w_b + x_a s w_a).
+// A unit's 2V entries are held as V entries a and their V mates b; the
+// interleaved layout is taken apart while unpacking, which costs nothing, so
+// both layouts share all arithmetic.
+template <typename T, bool kInter>
+__device__ __forceinline__ void unpack_unit(const uint4& v0, const uint4& v1, uint64_t* f) {
   constexpr int V = Elem<T>::kVec;
-  constexpr int kRows = kMode == kRotate ? 2 : 1;   // heads in flight per thread
-  constexpr int kVecs = kMode == kNormBwd ? 4 : 2;  // vectors per head: x, and the gradient
-  // two tables in turn, so one barrier per step is enough: TB * half entries,
-  // at most (256 / units) * (units * V)
-  __shared__ __align__(16) float2 table[2][kVecThreads * V];
-  const int z = static_cast<int>(blockIdx.x) >= p.blocks[0] ? 1 : 0;
-  const RotTensor& t = p.t[z];
-  const int blk = blockIdx.x - (z ? p.blocks[0] : 0);
-  const int u = threadIdx.x & ((1 << p.lg_units) - 1), slot = threadIdx.x >> p.lg_units;
-  const int HS = 1 << p.lg_heads[z], h0 = slot & (HS - 1), tl = slot >> p.lg_heads[z];
-  const int TB = (kVecThreads >> p.lg_units) >> p.lg_heads[z];
-  const int turned_units = p.half / V;
-  const bool there = u < p.D / (2 * V), rot = u < turned_units;
-  const int e0 = rot ? (p.interleaved ? 2 * u * V : u * V) : 2 * u * V;
-  const int e1 = rot && !p.interleaved ? e0 + p.half : e0 + V;
-  const unsigned tokens = static_cast<unsigned>(p.tokens), M = p.M;
-
-  float w[2 * V], dw[2 * V];
-  if (kMode != kRotate) {
+  float t[2 * V];
+  Elem<T>::unpack(v0, t);
+  Elem<T>::unpack(v1, t + V);
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      w[i] = there ? weight_at<T>(p, t.w, e0 + i) : 0.f;
-      w[V + i] = there ? weight_at<T>(p, t.w, e1 + i) : 0.f;
-      dw[i] = dw[V + i] = 0.f;
+  for (int i = 0; i < V / 2; ++i) {
+    f[i] = kInter ? f2_pack(t[4 * i], t[4 * i + 2]) : f2_pack(t[2 * i], t[2 * i + 1]);
+    f[V / 2 + i] = kInter ? f2_pack(t[4 * i + 1], t[4 * i + 3]) : f2_pack(t[V + 2 * i], t[V + 2 * i + 1]);
+  }
+}
+template <typename T, bool kInter>
+__device__ __forceinline__ void pack_unit(const uint64_t* f, uint4& v0, uint4& v1) {
+  constexpr int V = Elem<T>::kVec;
+  float t[2 * V];
+#pragma unroll
+  for (int i = 0; i < V / 2; ++i) {
+    if (kInter) {
+      f2_unpack(f[i], t[4 * i], t[4 * i + 2]);
+      f2_unpack(f[V / 2 + i], t[4 * i + 1], t[4 * i + 3]);
+    } else {
+      f2_unpack(f[i], t[2 * i], t[2 * i + 1]);
+      f2_unpack(f[V / 2 + i], t[V + 2 * i], t[V + 2 * i + 1]);
     }
   }
+  v0 = Elem<T>::pack(t);
+  v1 = Elem<T>::pack(t + V);
+}
+
+template <typename T, int kMode, bool kInter>
+__global__ void __launch_bounds__(kVecThreads, kMode == kRotate ? 6 : kMode == kNormFwd ? 5 : 4)
+    rotary_vec(const RotParams p) {
+  constexpr int V = Elem<T>::kVec;
+  // two tables in turn, so one barrier per step is enough: TB * half entries,
+  // at most slots * (units * V). Tables lie as [chunk of 16 bytes][unit], so that
+  // a warp's units read neighbouring 16 bytes.
+  __shared__ __align__(16) float2 table[2][kVecThreads * V];
+  __shared__ __align__(16) float w_smem[2][kMode != kRotate ? 64 * V : 4];  // [chunk][32 units][4]
+  const int u = threadIdx.x & ((1 << p.lg_units) - 1), slot = threadIdx.x >> p.lg_units;
+  const int HS = p.q_slots + p.k_slots, TB = p.block_tokens;
+  const int tl = slot / HS, hs = slot - tl * HS;  // token and place of the slot
+  const bool z = hs >= p.q_slots;                 // a key slot
+  const RotTensor& t = z ? p.t[1] : p.t[0];
+  const int H = t.H, h0 = z ? hs - p.q_slots : hs, h_step = z ? p.k_slots : p.q_slots;
+  const unsigned stride = gridDim.x * TB;
+  const int units = p.D / (2 * V), turned_units = max(1, p.half / V);
+  const bool there = u < units, rot = u < p.half / V;
+  // the unit's vectors start at entries e0 and e0 + apart (a spare lane reads
+  // unit 0's)
+  const int e0 = !there ? 0 : rot && !kInter ? u * V : 2 * u * V;
+  const int apart = rot && !kInter ? p.half : V;
+  auto entry = [&](int i) {  // of the i-th a (i < V) or b
+    return kInter ? e0 + 2 * (i % V) + i / V : e0 + i % V + (i < V ? 0 : apart);
+  };
+  const unsigned tokens = static_cast<unsigned>(p.tokens);
+  const float inv_D = 1.f / p.D;
+  const long long x_step = h_step * t.x_sh, g_step = h_step * t.g_sh;
+  const int y_step = h_step * p.D;
+  // A thread fills table entries (token, pair) 256 apart; the pair stays the
+  // same, and its frequency in a register, when it can.
+  const int step_tok = kVecThreads / p.half, step_pair = kVecThreads - step_tok * p.half;
+  const int fill_tok = threadIdx.x / p.half, fill_pair = threadIdx.x - fill_tok * p.half;
+  unsigned long long fill_turns = 0;
+
+  uint64_t dw[kMode == kNormBwd ? V : 1];
+  if (kMode == kNormBwd) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) dw[i] = 0ull;
+  }
+  // the 2i-th and (2i + 1)-th pairs of the unit's weights
+  auto w_pairs = [&](int i, uint64_t& a, uint64_t& c) {
+    const float4 w = *reinterpret_cast<const float4*>(&w_smem[z][(i * 32 + u) * 4]);
+    a = f2_pack(w.x, w.y);
+    c = f2_pack(w.z, w.w);
+  };
+  bool first = true;
   int buf = 0;
-  for (unsigned tok0 = blk * TB; tok0 < tokens; tok0 += p.blocks[z] * TB, buf ^= 1) {
-    const unsigned tok = tok0 + tl;
-    const bool here = there && tok < tokens;
-    const long long b = tok / M, m = tok - tok / M * M;
-    const T* x = static_cast<const T*>(t.x) + b * t.x_sb + m * t.x_sm;
-    const T* g = static_cast<const T*>(t.g) + b * t.g_sb + m * t.g_sm;
-    T* y = static_cast<T*>(t.y) + static_cast<long long>(tok) * t.H * p.D;
-    uint4 raw[kRows][kVecs];
-    auto load = [&](int h) {
-#pragma unroll
-      for (int r = 0; r < kRows; ++r) {
-        const int hr = h + r * HS;
-        if (here && hr < t.H) {
-          raw[r][0] = ld_stream16(x + hr * t.x_sh + e0);
-          raw[r][1] = ld_stream16(x + hr * t.x_sh + e1);
-          if (kMode == kNormBwd) {
-            raw[r][kVecs - 2] = ld_stream16(g + hr * t.g_sh + e0);
-            raw[r][kVecs - 1] = ld_stream16(g + hr * t.g_sh + e1);
-          }
-        } else {
-#pragma unroll
-          for (int v = 0; v < kVecs; ++v) raw[r][v] = make_uint4(0, 0, 0, 0);
-        }
+  for (unsigned tok0 = blockIdx.x * TB; tok0 < tokens; tok0 += stride, buf ^= 1) {
+    const bool here = there && tl < TB && tok0 + tl < tokens;
+    // a thread without a token reads the block's first (its results go nowhere)
+    const unsigned tok = tl < TB && tok0 + tl < tokens ? tok0 + tl : tok0, tb = fast_div(tok, p.by_M);
+    const long long b = tb, m = tok - tb * p.by_M.d;
+    const T* x = static_cast<const T*>(t.x) + b * t.x_sb + m * t.x_sm + h0 * t.x_sh + e0;
+    const T* g = static_cast<const T*>(t.g) + b * t.g_sb + m * t.g_sm + h0 * t.g_sh + e0;
+    T* y = static_cast<T*>(t.y) + (static_cast<long long>(tok) * H + h0) * p.D + e0;
+    uint4 raw[4];
+    auto load = [&]() {
+      raw[0] = ld_stream16(x);
+      raw[1] = ld_stream16(x + apart);
+      if (kMode == kNormBwd) {
+        raw[2] = ld_stream16(g);
+        raw[3] = ld_stream16(g + apart);
       }
     };
-    load(h0);  // in flight while the angles are computed
-    for (int e = threadIdx.x; e < TB * p.half; e += kVecThreads) {
-      const int tt = e / p.half, i = e - tt * p.half;
+    load();  // in flight while the angles are computed
+    if (first) {
+      first = false;
+      fill_turns = turns_of(p.freq[fill_pair]);
+      if (kMode != kRotate) {
+        for (int e = threadIdx.x; e < p.D; e += kVecThreads) {
+          // entry e as the i-th a or b of its unit
+          const bool halves = !kInter && e < 2 * p.half;
+          const int c = halves ? e % p.half : e;
+          const int eu = halves ? c / V : e / (2 * V), r = halves ? c % V : e % (2 * V);
+          const int i = halves ? r + (e < p.half ? 0 : V) : kInter ? r / 2 + r % 2 * V : r;
+          const int at = ((i / 4) * 32 + eu) * 4 + i % 4;
+          w_smem[0][at] = weight_at<T>(p, p.t[0].w, e);
+          if (p.k_slots) w_smem[1][at] = weight_at<T>(p, p.t[1].w, e);
+        }
+      }
+    }
+    for (int tt = fill_tok, i = fill_pair; tt < TB;) {
       const unsigned at = tok0 + tt;
-      if (at < tokens)
-        table[buf][e] = turn_of(p, position_of(p, at / M, at - at / M * M), p.freq[i]);
+      if (at < tokens) {
+        const unsigned ab = fast_div(at, p.by_M);
+        const unsigned long long turns = step_pair == 0 ? fill_turns : turns_of(p.freq[i]);
+        table[buf][((tt * (V / 2) + i % V / 2) * turned_units + i / V) * 2 + i % 2] =
+            turn_of<T>(p, position_of(p, ab, at - ab * p.by_M.d), turns);
+      }
+      tt += step_tok;
+      i += step_pair;
+      if (i >= p.half) {
+        i -= p.half;
+        ++tt;
+      }
     }
     __syncthreads();
-    float2 cs[V];
+    // Factors: y_a = Ca a + Sa b, y_b = Cb b + Sb a, in pairs; Ca and Cb are
+    // one unless weights are folded in.
+    constexpr int kC = kMode == kNormFwd ? V : V / 2;
+    uint64_t C[kC], S[V];
 #pragma unroll
-    for (int i = 0; i < V; ++i)
-      cs[i] = rot && here ? table[buf][tl * p.half + u * V + i] : make_float2(1.f, 0.f);
-    // turn the unit's pairs (f[0..V) and f[V..2V) are its two vectors)
-    auto turn = [&](float (&f)[2 * V]) {
-      if (!rot) return;
-      if (p.interleaved) {
+    for (int i = 0; i < V / 2; ++i) {
+      float4 cs = make_float4(1.f, 0.f, 1.f, 0.f);
+      if (rot && here)
+        cs = *reinterpret_cast<const float4*>(&table[buf][((tl * (V / 2) + i) * turned_units + u) * 2]);
+      C[i] = f2_pack(cs.x, cs.z);
+      S[i] = f2_pack(-cs.y, -cs.w);
+      S[V / 2 + i] = f2_pack(cs.y, cs.w);
+    }
+    if constexpr (kMode == kNormFwd) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const float2 r = turned(f[2 * i], f[2 * i + 1], cs[i], true);
-          f[2 * i] = r.x;
-          f[2 * i + 1] = r.y;
+      for (int i = 0; i < V / 4; ++i) {
+        uint64_t wa[2], wb[2];
+        w_pairs(i, wa[0], wa[1]);
+        w_pairs(V / 4 + i, wb[0], wb[1]);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int k = 2 * i + j;
+          C[V / 2 + k] = f2_mul(C[k], wb[j]);
+          C[k] = f2_mul(C[k], wa[j]);
+          S[k] = f2_mul(S[k], wb[j]);
+          S[V / 2 + k] = f2_mul(S[V / 2 + k], wa[j]);
         }
-      } else {
+      }
+    }
+    auto turn = [&](uint64_t (&f)[V]) {
+      if (!rot) {  // passes through, whatever its neighbour
+        if constexpr (kMode == kNormFwd) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const float2 r = turned(f[i], f[V + i], cs[i], true);
-          f[i] = r.x;
-          f[V + i] = r.y;
+          for (int i = 0; i < V; ++i) f[i] = f2_mul(f[i], C[i]);
         }
+        return;
+      }
+#pragma unroll
+      for (int i = 0; i < V / 2; ++i) {
+        const uint64_t a = f[i], c = f[V / 2 + i];
+        f[i] = f2_fma(c, S[i], f2_mul(a, C[i]));
+        f[V / 2 + i] = f2_fma(a, S[V / 2 + i], f2_mul(c, C[(V / 2 + i) % kC]));
       }
     };
     // the sum over the lanes of a head
-    auto head_sum = [&](float v) {
-      for (int o = (1 << p.lg_units) >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(kFullMask, v, o);
+    auto head_sum = [&](uint64_t v2) {
+      float lo, hi;
+      f2_unpack(v2, lo, hi);
+      float v = lo + hi;
+#pragma unroll
+      for (int k = 0; k < 5; ++k)
+        if (k < p.lg_units) v += __shfl_xor_sync(kFullMask, v, 1 << k);
       return v;
     };
-    // every lane of a warp makes the same trips (shuffles): up to the block's
-    // first head slot
-    for (int h = h0; h - h0 < t.H; h += kRows * HS) {
-      float f[kRows][2 * V], gr[kMode == kNormBwd ? 2 * V : 1];
-#pragma unroll
-      for (int r = 0; r < kRows; ++r) {
-        Elem<T>::unpack(raw[r][0], f[r]);
-        Elem<T>::unpack(raw[r][1], f[r] + V);
+    // every lane makes the same trips (shuffles)
+    for (int k = 0, h = h0; k < p.trips; ++k, h += h_step) {
+      const bool row = here && h < H;
+      uint64_t f[V], gr[kMode == kNormBwd ? V : 1];
+      unpack_unit<T, kInter>(raw[0], raw[1], f);
+      if constexpr (kMode == kNormBwd) unpack_unit<T, kInter>(raw[2], raw[3], gr);
+      if (h + h_step < H) {  // else the same row again, for nothing
+        x += x_step;
+        if (kMode == kNormBwd) g += g_step;
       }
+      load();
       if constexpr (kMode == kNormBwd) {
-        Elem<T>::unpack(raw[0][2], gr);
-        Elem<T>::unpack(raw[0][3], gr + V);
+        // with u = w R^T g, both sums in one round of shuffles:
+        //   dx = r (u - x r^2 sum(u x) / D),  dw += (R^T g) (x r)
+        turn(gr);
+        uint64_t ss[2] = {0ull, 0ull}, ux[2] = {0ull, 0ull}, un[V];
+#pragma unroll
+        for (int i = 0; i < V; i += 2) {
+          uint64_t wa, wb;
+          w_pairs(i / 2, wa, wb);
+          un[i] = f2_mul(gr[i], wa);
+          un[i + 1] = f2_mul(gr[i + 1], wb);
+          ss[0] = f2_fma(f[i], f[i], ss[0]);
+          ss[1] = f2_fma(f[i + 1], f[i + 1], ss[1]);
+          ux[0] = f2_fma(un[i], f[i], ux[0]);
+          ux[1] = f2_fma(un[i + 1], f[i + 1], ux[1]);
+        }
+        if (!there) ss[0] = ss[1] = ux[0] = ux[1] = 0ull;
+        const float sum_xx = head_sum(f2_add(ss[0], ss[1])), sum_ux = head_sum(f2_add(ux[0], ux[1]));
+        const float inv = rsqrtf(fmaf(sum_xx, inv_D, p.eps)), nd = -inv * inv * (sum_ux * inv_D);
+        const uint64_t inv2 = f2_pack(inv, inv), nd2 = f2_pack(nd, nd);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          if (row) dw[i] = f2_fma(f2_mul(gr[i], inv2), f[i], dw[i]);
+          f[i] = f2_mul(f2_fma(f[i], nd2, un[i]), inv2);
+        }
+      } else {
+        if constexpr (kMode == kNormFwd) {
+          uint64_t ss[2] = {0ull, 0ull};
+#pragma unroll
+          for (int i = 0; i < V; ++i) ss[i & 1] = f2_fma(f[i], f[i], ss[i & 1]);
+          if (!there) ss[0] = ss[1] = 0ull;
+          const float inv = rsqrtf(fmaf(head_sum(f2_add(ss[0], ss[1])), inv_D, p.eps));
+          const uint64_t inv2 = f2_pack(inv, inv);
+#pragma unroll
+          for (int i = 0; i < V; ++i) f[i] = f2_mul(f[i], inv2);
+        }
+        turn(f);
       }
-      if (h - h0 + kRows * HS < t.H) load(h + kRows * HS);
-#pragma unroll
-      for (int r = 0; r < kRows; ++r) {
-        const int hr = h + r * HS;
-        float inv = 1.f;
-        if (kMode != kRotate) {
-          float ss = 0.f;
-#pragma unroll
-          for (int i = 0; i < 2 * V; ++i) ss += f[r][i] * f[r][i];
-          inv = rsqrtf(head_sum(ss) / p.D + p.eps);
-        }
-        if constexpr (kMode == kNormBwd) {
-          turn(gr);
-          float dot = 0.f;
-          const bool row = here && hr < t.H;
-#pragma unroll
-          for (int i = 0; i < 2 * V; ++i) {
-            f[r][i] *= inv;
-            dw[i] += row ? gr[i] * f[r][i] : 0.f;
-            gr[i] *= w[i];
-            dot += gr[i] * f[r][i];
-          }
-          dot = head_sum(dot) / p.D;
-#pragma unroll
-          for (int i = 0; i < 2 * V; ++i) f[r][i] = inv * (gr[i] - f[r][i] * dot);
-        } else {
-          if (kMode == kNormFwd) {
-#pragma unroll
-            for (int i = 0; i < 2 * V; ++i) f[r][i] *= inv * w[i];
-          }
-          turn(f[r]);
-        }
-        if (here && hr < t.H) {
-          st_stream16(y + hr * p.D + e0, Elem<T>::pack(f[r]));
-          st_stream16(y + hr * p.D + e1, Elem<T>::pack(f[r] + V));
-        }
+      if (row) {
+        uint4 v0, v1;
+        pack_unit<T, kInter>(f, v0, v1);
+        st_stream16(y, v0);
+        st_stream16(y + apart, v1);
       }
+      y += y_step;
     }
   }
   if constexpr (kMode == kNormBwd) {
-    // lanes of one unit within the warp, then the warps
-#pragma unroll
-    for (int i = 0; i < 2 * V; ++i)
-      for (int o = 16; o >= (1 << p.lg_units); o >>= 1) dw[i] += __shfl_xor_sync(kFullMask, dw[i], o);
-    float* part = reinterpret_cast<float*>(table);  // [warp][D]
+    // one sum per tensor over the slots, in their order
+    float* part = reinterpret_cast<float*>(table);  // [slot][D]
     __syncthreads();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if (lane < (1 << p.lg_units) && there) {
+    if (there) {
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        part[warp * p.D + e0 + i] = dw[i];
-        part[warp * p.D + e1 + i] = dw[V + i];
+        float lo, hi;
+        f2_unpack(dw[i], lo, hi);
+        part[slot * p.D + entry(2 * i)] = lo;
+        part[slot * p.D + entry(2 * i + 1)] = hi;
       }
     }
     __syncthreads();
-    for (int d = threadIdx.x; d < p.D; d += kVecThreads) {
+    for (int e = threadIdx.x; e < 2 * p.D; e += kVecThreads) {
+      const int zz = e >= p.D, d = e - zz * p.D;
+      if (zz && p.k_slots == 0) break;
       float sum = 0.f;
-#pragma unroll
-      for (int k = 0; k < kVecThreads / 32; ++k) sum += part[k * p.D + d];
-      t.dw_part[static_cast<long long>(blk) * p.D + d] = sum;
+      for (int tt = 0; tt < TB; ++tt)
+        for (int q = zz ? p.q_slots : 0; q < (zz ? HS : p.q_slots); ++q)
+          sum += part[(tt * HS + q) * p.D + d];
+      p.t[zz].dw_part[static_cast<long long>(blockIdx.x) * p.D + d] = sum;
     }
   }
 }
@@ -406,16 +533,20 @@ __global__ void __launch_bounds__(1024) reduce_dw(const DwParams p) {
 // ---------------------------------------------------------------------------
 constexpr int kMaxHeadDim = 1024;
 
-// Grid of a launch: blocks[i] blocks for tensor i, and the 16-byte path's
-// shape if the layout allows it.
+// Grid of a launch, and the 16-byte path's shape if the layout allows it.
 struct Launch {
   bool vec;
-  int lg_units, lg_heads[2], blocks[2];
+  int blocks, lg_units, block_tokens, q_slots, k_slots, trips;
 };
 int lg_ceil(int64_t n) {
   int lg = 0;
   while ((int64_t{1} << lg) < n) ++lg;
   return lg;
+}
+FastDiv fast_div_by(unsigned d) {
+  const unsigned l = static_cast<unsigned>(lg_ceil(d));
+  const uint64_t m = (((uint64_t{1} << l) - d) << 32) / d + 1;
+  return FastDiv{d, static_cast<unsigned>(m), l};
 }
 // The 16-byte path wants whole units (two vectors) in the rotated part and in
 // the rest, a head on at most one warp, and vectors on 16-byte boundaries.
@@ -442,29 +573,38 @@ Launch plan(const vlak_rotary_args* a, int mode, int sm_count) {
   Launch l{};
   l.vec = vectors_fit(a, mode);
   if (!l.vec) {
-    for (int i = 0; i < a->n_tensors; ++i)
-      l.blocks[i] = static_cast<int>(lane_blocks(a, sm_count));
+    l.blocks = static_cast<int>(lane_blocks(a, sm_count));
     return l;
   }
   l.lg_units = lg_ceil(a->D / (a->dtype == VLAK_F32 ? 8 : 16));
-  const int lg_slots = 8 - l.lg_units;
-  int64_t heads = 0;
-  for (int i = 0; i < a->n_tensors; ++i) heads += a->t[i].H;
-  for (int i = 0; i < a->n_tensors; ++i) {
-    // four or more heads one after the other on a thread, to spread the angles'
-    // and the block's fixed work, but side by side when that leaves SMs idle
-    int lg = 0;
-    while (a->t[i].H >> (lg + 3) != 0) ++lg;
-    lg = std::min(lg, lg_slots);
-    auto tiles = [&](int lg_h) { return (tokens + (1 << (lg_slots - lg_h)) - 1) >> (lg_slots - lg_h); };
-    while (lg < lg_slots && (int64_t{1} << lg) < a->t[i].H && tiles(lg) < 2 * sm_count) ++lg;
-    l.lg_heads[i] = lg;
-    // the weights' gradient writes one partial row per block: fewer blocks,
-    // shared out by the tensors' heads
-    const int64_t most = mode == kNormBwd ? std::max<int64_t>(1, 4ll * sm_count * a->t[i].H / heads)
-                                          : 64ll * sm_count;
-    l.blocks[i] = static_cast<int>(std::min(tiles(lg), most));
+  const int64_t slots = kVecThreads >> l.lg_units, Hq = a->t[0].H;
+  const int64_t Hk = a->n_tensors > 1 ? a->t[1].H : 0;
+  // Trips over the heads: a slot's cost per token is its trips plus about one
+  // trip's worth of fixed work, times the slots a token takes (unused ones
+  // included); the cheapest, but with more slots side by side while the tokens
+  // leave SMs without a block.
+  double best = 0;
+  for (int64_t trips = 1; trips <= std::max(Hq, Hk); ++trips) {
+    const int64_t q = (Hq + trips - 1) / trips, k = (Hk + trips - 1) / trips;
+    const int64_t tokens_here = slots / (q + k);
+    if (tokens_here == 0) continue;
+    const double cost = static_cast<double>(trips + 1) * slots / tokens_here;
+    const bool spread = (tokens + tokens_here - 1) / tokens_here >= 2 * sm_count;
+    if (best == 0 || (spread && cost < best)) {
+      best = cost;
+      l.block_tokens = static_cast<int>(tokens_here);
+      l.q_slots = static_cast<int>(q);
+      l.k_slots = static_cast<int>(k);
+      l.trips = static_cast<int>(trips);
+    }
+    if (!spread || trips >= 16) break;
   }
+  // Blocks: a tile each for the rotation, whose blocks start cheaply; the norm's
+  // lay out weights first, and the backward pass writes a partial weight
+  // gradient per block, so these loop (over resident blocks, twice as many
+  // forward: 37.4 -> 36.2 us for 8191 tokens of 40 heads of 128)
+  const int64_t tiles = (tokens + l.block_tokens - 1) / l.block_tokens;
+  l.blocks = static_cast<int>(std::min<int64_t>(tiles, (mode == kRotate ? 64ll : mode == kNormFwd ? 10ll : 4ll) * sm_count));
   return l;
 }
 
@@ -521,10 +661,11 @@ int64_t workspace_bytes(const vlak_rotary_args* a, int sm_count) {
 }
 
 template <typename T, int kMode>
-cudaError_t launch(const RotParams& p, bool vec, int n, cudaStream_t cs) {
-  const dim3 grid(p.blocks[0], n);  // lane path: as many blocks for each tensor
+cudaError_t launch(const RotParams& p, bool vec, int blocks, int n, cudaStream_t cs) {
+  const dim3 grid(blocks, n);
   if (vec)
-    rotary_vec<T, kMode><<<p.blocks[0] + p.blocks[1], kVecThreads, 0, cs>>>(p);
+    p.interleaved ? rotary_vec<T, kMode, true><<<blocks, kVecThreads, 0, cs>>>(p)
+                  : rotary_vec<T, kMode, false><<<blocks, kVecThreads, 0, cs>>>(p);
   else if (p.D <= 64)
     rotary_lane<T, 1, kMode><<<grid, 32 * kLaneWarps, 0, cs>>>(p);
   else if (p.D <= 128)
@@ -569,9 +710,7 @@ int run(const vlak_rotary_args* a, void* workspace, int64_t ws_bytes, void* stre
                        t.grad_stride[0], t.grad_stride[1], t.grad_stride[2],
                        static_cast<int>(t.H)};
     if (kMode == kNormBwd)
-      p.t[i].dw_part = static_cast<float*>(workspace) + (i ? static_cast<int64_t>(l.blocks[0]) * a->D : 0);
-    p.lg_heads[i] = l.lg_heads[i];
-    p.blocks[i] = l.blocks[i];
+      p.t[i].dw_part = static_cast<float*>(workspace) + static_cast<int64_t>(i) * l.blocks * a->D;
   }
   if (kMode == kNormBwd) {
     if (!workspace || ws_bytes < workspace_bytes(a, dev.sm_count))
@@ -580,6 +719,10 @@ int run(const vlak_rotary_args* a, void* workspace, int64_t ws_bytes, void* stre
       return set_errorf(VLAK_ERR_ALIGNMENT, "%s: workspace must be 16-byte aligned", op);
   }
   p.lg_units = l.lg_units;
+  p.block_tokens = l.block_tokens;
+  p.q_slots = l.q_slots;
+  p.k_slots = l.k_slots;
+  p.trips = l.trips;
   p.pos = a->positions;
   p.pos_i64 = a->pos_dtype == VLAK_I64;
   p.pos_sb = a->pos_stride[0];
@@ -587,6 +730,7 @@ int run(const vlak_rotary_args* a, void* workspace, int64_t ws_bytes, void* stre
   p.freq = a->inv_freq;
   p.tokens = a->B * a->M;
   p.M = static_cast<int>(a->M);
+  p.by_M = fast_div_by(static_cast<unsigned>(a->M));
   p.D = static_cast<int>(a->D);
   p.half = static_cast<int>(a->rotary_dim / 2);
   p.interleaved = a->interleaved != 0;
@@ -595,16 +739,16 @@ int run(const vlak_rotary_args* a, void* workspace, int64_t ws_bytes, void* stre
   p.sign = (kMode == kNormBwd) != (a->inverse != 0) ? -1.f : 1.f;
   p.eps = static_cast<float>(a->eps);
   p.w_f32 = a->weight_dtype == VLAK_F32;
-  cudaError_t e = a->dtype == VLAK_F32   ? launch<float, kMode>(p, l.vec, a->n_tensors, cs)
-                  : a->dtype == VLAK_F16 ? launch<__half, kMode>(p, l.vec, a->n_tensors, cs)
-                                         : launch<__nv_bfloat16, kMode>(p, l.vec, a->n_tensors, cs);
+  cudaError_t e = a->dtype == VLAK_F32   ? launch<float, kMode>(p, l.vec, l.blocks, a->n_tensors, cs)
+                  : a->dtype == VLAK_F16 ? launch<__half, kMode>(p, l.vec, l.blocks, a->n_tensors, cs)
+                                         : launch<__nv_bfloat16, kMode>(p, l.vec, l.blocks, a->n_tensors, cs);
   if (e != cudaSuccess) return set_cuda_error(op, e);
   if (kMode == kNormBwd) {
     DwParams d{};
     for (int i = 0; i < a->n_tensors; ++i) {
       d.part[i] = p.t[i].dw_part;
       d.dw[i] = a->t[i].grad_weight;
-      d.rows[i] = l.blocks[i];
+      d.rows[i] = l.blocks;
     }
     d.D = p.D;
     d.w_f32 = p.w_f32;
