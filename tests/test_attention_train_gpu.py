@@ -139,6 +139,27 @@ def test_lengths(shape, dtype):
     check(got, orc.train(q, k, v, do, orc.by_length(M, N, L)))
 
 
+@pytest.mark.parametrize("shape", [(300, 150, 150, 3, 1), (260, 200, 200, 2, 2), (700, 60, 60, 3, 1),
+                                   (400, 1, 64, 4, 2), (500, 70, 1, 2, 1)])
+@pytest.mark.parametrize("most", [1.0, 0.3])
+def test_many_samples_of_all_lengths(shape, most):
+    # far more pieces of work than the GPU takes at once, many of them empty or
+    # of a single step, in any order
+    B, M, N, H, Hkv = shape
+    q, k, v, do = make(*shape, seed=B)
+    g = torch.Generator(device="cuda").manual_seed(N)
+    L = torch.randint(0, int(most * N) + 1, (B,), device="cuda", generator=g)
+    L[B // 3: B // 2] = 0
+    check(step(q, k, v, do, lengths=L), orc.train(q, k, v, do, orc.by_length(M, N, L)))
+
+
+@pytest.mark.parametrize("shape", [(200, 50, 291, 15, 5, 241, 196, 240), (300, 64, 64, 2, 1, 0, 0, 0),
+                                   (90, 200, 40, 3, 1, 0, 0, 0), (500, 3, 130, 2, 2, 130, 0, 128)])
+def test_many_samples(shape):
+    B, M, N, H, Hkv, P, ds, de = shape
+    run(*shape[:5], P, ds, de, seed=B)
+
+
 def random_mask(B, M, N, seed, share=0.6):
     g = torch.Generator(device="cuda").manual_seed(seed)
     m = torch.rand(B, M, N, device="cuda", generator=g) < share

@@ -7,23 +7,36 @@
 // dK and dV summed over the G query heads of a kv head. Scores are taken in
 // the exp2 domain: P = 2^(scale log2(e) s - lse), lse from the forward pass.
 //
-// Two kernels, no atomics, so results repeat bit for bit:
-//   dq   one CTA per 128 query rows: walks the keys, S = Q K^T, dP = dO V^T,
-//        dS in bf16 back to TMEM, dQ += dS K. It also computes D and leaves
-//        (-lse, -D) of its rows in the workspace for the second kernel.
-//   dkv  one CTA per 128 keys: walks the query rows of all G heads,
-//        S^T = K Q^T, dP^T = V dO^T, then dV += P^T dO and dK += dS^T Q with
-//        P^T and dS^T in TMEM. Keys lie along TMEM lanes, so nothing is ever
-//        transposed through shared memory.
-// The scores and dP are computed in both (7 products instead of 5): joining
-// dQ across key blocks would take atomics or a pass over partial sums.
+// A first small kernel (attn_bwd_stats) computes D and lays (-lse, -D) out by
+// sub-tiles. The second, persistent, one works through two kinds of items, in
+// no shared sums, so without atomics on results, which repeat bit for bit:
+//   dkv  128 keys of a kv head, stationary K and V; walks the query rows of all
+//        G heads: S^T = K Q^T, dP^T = V dO^T, then dV += P^T dO, dK += dS^T Q
+//        with P^T and dS^T as TMEM operands (keys along the lanes, so nothing is
+//        transposed through shared memory);
+//   dq   128 query rows, stationary Q and dO; walks the keys: S = Q K^T,
+//        dP = dO V^T, then dQ += dS K with dS as a TMEM operand.
+// Both are one loop: two stationary tiles A0, A1 (128 x 64), a stream of pairs
+// B0, B1 (64 x 64), T0 = A0 B0^T and T1 = A1 B1^T, elementwise X1 = dS (and
+// X0 = P), acc1 += X1 B0 (and acc0 += X0 B1). Scores and dP are computed in both
+// (7 products instead of 5): joining dQ across key blocks would take atomics or
+// a pass over partial sums.
+//
+// Pipeline. One CTA per SM with all 512 columns of TMEM: two accumulators and
+// three stages of (T0, T1), so the products of the next steps, also those of the
+// next item, are issued while the current one's elementwise part runs. Sixteen
+// compute warps in two groups take the steps in turn. Items come from a counter,
+// the long ones first.
+//
+// Bound: by the products' shared-memory reads and issue. A step (128 x 64) is
+// 8 SS products of about 49 cycles and 4 (dq) or 8 (dkv) TS products of about 43.
 //
 // Rounding: P and dS are rounded to bf16 as operands of the second products,
 // as the forward pass rounds P; all sums, D and the statistics are fp32.
 //
 // Query rows are handled in sub-tiles of up to 64 rows, Gb heads x MT
 // positions with Gb a divisor of G, one TMA box each. Two sub-tiles make the
-// 128 lanes of a dq CTA; one is the 64 columns of a dkv step.
+// 128 rows of a dq item; one is the 64 columns of a dkv step.
 //
 // Every mbarrier wait is bounded as in the forward kernel.
 
@@ -36,6 +49,7 @@
 #include <algorithm>
 #include <atomic>
 #include <cstring>
+#include <type_traits>
 
 #include "attention_common.cuh"
 #include "vlak_device.cuh"
@@ -46,35 +60,48 @@ namespace {
 
 constexpr int kMaskAnalytic = 0, kMaskLength = 1, kMaskBool = 2;
 
-constexpr int kSub = 64;                     // query rows of a sub-tile
+constexpr int kSub = 64;                     // rows of a streamed tile
 constexpr int kRowBytes = 128;               // 64 bf16
 constexpr int kSubBytes = kSub * kRowBytes;  // 8 KB
 constexpr int kChunk = 64;                   // keys of a dq step
-constexpr int kKeys = 128;                   // keys of a dkv CTA
-constexpr int kDqStages = 3;                 // K/V chunks in flight
-constexpr int kDkvStages = 4;                // query sub-tiles in flight
-constexpr int kStatBytes = 2 * kSub * 4;     // -lse and -D of a sub-tile
-constexpr int kThreads = 192;                // four compute warps, producer, MMA
-constexpr int kWarpProducer = 4, kWarpMma = 5;
-constexpr uint32_t kTmemCols = 256;
-constexpr int kBarrierBytes = 256;
+constexpr int kKeys = 128;                   // keys of a dkv item
+constexpr int kRing = 6;                     // streamed pairs in flight (even: see the compute warps)
+constexpr int kStages = 3;                   // (T0, T1) pairs in TMEM
+constexpr int kQueue = 4;                    // items handed out and not yet seen by every warp
+constexpr int kStatFloats = 2 * kSub;        // -lse and -D of a sub-tile
+constexpr int kStatBytes = kStatFloats * 4;
 
-constexpr int kDqSmem = 6 * kSubBytes + kDqStages * 2 * kSubBytes + kBarrierBytes + 1024;
-constexpr int kDkvSmem =
-    4 * kSubBytes + kDkvStages * (2 * kSubBytes + kStatBytes) + kBarrierBytes + 1024;
-static_assert(2 * (kDqSmem + 1024) <= 228 * 1024, "two dq CTAs share an SM");
-static_assert(2 * (kDkvSmem + 1024) <= 228 * 1024, "two dkv CTAs share an SM");
+// Compute warps: two groups of eight that take the steps in turn; of a group,
+// two warps per lane quarter of TMEM, each with half of a step's 64 columns.
+constexpr int kGroupWarps = 8;
+constexpr int kComputeWarps = 2 * kGroupWarps;
+// One warp issues the scores, another the accumulating products: one alone
+// took about 1.6K cycles per step for both, three times the products' own time.
+constexpr int kWarpProducer = kComputeWarps, kWarpScores = kComputeWarps + 1,
+              kWarpAccum = kComputeWarps + 2;
+constexpr int kThreads = 32 * (kComputeWarps + 3);
+
+// TMEM columns: accumulators, then the stages; X0 and X1 (bf16 pairs) overwrite
+// parts of T0 and T1
+constexpr uint32_t kTmemCols = 512;
+constexpr uint32_t kAcc0 = 0, kAcc1 = 64, kStage0 = 128, kStageCols = 128, kT1 = 64;
+static_assert(kStage0 + kStages * kStageCols <= kTmemCols, "TMEM");
 
 struct __align__(64) BwdParams {
-  CUtensorMap tm_q, tm_do, tm_o, tm_dq;      // dims (64, H, M, B), box (64, Gb, MT, 1)
+  CUtensorMap tm_q, tm_do, tm_dq;            // dims (64, H, M, B), box (64, Gb, MT, 1)
   CUtensorMap tm_k64, tm_v64;                // dims (64, Hkv, N, B), box (64, 1, 64, 1)
   CUtensorMap tm_k, tm_v, tm_dk, tm_dv;      // the same, box (64, 1, 128, 1)
   __nv_bfloat16 *dq, *dk, *dv;               // contiguous
+  const __nv_bfloat16 *o, *d_o;
+  long long o_s[3], do_s[3];                 // (b, m, h) element strides
   const float* lse;                          // (B, M, H), log2 units
   float* stats;                              // [B * Hkv][n_sub][-lse 64, -D 64]
+  unsigned* counter;                         // next item
   int B, M, N, H, Hkv, G;
   int Gb, MT;                                // heads and positions of a sub-tile
   int n_mt, n_sub, n_pair, n_kblk, n_chunks;
+  int n_bk, n_dkv, n_items;                  // B * Hkv; dkv items; all items
+  int bk_inner;                              // items run over (b, kv head) first
   int P, ds, de;
   float scale_log2, out_scale;
   int* host_err;
@@ -96,337 +123,177 @@ __device__ __forceinline__ uint32_t low_bits(int n) {
   return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : ((1u << n) - 1u);
 }
 
+// TMEM column of the k-th 16 of a step's 64 bf16 operands: each half of them is
+// packed over the first half of the 32 fp32 columns it was computed from, which
+// the warp that packs them has read.
+__device__ __forceinline__ uint32_t packed_col(int k) { return (k >> 1) * 32 + (k & 1) * 8; }
+
 // 1024-byte aligned start of the dynamic shared memory
 __device__ __forceinline__ uint8_t* aligned_smem(uint8_t* raw) {
   return raw + (((smem_u32(raw) + 1023u) & ~1023u) - smem_u32(raw));
 }
 
-// ---------------------------------------------------------------------------
-// dq kernel
-
-struct DqBarriers {
-  uint64_t q_full, k_full[kDqStages], k_empty[kDqStages], s_full, ds_full, out_full, staged[2], drain;
-  uint32_t tmem_base;
-  int abort_flag;
+// Row `row` of sub-tile st of a (b, kv head): position m, head h within the kv
+// head, and whether it exists.
+struct SubRow {
+  int m, g;
+  bool valid;
 };
-static_assert(sizeof(DqBarriers) <= kBarrierBytes, "barrier block");
+__device__ __forceinline__ SubRow sub_row(const BwdParams& p, int st, int row) {
+  const int hb = st / p.n_mt, mt = st - hb * p.n_mt;
+  const int local = row / p.Gb;
+  SubRow r;
+  r.m = mt * p.MT + local;
+  r.g = hb * p.Gb + row - local * p.Gb;
+  r.valid = st < p.n_sub && local < p.MT && r.m < p.M;
+  return r;
+}
 
-// TMEM columns of the dq kernel; dS (bf16 pairs) overwrites the first half of S
-constexpr uint32_t kDqS = 0, kDqP = 64, kDqO = 128;
-
-template <int kMode>
-__global__ void __launch_bounds__(kThreads, 2) attn_bwd_dq(const __grid_constant__ BwdParams p) {
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = aligned_smem(smem_raw);
-  uint8_t* q_smem = smem;                      // [2 sub-tiles][64 x 128 B]
-  uint8_t* do_smem = q_smem + 2 * kSubBytes;
-  uint8_t* o_smem = do_smem + 2 * kSubBytes;   // O, then the staged dQ
-  uint8_t* k_smem = o_smem + 2 * kSubBytes;    // [stage][64 x 128 B]
-  uint8_t* v_smem = k_smem + kDqStages * kSubBytes;
-  DqBarriers* bars = reinterpret_cast<DqBarriers*>(v_smem + kDqStages * kSubBytes);
-  volatile int* abort_flag = &bars->abort_flag;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-
-  // item: a pair of sub-tiles of one (b, kv head); later rows, which see more
-  // keys under a staircase, first
-  const int bk = blockIdx.x / p.n_pair;
-  const int pair = p.n_pair - 1 - (blockIdx.x - bk * p.n_pair);
+// ---------------------------------------------------------------------------
+// D = rowsum(dO * O) and -lse by sub-tile rows: eight threads per row, 16 bytes
+// each. Rows that do not exist or see no key get -lse = -inf (every P is 0) and
+// D = 0, whatever memory holds there. Bound: HBM, one read of O and dO.
+constexpr int kStatThreads = 512;
+__global__ void __launch_bounds__(kStatThreads) attn_bwd_stats(const __grid_constant__ BwdParams p) {
+  if (blockIdx.x == 0 && threadIdx.x == 0) *p.counter = 0u;
+  const int bk = blockIdx.x / p.n_sub, st = blockIdx.x - bk * p.n_sub;
   const int b = bk / p.Hkv, kvh = bk - b * p.Hkv;
-  const int s0 = 2 * pair, n_here = min(2, p.n_sub - s0);
-  const int L = kMode == kMaskLength ? length_of(p, b) : 0;
-
-  // first and last position of the pair's rows
-  const int mt0 = s0 % p.n_mt, mt1 = (s0 + n_here - 1) % p.n_mt;
-  const int m_lo = min(mt0, mt1) * p.MT;
-  const int m_hi = min(p.M, (max(mt0, mt1) + 1) * p.MT) - 1;
-
-  // live key chunks [0, a1) and [b0, b1), as in the forward kernel
-  int a1 = 0, b0 = 0, b1 = 0;
-  if (kMode == kMaskBool) {
-    a1 = p.n_chunks;
-  } else if (kMode == kMaskLength) {
-    a1 = m_lo < L ? (L + kChunk - 1) / kChunk : 0;
-  } else {
-    a1 = (p.ds + kChunk - 1) / kChunk;
-    if (p.de < p.N) {
-      const int e2 = max(p.P, min(p.N, p.N - p.M + m_hi + 1));
-      b0 = max(p.de / kChunk, a1);
-      b1 = (e2 + kChunk - 1) / kChunk;
+  const int row = threadIdx.x >> 3, v = threadIdx.x & 7;
+  const SubRow r = sub_row(p, st, row);
+  const int h = kvh * p.G + r.g;
+  float nl = -INFINITY, d = 0.f;
+  if (r.valid) {
+    const float lse = p.lse[(static_cast<long long>(b) * p.M + r.m) * p.H + h];
+    if (lse != -INFINITY) {
+      nl = -lse;
+      const uint4 x = *reinterpret_cast<const uint4*>(p.o + b * p.o_s[0] + r.m * p.o_s[1] +
+                                                      h * p.o_s[2] + v * 8);
+      const uint4 y = *reinterpret_cast<const uint4*>(p.d_o + b * p.do_s[0] + r.m * p.do_s[1] +
+                                                      h * p.do_s[2] + v * 8);
+      float fx[8], fy[8];
+      Elem<__nv_bfloat16>::unpack(x, fx);
+      Elem<__nv_bfloat16>::unpack(y, fy);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) d += fx[i] * fy[i];
     }
   }
-  const int n_live = a1 + max(0, b1 - b0);
-  auto chunk_at = [&](int j) { return j < a1 ? j : b0 + j - a1; };
-
-  if (threadIdx.x == 0) {
-    mbar_init(&bars->q_full, 1);
-    for (int i = 0; i < kDqStages; ++i) {
-      mbar_init(&bars->k_full[i], 1);
-      mbar_init(&bars->k_empty[i], 1);
-    }
-    mbar_init(&bars->s_full, 1);
-    mbar_init(&bars->ds_full, 4);
-    mbar_init(&bars->staged[0], 2);
-    mbar_init(&bars->staged[1], 2);
-    mbar_init(&bars->out_full, 1);
-    mbar_init(&bars->drain, 1);
-    bars->abort_flag = 0;
-    fence_mbar_init();
-  }
-  if (warp == kWarpMma) {
-    tmem_alloc(&bars->tmem_base, kTmemCols);
-    tmem_relinquish();
-  }
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = bars->tmem_base;
-
-  if (warp == kWarpProducer) {
-    // Loads: Q, dO and O of the pair, then the live K/V chunks through a ring.
-    int issued = 0;
-    if (n_live > 0) {
-      mbar_arrive_expect_tx_elect(&bars->q_full,
-                                  static_cast<uint32_t>(3 * n_here * p.Gb * p.MT * kRowBytes));
-      for (int i = 0; i < n_here; ++i) {
-        const int hb = (s0 + i) / p.n_mt, m0 = (s0 + i - hb * p.n_mt) * p.MT;
-        const int h = kvh * p.G + hb * p.Gb;
-        tma_load_4d_elect(q_smem + i * kSubBytes, &p.tm_q, &bars->q_full, 0, h, m0, b);
-        tma_load_4d_elect(do_smem + i * kSubBytes, &p.tm_do, &bars->q_full, 0, h, m0, b);
-        tma_load_4d_elect(o_smem + i * kSubBytes, &p.tm_o, &bars->q_full, 0, h, m0, b);
-      }
-    }
-    for (int j = 0; j < n_live; ++j) {
-      const int s = j % kDqStages;
-      if (!__all_sync(kFullMask, bounded_wait(&bars->k_empty[s], ((j / kDqStages) & 1) ^ 1, abort_flag))) {
-        break;
-      }
-      mbar_arrive_expect_tx_elect(&bars->k_full[s], 2 * kSubBytes);
-      tma_load_4d_elect(k_smem + s * kSubBytes, &p.tm_k64, &bars->k_full[s], 0, kvh, chunk_at(j) * kChunk, b);
-      tma_load_4d_elect(v_smem + s * kSubBytes, &p.tm_v64, &bars->k_full[s], 0, kvh, chunk_at(j) * kChunk, b);
-      issued = j + 1;
-    }
-    if (n_live > 0) {
-      // never leave the CTA with copies in flight (bounded, abort or not)
-      bounded_wait(&bars->q_full, 0, abort_flag, false);
-      for (int j = max(0, issued - kDqStages); j < issued; ++j)
-        bounded_wait(&bars->k_full[j % kDqStages], (j / kDqStages) & 1, abort_flag, false);
-    }
-    __syncwarp();
-  } else if (warp == kWarpMma) {
-    if (n_live > 0) {
-      const uint32_t id_kk = idesc_bf16_f32(128, 64, false), id_kn = idesc_bf16_f32(128, 64, true);
-      const uint32_t q0 = smem_u32(q_smem), do0 = smem_u32(do_smem);
-      auto issue_scores = [&](int j) {  // S = Q K^T, dP = dO V^T of chunk j
-        const int s = j % kDqStages;
-        if (!__all_sync(kFullMask, bounded_wait<1>(&bars->k_full[s], (j / kDqStages) & 1, abort_flag)))
-          return false;
-        if (kMode != kMaskBool) {  // K rows that no query sees feed dS K: 0 times NaN
-          const int c0 = chunk_at(j) * kChunk;
-          const int lo = kMode == kMaskLength ? L - c0 : p.ds - c0;
-          const int hi = kMode == kMaskLength ? kChunk : p.de - c0;
-          clear_rows(k_smem + s * kSubBytes, max(lo, 0), min(hi, kChunk));
-        }
-        tc_fence_after();
-        const uint32_t k0 = smem_u32(k_smem + s * kSubBytes), v0 = smem_u32(v_smem + s * kSubBytes);
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-          umma_ss_elect(tmem + kDqS, sdesc_sw128(q0 + 32 * k), sdesc_sw128(k0 + 32 * k), id_kk, k > 0);
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          umma_ss_elect(tmem + kDqP, sdesc_sw128(do0 + 32 * k), sdesc_sw128(v0 + 32 * k), id_kk, k > 0);
-        umma_commit_elect(&bars->s_full);
-        return true;
-      };
-      bool ok = __all_sync(kFullMask, bounded_wait(&bars->q_full, 0, abort_flag));
-      tc_fence_after();
-      ok = ok && issue_scores(0);
-      for (int j = 0; ok && j < n_live; ++j) {
-        if (!__all_sync(kFullMask, bounded_wait<1>(&bars->ds_full, j & 1, abort_flag))) break;
-        tc_fence_after();
-        const int s = j % kDqStages;
-        const uint32_t k0 = smem_u32(k_smem + s * kSubBytes);
-#pragma unroll
-        for (int k = 0; k < 4; ++k)  // dQ += dS K
-          umma_ts_elect(tmem + kDqO, tmem + kDqS + 8 * k, sdesc_sw128(k0 + 2048 * k), id_kn,
-                        (j > 0 || k > 0) ? 1u : 0u);
-        umma_commit_elect(&bars->k_empty[s]);
-        if (j + 1 < n_live) {
-          ok = issue_scores(j + 1);
-        } else {
-          umma_commit_elect(&bars->out_full);
-        }
-      }
-      // every issued MMA completes before TMEM is released
-      umma_commit_elect(&bars->drain);
-      bounded_wait(&bars->drain, 0, abort_flag, false);
-    }
-    __syncwarp();
-  } else {
-    // Compute warps: lane quarter w of TMEM, one query row per thread.
-    const int half = warp >> 1;  // sub-tile of the pair
-    const int st = s0 + half;
-    const int row64 = (warp & 1) * 32 + lane;
-    const int hb = st / p.n_mt, mt = st - hb * p.n_mt;
-    const int m_local = row64 / p.Gb, g = row64 - m_local * p.Gb;
-    const int m = mt * p.MT + m_local;
-    const bool valid = st < p.n_sub && m_local < p.MT && m < p.M;
-    const int h = kvh * p.G + hb * p.Gb + g;
-    const long long row = (static_cast<long long>(b) * p.M + m) * p.H + h;
-    const uint32_t tbase = tmem + (static_cast<uint32_t>(warp * 32) << 16);
-    // visible keys [0, rds) U [rde, e2)
-    const int rds = kMode == kMaskAnalytic ? p.ds : 0;
-    const int rde = kMode == kMaskAnalytic ? p.de : 0;
-    const int e2 = kMode == kMaskAnalytic ? max(p.P, min(p.N, p.N - p.M + m + 1))
-                   : kMode == kMaskLength ? (m < L ? L : 0) : 0;
-    const uint8_t* mrow = nullptr;
-    if (kMode == kMaskBool && valid)
-      mrow = p.mask + static_cast<long long>(b) * p.mask_sb + static_cast<long long>(m) * p.mask_sm;
-
-    bool ok = true;
-    float nl = -INFINITY, nD = 0.f;
-    if (n_live > 0) {
-      if (valid) {
-        const float lse = p.lse[row];
-        nl = lse == -INFINITY ? -INFINITY : -lse;  // a row without keys: every P is 0
-      }
-      ok = __all_sync(kFullMask, bounded_wait(&bars->q_full, 0, abort_flag));
-      if (ok && valid && nl != -INFINITY) {
-        const uint8_t* dor = do_smem + half * kSubBytes + row64 * kRowBytes;
-        const uint8_t* orow = o_smem + half * kSubBytes + row64 * kRowBytes;
-        float acc[2] = {0.f, 0.f};
-#pragma unroll
-        for (int v = 0; v < 8; ++v) {
-          const uint4 a = *reinterpret_cast<const uint4*>(dor + ((v ^ (row64 & 7)) * 16));
-          const uint4 o = *reinterpret_cast<const uint4*>(orow + ((v ^ (row64 & 7)) * 16));
-          float fa[8], fo[8];
-          Elem<__nv_bfloat16>::unpack(a, fa);
-          Elem<__nv_bfloat16>::unpack(o, fo);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) acc[i & 1] += fa[i] * fo[i];
-        }
-        nD = -(acc[0] + acc[1]);
-      }
-    }
-    if (st < p.n_sub) {
-      float* stat = p.stats + (static_cast<long long>(bk) * p.n_sub + st) * (2 * kSub);
-      stat[row64] = nl;
-      stat[kSub + row64] = nD;
-    }
-    const bool warp_active = __any_sync(kFullMask, valid);
-    const uint64_t sl2 = f2_pack(p.scale_log2, p.scale_log2);
-    const uint64_t nl2 = f2_pack(nl, nl), nD2 = f2_pack(nD, nD);
-    for (int j = 0; ok && j < n_live; ++j) {
-      if (!__all_sync(kFullMask, bounded_wait<1>(&bars->s_full, j & 1, abort_flag))) {
-        ok = false;
-        break;
-      }
-      tc_fence_after();
-      if (warp_active) {
-        const int c0 = chunk_at(j) * kChunk;
-#pragma unroll
-        for (int gq = 0; gq < 2; ++gq) {
-          const int g0 = c0 + 32 * gq;
-          uint32_t vm = 0u;
-          if (kMode == kMaskBool) {
-            if (mrow != nullptr && g0 < p.N) vm = mask_bits32(mrow, g0, p.N, p.mask_words);
-          } else {
-            vm = low_bits(rds - g0) | (low_bits(e2 - g0) & ~low_bits(rde - g0));
-          }
-          const bool full = __all_sync(kFullMask, !valid || vm == 0xffffffffu);
-          const bool none = __all_sync(kFullMask, !valid || vm == 0u);
-          uint32_t pk[16];
-          if (none) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) pk[i] = 0u;
-          } else {
-            float s[32], dp[32];
-            tmem_ld32(tbase + kDqS + 32 * gq, s);
-            tmem_ld32(tbase + kDqP + 32 * gq, dp);
-            tmem_wait_ld();
-#pragma unroll
-            for (int k = 0; k < 16; ++k) {
-              float x0, x1, d0, d1;
-              f2_unpack(f2_fma(f2_pack(s[2 * k], s[2 * k + 1]), sl2, nl2), x0, x1);
-              const uint64_t e = f2_pack(ex2(x0), ex2(x1));
-              f2_unpack(f2_mul(e, f2_add(f2_pack(dp[2 * k], dp[2 * k + 1]), nD2)), d0, d1);
-              if (!full) {
-                d0 = (vm >> (2 * k)) & 1u ? d0 : 0.f;
-                d1 = (vm >> (2 * k + 1)) & 1u ? d1 : 0.f;
-              }
-              pk[k] = pack_bf16x2(d0, d1);
-            }
-          }
-          tmem_st16(tbase + kDqS + 16 * gq, pk);
-        }
-        tmem_wait_st();
-      }
-      tc_fence_before();
-      mbar_arrive_elect(&bars->ds_full);
-    }
-    // Epilogue: scale dQ, stage its rows where O was, one TMA store per
-    // sub-tile.
-    if (ok && n_live > 0 &&
-        !__all_sync(kFullMask, bounded_wait(&bars->out_full, 0, abort_flag)))
-      ok = false;
-    if (ok && n_live > 0) {
-      tc_fence_after();
-      if (warp_active) {
-        uint8_t* stage = o_smem + half * kSubBytes + row64 * kRowBytes;
-#pragma unroll 1
-        for (int q4 = 0; q4 < 4; ++q4) {
-          float o[16];
-          tmem_ld16(tbase + kDqO + 16 * q4, o);
-          tmem_wait_ld();
-#pragma unroll
-          for (int v = 0; v < 2; ++v) {
-            uint32_t w[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              w[e] = pack_bf16x2(o[v * 8 + 2 * e] * p.out_scale, o[v * 8 + 2 * e + 1] * p.out_scale);
-            const uint32_t c = static_cast<uint32_t>(2 * q4 + v) ^ static_cast<uint32_t>(row64 & 7);
-            st_shared_v4(stage + c * 16, w[0], w[1], w[2], w[3]);
-          }
-        }
-      }
-      fence_proxy_async_smem();
-      __syncwarp();
-      mbar_arrive_elect(&bars->staged[half]);
-      if ((warp & 1) == 0 && lane == 0 && st < p.n_sub &&
-          bounded_wait(&bars->staged[half], 0, abort_flag)) {
-        tma_store_4d(&p.tm_dq, o_smem + half * kSubBytes, 0, kvh * p.G + hb * p.Gb, mt * p.MT, b);
-        bulk_commit_group();
-        bulk_wait_all0();
-      }
-    } else if (n_live == 0 && valid) {
-      uint4* dst = reinterpret_cast<uint4*>(p.dq + row * 64);
-#pragma unroll
-      for (int v = 0; v < 8; ++v) dst[v] = make_uint4(0, 0, 0, 0);
-    }
-    __syncwarp();
-  }
-
-  tc_fence_before();
-  __syncthreads();
-  if (threadIdx.x == 0 && *abort_flag) publish_device_error(p.host_err, VLAK_ERR_DEVICE_TIMEOUT);
-  if (warp == kWarpMma) {
-    tc_fence_after();
-    tmem_dealloc(tmem, kTmemCols);
+  for (int o = 1; o < 8; o <<= 1) d += __shfl_xor_sync(kFullMask, d, o);
+  if (v == 0) {
+    float* stat = p.stats + static_cast<long long>(blockIdx.x) * kStatFloats;
+    stat[row] = nl;
+    stat[kSub + row] = -d;
   }
 }
 
 // ---------------------------------------------------------------------------
-// dkv kernel
+// Items
 
-struct DkvBarriers {
-  uint64_t kv_full, q_full[kDkvStages], q_empty[kDkvStages], s_full, p_full, out_full, staged, drain;
+// An item as the producer hands it out through shared memory (16 bytes at a
+// time).
+struct __align__(16) Item {
+  int live;           // -1: no more items; else its steps
+  int dkv, b, kvh;
+  int L;              // length of the sample (lengths only)
+  int k0;             // dkv: first key
+  int s0, n_here;     // dq: first sub-tile and how many (1 or 2)
+  int a1, b0;         // dq: live chunks [0, a1) and [b0, ...)
+  int mt_lo, mt_hi;   // dkv: live position blocks of each head block
+};
+static_assert(sizeof(Item) == 48, "three vectors");
+
+// The steps of an item in order: chunk `pos` (dq), or position block `pos` of
+// head block `hb` (dkv).
+struct Steps {
+  int pos, hb;
+  __device__ __forceinline__ void begin(const Item& it) {
+    hb = 0;
+    pos = it.dkv ? it.mt_lo : it.a1 > 0 ? 0 : it.b0;
+  }
+  __device__ __forceinline__ void next(const Item& it) {
+    ++pos;
+    if (it.dkv) {
+      if (pos == it.mt_hi) {
+        pos = it.mt_lo;
+        ++hb;
+      }
+    } else if (pos == it.a1) {
+      pos = it.b0;
+    }
+  }
+};
+
+struct Barriers {
+  uint64_t a_full[2], a_empty[2];          // stationary tiles of an item
+  uint64_t b_full[kRing], b_empty[kRing];  // streamed pairs
+  uint64_t s_full[kStages], x_full[kStages], t_empty[kStages];
+  uint64_t out_full[2], staged[2];         // by the group that stores the item
+  uint64_t acc_empty, drain[2];
+  uint64_t it_full[kQueue], it_empty[kQueue];
+  Item item[kQueue];
   uint32_t tmem_base;
   int abort_flag;
 };
-static_assert(sizeof(DkvBarriers) <= kBarrierBytes, "barrier block");
+constexpr int kBarrierBytes = 640;
+static_assert(sizeof(Barriers) <= kBarrierBytes, "barrier block");
+constexpr int kSmem = 2 * 4 * kSubBytes + kRing * (2 * kSubBytes + kStatBytes) + 2 * 2 * kStatBytes +
+                      kBarrierBytes + 1024;
+static_assert(kSmem <= 227 * 1024, "shared memory");
 
-// TMEM columns of the dkv kernel; P^T and dS^T (bf16 pairs) overwrite the
-// first halves of S^T and dP^T
-constexpr uint32_t kDkvS = 0, kDkvP = 64, kDkvV = 128, kDkvK = 192;
+template <int kMode>
+__device__ __forceinline__ Item decode_item(const BwdParams& p, int id) {
+  Item it{};
+  it.dkv = id < p.n_dkv;
+  const int i = it.dkv ? id : id - p.n_dkv;
+  const int inner = it.dkv ? p.n_kblk : p.n_pair;
+  // blk: key block, or pair of sub-tiles counted from the last, whose rows see
+  // the most keys under a staircase, as the first keys are seen by the most rows
+  const int blk = p.bk_inner ? i / p.n_bk : i % inner;
+  const int bk = p.bk_inner ? i - blk * p.n_bk : i / inner;
+  it.b = bk / p.Hkv;
+  it.kvh = bk - it.b * p.Hkv;
+  it.L = kMode == kMaskLength ? length_of(p, it.b) : 0;
+  if (it.dkv) {
+    // position blocks [mt_lo, mt_hi) holding a row that sees a key of the item
+    it.k0 = blk * kKeys;
+    int mt_lo = 0, mt_hi = p.n_mt;
+    if (kMode == kMaskLength) {
+      mt_hi = it.k0 < it.L ? min(p.n_mt, (it.L + p.MT - 1) / p.MT) : 0;
+    } else if (kMode == kMaskAnalytic) {
+      const int pe = min(it.k0 + kKeys, p.P);  // prefix keys of the item: [k0, pe)
+      const bool prefix = it.k0 < min(pe, p.ds) || max(it.k0, p.de) < pe;
+      if (!prefix) {
+        const int c = max(it.k0, p.P);  // the first staircase key: visible from row c - (N - M)
+        mt_lo = c < min(it.k0 + kKeys, p.N) ? min(p.n_mt, max(0, c - (p.N - p.M)) / p.MT) : p.n_mt;
+      }
+    }
+    it.mt_lo = mt_lo;
+    it.mt_hi = mt_hi;
+    it.live = p.n_sub / p.n_mt * max(0, mt_hi - mt_lo);
+  } else {
+    it.s0 = 2 * (p.n_pair - 1 - blk);
+    it.n_here = min(2, p.n_sub - it.s0);
+    // first and last position of the rows
+    const int mt0 = it.s0 % p.n_mt, mt1 = (it.s0 + it.n_here - 1) % p.n_mt;
+    const int m_lo = min(mt0, mt1) * p.MT;
+    const int m_hi = min(p.M, (max(mt0, mt1) + 1) * p.MT) - 1;
+    int b1 = 0;
+    if (kMode == kMaskBool) {
+      it.a1 = p.n_chunks;
+    } else if (kMode == kMaskLength) {
+      it.a1 = m_lo < it.L ? (it.L + kChunk - 1) / kChunk : 0;
+    } else {
+      it.a1 = (p.ds + kChunk - 1) / kChunk;
+      if (p.de < p.N) {
+        const int e2 = max(p.P, min(p.N, p.N - p.M + m_hi + 1));
+        it.b0 = max(p.de / kChunk, it.a1);
+        b1 = (e2 + kChunk - 1) / kChunk;
+      }
+    }
+    it.live = it.a1 + max(0, b1 - it.b0);
+  }
+  return it;
+}
 
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
   asm volatile(
@@ -438,65 +305,55 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
 }
 
 template <int kMode>
-__global__ void __launch_bounds__(kThreads, 2) attn_bwd_dkv(const __grid_constant__ BwdParams p) {
+__global__ void __launch_bounds__(kThreads, 1) attn_bwd(const __grid_constant__ BwdParams p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = aligned_smem(smem_raw);
-  uint8_t* k_smem = smem;                       // [128 x 128 B], then the staged dK
-  uint8_t* v_smem = k_smem + 2 * kSubBytes;     // then the staged dV
-  uint8_t* q_smem = v_smem + 2 * kSubBytes;     // [stage][64 x 128 B]
-  uint8_t* do_smem = q_smem + kDkvStages * kSubBytes;
-  float* stat_smem = reinterpret_cast<float*>(do_smem + kDkvStages * kSubBytes);  // [stage][128]
-  DkvBarriers* bars =
-      reinterpret_cast<DkvBarriers*>(reinterpret_cast<uint8_t*>(stat_smem) + kDkvStages * kStatBytes);
+  uint8_t* a_smem = smem;                             // [2][A0 16 KB, A1 16 KB]; then the staged output
+  uint8_t* b_smem = a_smem + 2 * 4 * kSubBytes;       // [kRing][B0 8 KB, B1 8 KB]
+  float* b_stat = reinterpret_cast<float*>(b_smem + kRing * 2 * kSubBytes);  // [kRing][128]: dkv
+  float* a_stat = b_stat + kRing * kStatFloats;       // [2][2 sub-tiles][128]: dq
+  Barriers* bars = reinterpret_cast<Barriers*>(a_stat + 2 * 2 * kStatFloats);
   volatile int* abort_flag = &bars->abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-  const int bk = blockIdx.x / p.n_kblk;
-  const int k0 = (blockIdx.x - bk * p.n_kblk) * kKeys;
-  const int b = bk / p.Hkv, kvh = bk - b * p.Hkv;
-  const int L = kMode == kMaskLength ? length_of(p, b) : 0;
-
-  // position blocks [mt_lo, mt_hi) holding a row that sees a key of this CTA
-  int mt_lo = 0, mt_hi = p.n_mt;
-  if (kMode == kMaskLength) {
-    mt_hi = k0 < L ? min(p.n_mt, (L + p.MT - 1) / p.MT) : 0;
-  } else if (kMode == kMaskAnalytic) {
-    const int pe = min(k0 + kKeys, p.P);  // prefix keys of the CTA: [k0, pe)
-    const bool prefix = k0 < min(pe, p.ds) || max(k0, p.de) < pe;
-    if (!prefix) {
-      const int c = max(k0, p.P);  // the first staircase key: visible from row c - (N - M)
-      const int m_first = c - (p.N - p.M);
-      mt_lo = c < min(k0 + kKeys, p.N) ? min(p.n_mt, max(0, m_first) / p.MT) : p.n_mt;
-    }
-  }
-  const int per_head = max(0, mt_hi - mt_lo);
-  const int n_live = p.n_sub / p.n_mt * per_head;
-
   if (threadIdx.x == 0) {
-    mbar_init(&bars->kv_full, 1);
-    for (int i = 0; i < kDkvStages; ++i) {
-      mbar_init(&bars->q_full[i], 1);
-      mbar_init(&bars->q_empty[i], 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bars->a_full[i], 1);
+      mbar_init(&bars->a_empty[i], 1);
+      mbar_init(&bars->out_full[i], 1);
+      mbar_init(&bars->staged[i], kGroupWarps);
     }
-    mbar_init(&bars->s_full, 1);
-    mbar_init(&bars->p_full, 4);
-    mbar_init(&bars->staged, 4);
-    mbar_init(&bars->out_full, 1);
-    mbar_init(&bars->drain, 1);
+    for (int i = 0; i < kRing; ++i) {
+      mbar_init(&bars->b_full[i], 1);
+      mbar_init(&bars->b_empty[i], 1);
+    }
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&bars->s_full[i], 1);
+      mbar_init(&bars->x_full[i], kGroupWarps);
+      mbar_init(&bars->t_empty[i], 1);
+    }
+    for (int i = 0; i < kQueue; ++i) {
+      mbar_init(&bars->it_full[i], 1);
+      mbar_init(&bars->it_empty[i], kComputeWarps + 2);
+    }
+    mbar_init(&bars->acc_empty, kGroupWarps);
+    mbar_init(&bars->drain[0], 1);
+    mbar_init(&bars->drain[1], 1);
     bars->abort_flag = 0;
     fence_mbar_init();
   }
-  if (warp == kWarpMma) {
+  if (warp == kWarpAccum) {
     tmem_alloc(&bars->tmem_base, kTmemCols);
     tmem_relinquish();
   }
-  // Rows of the ring that no box covers meet P = dS = 0 in the products; clear
-  // them once, so that they are finite.
+  // Rows of the ring that no query box covers meet P = dS = 0 in the dkv
+  // products; clear them once, so that they are finite. (dq steps, which fill
+  // whole tiles, only follow the dkv items.)
   {
     const int row0 = p.Gb * p.MT, n = (kSub - row0) * 8;
-    for (int i = threadIdx.x; i < 2 * kDkvStages * n; i += kThreads) {
+    for (int i = threadIdx.x; i < 2 * kRing * n; i += kThreads) {
       const int t = i / n;
-      reinterpret_cast<uint4*>(q_smem + t * kSubBytes + row0 * kRowBytes)[i - t * n] =
+      reinterpret_cast<uint4*>(b_smem + t * kSubBytes + row0 * kRowBytes)[i - t * n] =
           make_uint4(0, 0, 0, 0);
     }
     fence_proxy_async_smem();
@@ -505,235 +362,434 @@ __global__ void __launch_bounds__(kThreads, 2) attn_bwd_dkv(const __grid_constan
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = bars->tmem_base;
-  // i-th live sub-tile: head block and position block
-  auto sub_at = [&](int i) {
-    const int hb = i / per_head;
-    return hb * p.n_mt + mt_lo + (i - hb * per_head);
+
+  // The n-th item handed out (live < 0: no more); every warp but the producer
+  // takes each once.
+  auto take_item = [&](uint32_t n, Item& it) {
+    const uint32_t q = n % kQueue;
+    if (!__all_sync(kFullMask, bounded_wait<1>(&bars->it_full[q], (n / kQueue) & 1, abort_flag)))
+      return false;
+    const int4* src = reinterpret_cast<const int4*>(&bars->item[q]);
+    int4* dst = reinterpret_cast<int4*>(&it);
+#pragma unroll
+    for (int i = 0; i < 3; ++i) dst[i] = src[i];
+    __syncwarp();
+    mbar_arrive_elect(&bars->it_empty[q]);
+    return true;
   };
 
   if (warp == kWarpProducer) {
-    int issued = 0;
-    if (n_live > 0) {
-      mbar_arrive_expect_tx_elect(&bars->kv_full, 4 * kSubBytes);
-      tma_load_4d_elect(k_smem, &p.tm_k, &bars->kv_full, 0, kvh, k0, b);
-      tma_load_4d_elect(v_smem, &p.tm_v, &bars->kv_full, 0, kvh, k0, b);
-    }
-    for (int j = 0; j < n_live; ++j) {
-      const int s = j % kDkvStages;
-      if (!__all_sync(kFullMask, bounded_wait(&bars->q_empty[s], ((j / kDkvStages) & 1) ^ 1, abort_flag))) {
+    uint32_t t = 0, live = 0;  // steps and live items issued
+    bool ok = true;
+    for (uint32_t n = 0; ok; ++n) {
+      const uint32_t q = n % kQueue;
+      if (!__all_sync(kFullMask, bounded_wait(&bars->it_empty[q], ((n / kQueue) & 1) ^ 1, abort_flag)))
         break;
+      int id = 0;
+      if (lane == 0) id = static_cast<int>(min(atomicAdd(p.counter, 1u), static_cast<unsigned>(p.n_items)));
+      id = __shfl_sync(kFullMask, id, 0);
+      Item it{};
+      if (id < p.n_items)
+        it = decode_item<kMode>(p, id);
+      else
+        it.live = -1;
+      if (lane == 0) {
+        bars->item[q] = it;
+        mbar_arrive(&bars->it_full[q]);
       }
-      const int st = sub_at(j), hb = st / p.n_mt, m0 = (st - hb * p.n_mt) * p.MT;
-      const int h = kvh * p.G + hb * p.Gb;
-      mbar_arrive_expect_tx_elect(&bars->q_full[s],
-                                  static_cast<uint32_t>(2 * p.Gb * p.MT * kRowBytes + kStatBytes));
-      tma_load_4d_elect(q_smem + s * kSubBytes, &p.tm_q, &bars->q_full[s], 0, h, m0, b);
-      tma_load_4d_elect(do_smem + s * kSubBytes, &p.tm_do, &bars->q_full[s], 0, h, m0, b);
-      bulk_load(stat_smem + s * 2 * kSub, p.stats + (static_cast<long long>(bk) * p.n_sub + st) * (2 * kSub),
-                kStatBytes, &bars->q_full[s]);
-      issued = j + 1;
-    }
-    if (n_live > 0) {
-      bounded_wait(&bars->kv_full, 0, abort_flag, false);
-      for (int j = max(0, issued - kDkvStages); j < issued; ++j)
-        bounded_wait(&bars->q_full[j % kDkvStages], (j / kDkvStages) & 1, abort_flag, false);
-    }
-    __syncwarp();
-  } else if (warp == kWarpMma) {
-    if (n_live > 0) {
-      const uint32_t id_kk = idesc_bf16_f32(128, 64, false), id_kn = idesc_bf16_f32(128, 64, true);
-      const uint32_t ks = smem_u32(k_smem), vs = smem_u32(v_smem);
-      auto issue_scores = [&](int j) {  // S^T = K Q^T, dP^T = V dO^T of sub-tile j
-        const int s = j % kDkvStages;
-        if (!__all_sync(kFullMask, bounded_wait<1>(&bars->q_full[s], (j / kDkvStages) & 1, abort_flag)))
-          return false;
-        if (kMode == kMaskLength) {  // rows past L meet P = dS = 0: 0 times NaN
-          const int st = sub_at(j), m0 = st % p.n_mt * p.MT;
-          const int lo = max(0, L - m0) * p.Gb;
-          clear_rows(q_smem + s * kSubBytes, lo, kSub);
-          clear_rows(do_smem + s * kSubBytes, lo, kSub);
+      __syncwarp();
+      if (it.live < 0) break;
+      if (it.live == 0) continue;
+      const int bk = it.b * p.Hkv + it.kvh;
+      const uint32_t ab = live & 1;
+      if (!__all_sync(kFullMask, bounded_wait(&bars->a_empty[ab], ((live >> 1) & 1) ^ 1, abort_flag)))
+        break;
+      uint8_t* a0 = a_smem + ab * 4 * kSubBytes;
+      uint8_t* a1 = a0 + 2 * kSubBytes;
+      if (it.dkv) {
+        mbar_arrive_expect_tx_elect(&bars->a_full[ab], 4 * kSubBytes);
+        tma_load_4d_elect(a0, &p.tm_k, &bars->a_full[ab], 0, it.kvh, it.k0, it.b);
+        tma_load_4d_elect(a1, &p.tm_v, &bars->a_full[ab], 0, it.kvh, it.k0, it.b);
+      } else {
+        mbar_arrive_expect_tx_elect(
+            &bars->a_full[ab],
+            static_cast<uint32_t>(it.n_here * (2 * p.Gb * p.MT * kRowBytes + kStatBytes)));
+        for (int i = 0; i < it.n_here; ++i) {
+          const int hb = (it.s0 + i) / p.n_mt, m0 = (it.s0 + i - hb * p.n_mt) * p.MT;
+          const int h = it.kvh * p.G + hb * p.Gb;
+          tma_load_4d_elect(a0 + i * kSubBytes, &p.tm_q, &bars->a_full[ab], 0, h, m0, it.b);
+          tma_load_4d_elect(a1 + i * kSubBytes, &p.tm_do, &bars->a_full[ab], 0, h, m0, it.b);
         }
-        tc_fence_after();
-        const uint32_t q0 = smem_u32(q_smem + s * kSubBytes), do0 = smem_u32(do_smem + s * kSubBytes);
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          umma_ss_elect(tmem + kDkvS, sdesc_sw128(ks + 32 * k), sdesc_sw128(q0 + 32 * k), id_kk, k > 0);
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          umma_ss_elect(tmem + kDkvP, sdesc_sw128(vs + 32 * k), sdesc_sw128(do0 + 32 * k), id_kk, k > 0);
-        umma_commit_elect(&bars->s_full);
-        return true;
-      };
-      bool ok = __all_sync(kFullMask, bounded_wait(&bars->kv_full, 0, abort_flag));
-      tc_fence_after();
-      ok = ok && issue_scores(0);
-      for (int j = 0; ok && j < n_live; ++j) {
-        if (!__all_sync(kFullMask, bounded_wait<1>(&bars->p_full, j & 1, abort_flag))) break;
-        tc_fence_after();
-        const int s = j % kDkvStages;
-        const uint32_t q0 = smem_u32(q_smem + s * kSubBytes), do0 = smem_u32(do_smem + s * kSubBytes);
-#pragma unroll
-        for (int k = 0; k < 4; ++k)  // dV += P^T dO
-          umma_ts_elect(tmem + kDkvV, tmem + kDkvS + 8 * k, sdesc_sw128(do0 + 2048 * k), id_kn,
-                        (j > 0 || k > 0) ? 1u : 0u);
-#pragma unroll
-        for (int k = 0; k < 4; ++k)  // dK += dS^T Q
-          umma_ts_elect(tmem + kDkvK, tmem + kDkvP + 8 * k, sdesc_sw128(q0 + 2048 * k), id_kn,
-                        (j > 0 || k > 0) ? 1u : 0u);
-        umma_commit_elect(&bars->q_empty[s]);
-        if (j + 1 < n_live) {
-          ok = issue_scores(j + 1);
+        bulk_load(a_stat + ab * 2 * kStatFloats,
+                  p.stats + (static_cast<long long>(bk) * p.n_sub + it.s0) * kStatFloats,
+                  it.n_here * kStatBytes, &bars->a_full[ab]);
+      }
+      ++live;
+      Steps step;
+      step.begin(it);
+      for (int j = 0; j < it.live; ++j, ++t, step.next(it)) {
+        const uint32_t s = t % kRing;
+        if (!__all_sync(kFullMask, bounded_wait(&bars->b_empty[s], ((t / kRing) & 1) ^ 1, abort_flag))) {
+          ok = false;
+          break;
+        }
+        uint8_t* b0 = b_smem + s * 2 * kSubBytes;
+        uint8_t* b1 = b0 + kSubBytes;
+        if (it.dkv) {
+          const int m0 = step.pos * p.MT, h = it.kvh * p.G + step.hb * p.Gb;
+          mbar_arrive_expect_tx_elect(&bars->b_full[s],
+                                      static_cast<uint32_t>(2 * p.Gb * p.MT * kRowBytes + kStatBytes));
+          tma_load_4d_elect(b0, &p.tm_q, &bars->b_full[s], 0, h, m0, it.b);
+          tma_load_4d_elect(b1, &p.tm_do, &bars->b_full[s], 0, h, m0, it.b);
+          bulk_load(b_stat + s * kStatFloats,
+                    p.stats + (static_cast<long long>(bk) * p.n_sub + step.hb * p.n_mt + step.pos) * kStatFloats,
+                    kStatBytes, &bars->b_full[s]);
         } else {
-          umma_commit_elect(&bars->out_full);
+          mbar_arrive_expect_tx_elect(&bars->b_full[s], 2 * kSubBytes);
+          tma_load_4d_elect(b0, &p.tm_k64, &bars->b_full[s], 0, it.kvh, step.pos * kChunk, it.b);
+          tma_load_4d_elect(b1, &p.tm_v64, &bars->b_full[s], 0, it.kvh, step.pos * kChunk, it.b);
         }
       }
-      umma_commit_elect(&bars->drain);
-      bounded_wait(&bars->drain, 0, abort_flag, false);
     }
+    // never leave the CTA with copies in flight (bounded, abort or not)
+    for (uint32_t k = live > 2 ? live - 2 : 0; k < live; ++k)
+      bounded_wait(&bars->a_full[k & 1], (k >> 1) & 1, abort_flag, false);
+    for (uint32_t k = t > kRing ? t - kRing : 0; k < t; ++k)
+      bounded_wait(&bars->b_full[k % kRing], (k / kRing) & 1, abort_flag, false);
+    __syncwarp();
+  } else if (warp == kWarpScores) {
+    // T0 = A0 B0^T and T1 = A1 B1^T of every step, up to kStages steps (and one
+    // item, by the stationary tiles) ahead of the accumulating products.
+    const uint32_t id_kk = idesc_bf16_f32(128, 64, false);
+    uint32_t t = 0, live = 0;
+    bool ok = true;
+    for (uint32_t n = 0; ok; ++n) {
+      Item it;
+      if (!take_item(n, it) || it.live < 0) break;
+      if (it.live == 0) continue;
+      const uint32_t ab = live & 1;
+      if (!__all_sync(kFullMask, bounded_wait<1>(&bars->a_full[ab], (live >> 1) & 1, abort_flag))) break;
+      ++live;
+      // descriptors step by 16 of the 64 columns: 32 bytes of a swizzled row
+      const uint64_t a0 = sdesc_sw128(smem_u32(a_smem + ab * 4 * kSubBytes));
+      const uint64_t a1 = a0 + 2 * kSubBytes / 16;
+      Steps step;
+      step.begin(it);
+      for (int j = 0; j < it.live; ++j, ++t, step.next(it)) {
+        const uint32_t s = t % kRing, st = t % kStages;
+        if (!__all_sync(kFullMask,
+                        bounded_wait<1>(&bars->t_empty[st], ((t / kStages) & 1) ^ 1, abort_flag) &&
+                            bounded_wait<1>(&bars->b_full[s], (t / kRing) & 1, abort_flag))) {
+          ok = false;
+          break;
+        }
+        uint8_t* bp = b_smem + s * 2 * kSubBytes;
+        // streamed rows that meet X = 0 only, and may hold NaN: keys that no
+        // query sees (dq), query rows past L (dkv)
+        if (kMode != kMaskBool && !it.dkv) {
+          const int c0 = step.pos * kChunk;
+          const int lo = kMode == kMaskLength ? it.L - c0 : p.ds - c0;
+          const int hi = kMode == kMaskLength ? kChunk : p.de - c0;
+          clear_rows(bp, max(lo, 0), min(hi, kChunk));
+        }
+        if (kMode == kMaskLength && it.dkv) {
+          const int lo = max(0, it.L - step.pos * p.MT) * p.Gb;
+          clear_rows(bp, lo, kSub);
+          clear_rows(bp + kSubBytes, lo, kSub);
+        }
+        tc_fence_after();
+        const uint64_t b0 = sdesc_sw128(smem_u32(bp)), b1 = b0 + kSubBytes / 16;
+        const uint32_t d = tmem + kStage0 + st * kStageCols;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) umma_ss_elect(d, a0 + 2 * k, b0 + 2 * k, id_kk, k > 0);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) umma_ss_elect(d + kT1, a1 + 2 * k, b1 + 2 * k, id_kk, k > 0);
+        umma_commit_elect(&bars->s_full[st]);
+      }
+    }
+    // every issued product completes before TMEM is released
+    umma_commit_elect(&bars->drain[0]);
+    bounded_wait(&bars->drain[0], 0, abort_flag, false);
+    __syncwarp();
+  } else if (warp == kWarpAccum) {
+    // acc1 += X1 B0, and acc0 += X0 B1 of a dkv item.
+    const uint32_t id_kn = idesc_bf16_f32(128, 64, true);
+    uint32_t t = 0, live = 0;
+    bool ok = true;
+    for (uint32_t n = 0; ok; ++n) {
+      Item it;
+      if (!take_item(n, it) || it.live < 0) break;
+      if (it.live == 0) continue;
+      for (int j = 0; j < it.live; ++j, ++t) {
+        const uint32_t s = t % kRing, st = t % kStages;
+        // the step's X, and at an item's first step the previous item's
+        // accumulators read
+        if (!__all_sync(kFullMask,
+                        (j > 0 || live == 0 ||
+                         bounded_wait<1>(&bars->acc_empty, (live - 1) & 1, abort_flag)) &&
+                            bounded_wait<1>(&bars->x_full[st], (t / kStages) & 1, abort_flag))) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint64_t b0 = sdesc_sw128(smem_u32(b_smem + s * 2 * kSubBytes)), b1 = b0 + kSubBytes / 16;
+        const uint32_t x = tmem + kStage0 + st * kStageCols;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)  // dV += P^T dO: 16 rows are 2 KB
+          umma_ts_elect(tmem + kAcc0, x + packed_col(k), b1 + 128 * k, id_kn,
+                        (j > 0 || k > 0) ? 1u : 0u, it.dkv);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)  // dK += dS^T Q, dQ += dS K
+          umma_ts_elect(tmem + kAcc1, x + kT1 + packed_col(k), b0 + 128 * k, id_kn,
+                        (j > 0 || k > 0) ? 1u : 0u);
+        umma_commit_elect(&bars->b_empty[s]);
+        umma_commit_elect(&bars->t_empty[st]);
+      }
+      if (!ok) break;
+      umma_commit_elect(&bars->out_full[live & 1]);
+      ++live;
+    }
+    umma_commit_elect(&bars->drain[1]);
+    bounded_wait(&bars->drain[1], 0, abort_flag, false);
     __syncwarp();
   } else {
-    // Compute warps: one key per thread, a sub-tile's rows along the columns.
-    const int key = k0 + warp * 32 + lane;
-    const bool valid = key < p.N;
-    const uint32_t tbase = tmem + (static_cast<uint32_t>(warp * 32) << 16);
-    // rows m in [m_see, m_end) see this key (all of them, none, or from the
-    // staircase's step on)
-    int m_see = 0, m_end = p.M;
-    if (kMode == kMaskAnalytic) {
-      if (key >= p.P)
-        m_see = key - (p.N - p.M);
-      else if (key >= p.ds && key < p.de)
-        m_end = 0;
-    } else if (kMode == kMaskLength) {
-      m_end = key < L ? L : 0;
-    }
-    if (!valid) m_end = 0;
+    // Compute warps. A step belongs to the group of its parity, an item's
+    // output to the group of the item's.
+    const int group = warp >> 3, quarter = warp & 3, gq = (warp >> 2) & 1;
+    const int tl = quarter * 32 + lane;  // TMEM lane: key of a dkv item, row of a dq item
+    const uint32_t tbase = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
     const uint64_t sl2 = f2_pack(p.scale_log2, p.scale_log2);
+    uint32_t t = 0, live = 0;
     bool ok = true;
-    for (int j = 0; ok && j < n_live; ++j) {
-      const int st = sub_at(j), m0 = st % p.n_mt * p.MT, s = j % kDkvStages;
-      // columns of the sub-tile that see the key (rows past M or the box carry
-      // -lse = -inf, so their P is 0 without a mask)
-      uint32_t vm[2];
-      if (kMode == kMaskBool) {
-        vm[0] = vm[1] = 0u;
-        if (valid) {
-          const uint8_t* col = p.mask + static_cast<long long>(b) * p.mask_sb + key;
-          const uint64_t heads = ~0ull >> (64 - p.Gb);
-          const int n = min(p.MT, p.M - m0);
-          for (int i = 0; i < n; ++i) {
-            if (__ldg(col + static_cast<long long>(m0 + i) * p.mask_sm) == 0) continue;
-            const uint64_t bits = heads << (i * p.Gb);
-            vm[0] |= static_cast<uint32_t>(bits);
-            vm[1] |= static_cast<uint32_t>(bits >> 32);
+    for (uint32_t n = 0; ok; ++n) {
+      Item it;
+      if (!take_item(n, it) || it.live < 0) break;
+      // this lane's key, or row
+      const int key = it.k0 + tl;
+      const SubRow r = sub_row(p, it.s0 + (quarter >> 1), (quarter & 1) * 32 + lane);
+      const bool valid = it.dkv ? key < p.N : r.valid;
+      if (it.live == 0) {  // nothing seen: zeros
+        if (group == static_cast<int>(n & 1) && gq == 0 && valid) {
+          __nv_bfloat16* dst[2];
+          if (it.dkv) {
+            const long long at = ((static_cast<long long>(it.b) * p.N + key) * p.Hkv + it.kvh) * 64;
+            dst[0] = p.dk + at;
+            dst[1] = p.dv + at;
+          } else {
+            dst[0] = dst[1] = p.dq + ((static_cast<long long>(it.b) * p.M + r.m) * p.H +
+                                      it.kvh * p.G + r.g) * 64;
+          }
+#pragma unroll
+          for (int v = 0; v < 8; ++v) {
+            reinterpret_cast<uint4*>(dst[0])[v] = make_uint4(0, 0, 0, 0);
+            reinterpret_cast<uint4*>(dst[1])[v] = make_uint4(0, 0, 0, 0);
           }
         }
+        continue;
+      }
+      const uint32_t ab = live & 1;
+      // dkv: rows m in [from, to) see the key; dq: keys [0, from) and [mid, to)
+      // are seen by the row
+      int from = 0, mid = 0, to = 0;
+      const uint8_t* mrow = nullptr;
+      if (it.dkv) {
+        to = p.M;
+        if (kMode == kMaskAnalytic) {
+          if (key >= p.P)
+            from = key - (p.N - p.M);
+          else if (key >= p.ds && key < p.de)
+            to = 0;
+        } else if (kMode == kMaskLength) {
+          to = key < it.L ? it.L : 0;
+        }
+        if (!valid) to = 0;
+        if (kMode == kMaskBool && valid) mrow = p.mask + it.b * p.mask_sb + key;
       } else {
-        const int lo = min(max(m_see - m0, 0), kSub) * p.Gb;
-        const int hi = min(max(m_end - m0, 0), kSub) * p.Gb;
-        const bool last = m_end >= p.M && valid;  // rows past M are masked by their statistics
-        vm[0] = ~low_bits(lo) & (last && hi > 0 ? 0xffffffffu : low_bits(hi));
-        vm[1] = ~low_bits(lo - 32) & (last && hi > 0 ? 0xffffffffu : low_bits(hi - 32));
+        if (kMode == kMaskAnalytic) {
+          from = p.ds;
+          mid = p.de;
+          to = max(p.P, min(p.N, p.N - p.M + r.m + 1));
+        } else if (kMode == kMaskLength) {
+          to = r.m < it.L ? it.L : 0;
+        }
+        if (kMode == kMaskBool && valid) mrow = p.mask + it.b * p.mask_sb + r.m * p.mask_sm;
       }
-      if (!__all_sync(kFullMask, bounded_wait<1>(&bars->q_full[s], (j / kDkvStages) & 1, abort_flag)) ||
-          !__all_sync(kFullMask, bounded_wait<1>(&bars->s_full, j & 1, abort_flag))) {
-        ok = false;
-        break;
-      }
-      tc_fence_after();
-      const float4* stat = reinterpret_cast<const float4*>(stat_smem + s * 2 * kSub);
-#pragma unroll
-      for (int gq = 0; gq < 2; ++gq) {
-        const bool full = __all_sync(kFullMask, !valid || vm[gq] == 0xffffffffu);
-        const bool none = __all_sync(kFullMask, vm[gq] == 0u);
+      uint64_t nl2 = 0ull, nD2 = 0ull;
+      bool first = !it.dkv;
+      Steps step;
+      step.begin(it);
+      for (int j = 0; ok && j < it.live; ++j, ++t, step.next(it)) {
+        if (static_cast<int>(t & 1) != group) continue;
+        if (first) {
+          // the row's statistics (only with a step to do: a group without one
+          // may come here after the tiles have been replaced)
+          if (!__all_sync(kFullMask, bounded_wait<1>(&bars->a_full[ab], (live >> 1) & 1, abort_flag))) {
+            ok = false;
+            break;
+          }
+          const float* stat = a_stat + (ab * 2 + (quarter >> 1)) * kStatFloats + (quarter & 1) * 32 + lane;
+          nl2 = f2_pack(stat[0], stat[0]);
+          nD2 = f2_pack(stat[kSub], stat[kSub]);
+          first = false;
+        }
+        const uint32_t st = t % kStages, s = t % kRing;
+        // which of the warp's 32 columns this lane sees
+        uint32_t vm = 0u;
+        if (it.dkv) {
+          // (rows past M or the box have -lse = -inf: their P is 0 unmasked)
+          const int m0 = step.pos * p.MT;
+          if (kMode == kMaskBool) {
+            if (valid) {
+              const uint64_t heads = ~0ull >> (64 - p.Gb);
+              const int rows = min(p.MT, p.M - m0);
+              for (int i = 0; i < rows; ++i)
+                if (__ldg(mrow + static_cast<long long>(m0 + i) * p.mask_sm) != 0)
+                  vm |= static_cast<uint32_t>((heads << (i * p.Gb)) >> (32 * gq));
+            }
+          } else {
+            const int lo = min(max(from - m0, 0), kSub) * p.Gb - 32 * gq;
+            const int hi = min(max(to - m0, 0), kSub) * p.Gb - 32 * gq;
+            vm = ~low_bits(lo) & (to >= p.M ? 0xffffffffu : low_bits(hi));
+          }
+        } else {
+          const int g0 = step.pos * kChunk + 32 * gq;
+          if (kMode == kMaskBool) {
+            if (mrow != nullptr && g0 < p.N) vm = mask_bits32(mrow, g0, p.N, p.mask_words);
+          } else {
+            vm = low_bits(from - g0) | (low_bits(to - g0) & ~low_bits(mid - g0));
+          }
+        }
+        const bool full = __all_sync(kFullMask, !valid || vm == 0xffffffffu);
+        const bool none = __all_sync(kFullMask, !valid || vm == 0u);
+        // A group sees every phase of its ring slots (kRing is even), and a
+        // stage's skipped phase completes before the step it sees in between.
+        if ((it.dkv && !__all_sync(kFullMask, bounded_wait<1>(&bars->b_full[s], (t / kRing) & 1, abort_flag))) ||
+            !__all_sync(kFullMask, bounded_wait<1>(&bars->s_full[st], (t / kStages) & 1, abort_flag))) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t t0 = tbase + kStage0 + st * kStageCols + 32 * gq;
         uint32_t pp[16], pd[16];
         if (none) {
 #pragma unroll
           for (int i = 0; i < 16; ++i) pp[i] = pd[i] = 0u;
         } else {
           float sv[32], dp[32];
-          tmem_ld32(tbase + kDkvS + 32 * gq, sv);
-          tmem_ld32(tbase + kDkvP + 32 * gq, dp);
+          tmem_ld32(t0, sv);
+          tmem_ld32(t0 + kT1, dp);
           tmem_wait_ld();
+          const float4* stat = reinterpret_cast<const float4*>(b_stat + s * kStatFloats) + 8 * gq;
+          // four bodies: per-column or per-lane statistics, all shown or not
+          auto grads = [&](auto dkv, auto masked) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {  // four rows
-            const float4 l4 = stat[8 * gq + i], d4 = stat[16 + 8 * gq + i];
-            const uint64_t nl2[2] = {f2_pack(l4.x, l4.y), f2_pack(l4.z, l4.w)};
-            const uint64_t nD2[2] = {f2_pack(d4.x, d4.y), f2_pack(d4.z, d4.w)};
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              const int k = 2 * i + u;
-              float x0, x1, d0, d1;
-              f2_unpack(f2_fma(f2_pack(sv[2 * k], sv[2 * k + 1]), sl2, nl2[u]), x0, x1);
-              float e0 = ex2(x0), e1 = ex2(x1);
-              f2_unpack(f2_mul(f2_pack(e0, e1),
-                               f2_add(f2_pack(dp[2 * k], dp[2 * k + 1]), nD2[u])), d0, d1);
-              if (!full) {
-                const bool see0 = (vm[gq] >> (2 * k)) & 1u, see1 = (vm[gq] >> (2 * k + 1)) & 1u;
-                e0 = see0 ? e0 : 0.f;
-                d0 = see0 ? d0 : 0.f;
-                e1 = see1 ? e1 : 0.f;
-                d1 = see1 ? d1 : 0.f;
+            for (int i = 0; i < 8; ++i) {  // four columns
+              uint64_t l2[2] = {nl2, nl2}, d2[2] = {nD2, nD2};
+              if (decltype(dkv)::value) {
+                const float4 l4 = stat[i], d4 = stat[16 + i];
+                l2[0] = f2_pack(l4.x, l4.y);
+                l2[1] = f2_pack(l4.z, l4.w);
+                d2[0] = f2_pack(d4.x, d4.y);
+                d2[1] = f2_pack(d4.z, d4.w);
               }
-              pp[k] = pack_bf16x2(e0, e1);
-              pd[k] = pack_bf16x2(d0, d1);
+#pragma unroll
+              for (int u = 0; u < 2; ++u) {
+                const int k = 2 * i + u;
+                float x0, x1, d0, d1;
+                f2_unpack(f2_fma(f2_pack(sv[2 * k], sv[2 * k + 1]), sl2, l2[u]), x0, x1);
+                float e0 = ex2(x0), e1 = ex2(x1);
+                f2_unpack(f2_mul(f2_pack(e0, e1),
+                                 f2_add(f2_pack(dp[2 * k], dp[2 * k + 1]), d2[u])), d0, d1);
+                if (decltype(masked)::value) {
+                  const bool see0 = (vm >> (2 * k)) & 1u, see1 = (vm >> (2 * k + 1)) & 1u;
+                  e0 = see0 ? e0 : 0.f;
+                  d0 = see0 ? d0 : 0.f;
+                  e1 = see1 ? e1 : 0.f;
+                  d1 = see1 ? d1 : 0.f;
+                }
+                if (decltype(dkv)::value) pp[k] = pack_bf16x2(e0, e1);
+                pd[k] = pack_bf16x2(d0, d1);
+              }
             }
+          };
+          using Yes = std::true_type;
+          using No = std::false_type;
+          if (it.dkv)
+            full ? grads(Yes(), No()) : grads(Yes(), Yes());
+          else
+            full ? grads(No(), No()) : grads(No(), Yes());
+        }
+        if (it.dkv) tmem_st16(t0, pp);
+        tmem_st16(t0 + kT1, pd);
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive_elect(&bars->x_full[st]);
+      }
+      if (!ok) break;
+      if (static_cast<int>(ab) == group) {
+        // Output: the accumulators, scaled, staged over the item's stationary
+        // tiles in the swizzled layout of the maps, then TMA stores.
+        if (!__all_sync(kFullMask, bounded_wait(&bars->out_full[group], (live >> 1) & 1, abort_flag))) break;
+        tc_fence_after();
+        uint8_t* a0 = a_smem + ab * 4 * kSubBytes;
+        // dkv: dV (first warps of a quarter) over V, dK (second) over K, 64
+        // columns each; dq: 32 columns of dQ each, over Q
+        const float scale = it.dkv && gq == 0 ? 1.f : p.out_scale;
+        uint8_t* stage = a0 + (it.dkv && gq == 0 ? 2 * kSubBytes : 0) + tl * kRowBytes;
+        const uint32_t acc = tbase + (it.dkv && gq == 0 ? kAcc0 : kAcc1);
+        const int blocks = it.dkv ? 2 : 1;  // of 32 columns
+        for (int q = 0; q < blocks; ++q) {
+          const int col = it.dkv ? 32 * q : 32 * gq;
+          float o[32];
+          tmem_ld32(acc + col, o);
+          tmem_wait_ld();
+          if (q == blocks - 1) {  // read: the next item may accumulate
+            tc_fence_before();
+            mbar_arrive_elect(&bars->acc_empty);
+          }
+#pragma unroll
+          for (int v = 0; v < 4; ++v) {
+            uint32_t w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              w[e] = pack_bf16x2(o[v * 8 + 2 * e] * scale, o[v * 8 + 2 * e + 1] * scale);
+            const uint32_t c = static_cast<uint32_t>(col / 8 + v) ^ static_cast<uint32_t>(tl & 7);
+            st_shared_v4(stage + c * 16, w[0], w[1], w[2], w[3]);
           }
         }
-        tmem_st16(tbase + kDkvS + 16 * gq, pp);
-        tmem_st16(tbase + kDkvP + 16 * gq, pd);
-      }
-      tmem_wait_st();
-      tc_fence_before();
-      mbar_arrive_elect(&bars->p_full);
-    }
-    if (ok && n_live > 0 &&
-        !__all_sync(kFullMask, bounded_wait(&bars->out_full, 0, abort_flag)))
-      ok = false;
-    const int row = warp * 32 + lane;
-    if (ok && n_live > 0) {
-      tc_fence_after();
-#pragma unroll 1
-      for (int q = 0; q < 8; ++q) {  // dV, then dK, 16 columns at a time
-        const float scale = q < 4 ? 1.f : p.out_scale;
-        float o[16];
-        tmem_ld16(tbase + kDkvV + 16 * q, o);
-        tmem_wait_ld();
-        uint8_t* stage = (q < 4 ? v_smem : k_smem) + row * kRowBytes;
-#pragma unroll
-        for (int v = 0; v < 2; ++v) {
-          uint32_t w[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            w[e] = pack_bf16x2(o[v * 8 + 2 * e] * scale, o[v * 8 + 2 * e + 1] * scale);
-          const uint32_t c = static_cast<uint32_t>(2 * (q & 3) + v) ^ static_cast<uint32_t>(row & 7);
-          st_shared_v4(stage + c * 16, w[0], w[1], w[2], w[3]);
+        fence_proxy_async_smem();
+        __syncwarp();
+        mbar_arrive_elect(&bars->staged[group]);
+        if ((warp & 7) == 0) {
+          if (!__all_sync(kFullMask, bounded_wait(&bars->staged[group], (live >> 1) & 1, abort_flag))) break;
+          if (lane == 0) {
+            if (it.dkv) {
+              tma_store_4d(&p.tm_dk, a0, 0, it.kvh, it.k0, it.b);
+              tma_store_4d(&p.tm_dv, a0 + 2 * kSubBytes, 0, it.kvh, it.k0, it.b);
+            } else {
+              for (int i = 0; i < it.n_here; ++i) {
+                const int hb = (it.s0 + i) / p.n_mt, m0 = (it.s0 + i - hb * p.n_mt) * p.MT;
+                tma_store_4d(&p.tm_dq, a0 + i * kSubBytes, 0, it.kvh * p.G + hb * p.Gb, m0, it.b);
+              }
+            }
+            bulk_commit_group();
+            bulk_wait_read0();
+            mbar_arrive(&bars->a_empty[ab]);
+          }
+          __syncwarp();
         }
       }
-      fence_proxy_async_smem();
-      __syncwarp();
-      mbar_arrive_elect(&bars->staged);
-      if (threadIdx.x == 0 && bounded_wait(&bars->staged, 0, abort_flag)) {
-        tma_store_4d(&p.tm_dv, v_smem, 0, kvh, k0, b);
-        tma_store_4d(&p.tm_dk, k_smem, 0, kvh, k0, b);
-        bulk_commit_group();
-        bulk_wait_all0();
-      }
-    } else if (n_live == 0 && valid) {
-      const long long at = ((static_cast<long long>(b) * p.N + key) * p.Hkv + kvh) * 64;
-#pragma unroll
-      for (int v = 0; v < 8; ++v) {
-        reinterpret_cast<uint4*>(p.dk + at)[v] = make_uint4(0, 0, 0, 0);
-        reinterpret_cast<uint4*>(p.dv + at)[v] = make_uint4(0, 0, 0, 0);
-      }
+      ++live;
     }
+    // the stores of this warp complete before the CTA exits
+    if ((warp & 7) == 0 && lane == 0) bulk_wait_all0();
     __syncwarp();
   }
 
   tc_fence_before();
   __syncthreads();
   if (threadIdx.x == 0 && *abort_flag) publish_device_error(p.host_err, VLAK_ERR_DEVICE_TIMEOUT);
-  if (warp == kWarpMma) {
+  if (warp == kWarpAccum) {
     tc_fence_after();
     tmem_dealloc(tmem, kTmemCols);
   }
@@ -757,27 +813,26 @@ SubTiling sub_tiling(int G, int M) {
   return best;
 }
 
+// workspace: statistics of the sub-tiles, then the item counter
 int64_t stats_bytes(const vlak_attn_gqa_args* a) {
   const SubTiling t = sub_tiling(static_cast<int>(a->H / a->Hkv), static_cast<int>(a->M));
   return a->B * a->Hkv * t.n_sub * kStatBytes;
 }
+constexpr int64_t kCounterBytes = 256;
 
 template <int kMode>
-cudaError_t launch_both(const BwdParams& p, unsigned n_dq, unsigned n_dkv, cudaStream_t cs, int device) {
+cudaError_t launch_both(const BwdParams& p, unsigned n_stats, unsigned grid, cudaStream_t cs, int device) {
   static std::atomic<int> ready[64];
   if (ready[device].load() == 0) {
-    cudaError_t e = cudaFuncSetAttribute(attn_bwd_dq<kMode>,
-                                         cudaFuncAttributeMaxDynamicSharedMemorySize, kDqSmem);
-    if (e == cudaSuccess)
-      e = cudaFuncSetAttribute(attn_bwd_dkv<kMode>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                               kDkvSmem);
+    cudaError_t e = cudaFuncSetAttribute(attn_bwd<kMode>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         kSmem);
     if (e != cudaSuccess) return e;
     ready[device].store(1);
   }
-  attn_bwd_dq<kMode><<<n_dq, kThreads, kDqSmem, cs>>>(p);
+  attn_bwd_stats<<<n_stats, kStatThreads, 0, cs>>>(p);
   cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess || n_dkv == 0) return e;
-  attn_bwd_dkv<kMode><<<n_dkv, kThreads, kDkvSmem, cs>>>(p);
+  if (e != cudaSuccess) return e;
+  attn_bwd<kMode><<<grid, kThreads, kSmem, cs>>>(p);
   return cudaGetLastError();
 }
 
@@ -834,7 +889,7 @@ int run_bwd(const vlak_attn_train_args* t, void* workspace, int64_t ws_bytes, vo
   }
   if (!a->q || !a->k || !a->v || !a->o || !args.grad_o || !args.lse)
     return set_error(VLAK_ERR_INVALID_ARGUMENT, "fused_attention_gqa_bwd: null tensor pointer");
-  if (!workspace || ws_bytes < stats_bytes(a))
+  if (!workspace || ws_bytes < stats_bytes(a) + kCounterBytes)
     return set_error(VLAK_ERR_INVALID_ARGUMENT, "fused_attention_gqa_bwd: workspace missing or too small");
   if (reinterpret_cast<uintptr_t>(workspace) % 256 != 0)
     return set_error(VLAK_ERR_ALIGNMENT, "fused_attention_gqa_bwd: workspace must be 256-byte aligned");
@@ -863,10 +918,16 @@ int run_bwd(const vlak_attn_train_args* t, void* workspace, int64_t ws_bytes, vo
   p.n_pair = (tl.n_sub + 1) / 2;
   p.n_kblk = (p.N + kKeys - 1) / kKeys;
   p.n_chunks = (p.N + kChunk - 1) / kChunk;
-  const int64_t n_dq = a->B * a->Hkv * p.n_pair;
-  const int64_t n_dkv = keys_too ? a->B * a->Hkv * p.n_kblk : 0;
-  if (n_dq > INT32_MAX || n_dkv > INT32_MAX)
+  const int64_t n_bk = a->B * a->Hkv, n_dq = n_bk * p.n_pair;
+  const int64_t n_dkv = keys_too ? n_bk * p.n_kblk : 0;
+  if (n_dq + n_dkv > INT32_MAX - 4096 || n_bk * p.n_sub > INT32_MAX)
     return set_error(VLAK_ERR_INVALID_ARGUMENT, "fused_attention_gqa_bwd: too many work items");
+  p.n_bk = static_cast<int>(n_bk);
+  p.n_dkv = static_cast<int>(n_dkv);
+  p.n_items = static_cast<int>(n_dkv + n_dq);
+  // Few heads: all their long items first, for balance, their tensors stay in
+  // L2. Many: a head's items one after the other, while its tensors are there.
+  p.bk_inner = n_bk <= 2 * dev.sm_count;
   p.P = static_cast<int>(P);
   p.ds = static_cast<int>(a->dead_start);
   p.de = static_cast<int>(a->dead_end);
@@ -876,6 +937,13 @@ int run_bwd(const vlak_attn_train_args* t, void* workspace, int64_t ws_bytes, vo
   p.host_err = host_error_word(cs);
   p.lse = args.lse;
   p.stats = static_cast<float*>(workspace);
+  p.counter = reinterpret_cast<unsigned*>(static_cast<uint8_t*>(workspace) + stats_bytes(a));
+  p.o = static_cast<const __nv_bfloat16*>(a->o);
+  p.d_o = static_cast<const __nv_bfloat16*>(args.grad_o);
+  for (int d = 0; d < 3; ++d) {
+    p.o_s[d] = a->o_stride[d];
+    p.do_s[d] = args.grad_o_stride[d];
+  }
   p.dq = static_cast<__nv_bfloat16*>(args.dq);
   p.dk = static_cast<__nv_bfloat16*>(args.dk);
   p.dv = static_cast<__nv_bfloat16*>(args.dv);
@@ -896,7 +964,6 @@ int run_bwd(const vlak_attn_train_args* t, void* workspace, int64_t ws_bytes, vo
   };
   const int64_t qs[3] = {a->M * a->H * 64, a->H * 64, 64}, ks[3] = {a->N * a->Hkv * 64, a->Hkv * 64, 64};
   st = rows(&p.tm_q, a->q, a->q_stride, "q");
-  if (st == VLAK_OK) st = rows(&p.tm_o, a->o, a->o_stride, "o");
   if (st == VLAK_OK) st = rows(&p.tm_do, args.grad_o, args.grad_o_stride, "grad_o");
   if (st == VLAK_OK) st = rows(&p.tm_dq, args.dq, qs, "dq");
   if (st == VLAK_OK) st = keys(&p.tm_k64, a->k, a->k_stride, kChunk, "k");
@@ -908,10 +975,11 @@ int run_bwd(const vlak_attn_train_args* t, void* workspace, int64_t ws_bytes, vo
   if (keys_too && st == VLAK_OK) st = keys(&p.tm_dv, args.dv, ks, kKeys, "dv");
   if (st != VLAK_OK) return st;
 
-  const unsigned g_dq = static_cast<unsigned>(n_dq), g_dkv = static_cast<unsigned>(n_dkv);
-  cudaError_t e = args.lengths ? launch_both<kMaskLength>(p, g_dq, g_dkv, cs, dev.device)
-                  : args.mask  ? launch_both<kMaskBool>(p, g_dq, g_dkv, cs, dev.device)
-                               : launch_both<kMaskAnalytic>(p, g_dq, g_dkv, cs, dev.device);
+  const unsigned n_stats = static_cast<unsigned>(n_bk * p.n_sub);
+  const unsigned grid = static_cast<unsigned>(std::min(p.n_items, dev.sm_count));
+  cudaError_t e = args.lengths ? launch_both<kMaskLength>(p, n_stats, grid, cs, dev.device)
+                  : args.mask  ? launch_both<kMaskBool>(p, n_stats, grid, cs, dev.device)
+                               : launch_both<kMaskAnalytic>(p, n_stats, grid, cs, dev.device);
   if (e != cudaSuccess) return set_cuda_error("fused_attention_gqa_bwd launch failed", e);
   return VLAK_OK;
 }
@@ -942,7 +1010,8 @@ extern "C" int vlak_attn_gqa_bwd_workspace_size(const vlak_attn_train_args* args
   }
   int st = vlak_attn_gqa_check(&a, nullptr, nullptr);
   if (st != VLAK_OK) return st;
-  if (args->attn.B > 0 && args->attn.M > 0 && args->attn.N > 0) *bytes = stats_bytes(&args->attn);
+  if (args->attn.B > 0 && args->attn.M > 0 && args->attn.N > 0) 
+    *bytes = stats_bytes(&args->attn) + kCounterBytes;
   return VLAK_OK;
 }
 
