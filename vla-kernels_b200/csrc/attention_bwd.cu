@@ -123,10 +123,9 @@ __device__ __forceinline__ uint32_t low_bits(int n) {
   return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : ((1u << n) - 1u);
 }
 
-// TMEM column of the k-th 16 of a step's 64 bf16 operands: each half of them is
-// packed over the first half of the 32 fp32 columns it was computed from, which
-// the warp that packs them has read.
-__device__ __forceinline__ uint32_t packed_col(int k) { return (k >> 1) * 32 + (k & 1) * 8; }
+// A step's 64 bf16 operand columns: each half of them is packed over the first
+// half of the 32 fp32 columns it was computed from, which the warp that packs
+// them has read; so they lie at columns 0-15 and 32-47 (see umma_ts_x4).
 
 // 1024-byte aligned start of the dynamic shared memory
 __device__ __forceinline__ uint8_t* aligned_smem(uint8_t* raw) {
@@ -150,35 +149,40 @@ __device__ __forceinline__ SubRow sub_row(const BwdParams& p, int st, int row) {
 }
 
 // ---------------------------------------------------------------------------
-// D = rowsum(dO * O) and -lse by sub-tile rows: eight threads per row, 16 bytes
-// each. Rows that do not exist or see no key get -lse = -inf (every P is 0) and
-// D = 0, whatever memory holds there. Bound: HBM, one read of O and dO.
-constexpr int kStatThreads = 512;
+// D = rowsum(dO * O) and -lse by sub-tile rows: four threads per row, two 16-byte
+// vectors of each tensor per thread. Rows that do not exist or see no key get
+// -lse = -inf (every P is 0) and D = 0, whatever memory holds there. Bound: HBM,
+// one read of O and dO.
+constexpr int kStatThreads = 4 * kSub;
 __global__ void __launch_bounds__(kStatThreads) attn_bwd_stats(const __grid_constant__ BwdParams p) {
+  // the main kernel may set itself up meanwhile; it waits for this grid's end
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (blockIdx.x == 0 && threadIdx.x == 0) *p.counter = 0u;
   const int bk = blockIdx.x / p.n_sub, st = blockIdx.x - bk * p.n_sub;
   const int b = bk / p.Hkv, kvh = bk - b * p.Hkv;
-  const int row = threadIdx.x >> 3, v = threadIdx.x & 7;
+  const int row = threadIdx.x >> 2, v = threadIdx.x & 3;
   const SubRow r = sub_row(p, st, row);
   const int h = kvh * p.G + r.g;
   float nl = -INFINITY, d = 0.f;
   if (r.valid) {
     const float lse = p.lse[(static_cast<long long>(b) * p.M + r.m) * p.H + h];
+    const uint4* x = reinterpret_cast<const uint4*>(p.o + b * p.o_s[0] + r.m * p.o_s[1] + h * p.o_s[2]);
+    const uint4* y = reinterpret_cast<const uint4*>(p.d_o + b * p.do_s[0] + r.m * p.do_s[1] + h * p.do_s[2]);
+    const uint4 xv[2] = {x[v], x[v + 4]}, yv[2] = {y[v], y[v + 4]};
     if (lse != -INFINITY) {
       nl = -lse;
-      const uint4 x = *reinterpret_cast<const uint4*>(p.o + b * p.o_s[0] + r.m * p.o_s[1] +
-                                                      h * p.o_s[2] + v * 8);
-      const uint4 y = *reinterpret_cast<const uint4*>(p.d_o + b * p.do_s[0] + r.m * p.do_s[1] +
-                                                      h * p.do_s[2] + v * 8);
-      float fx[8], fy[8];
-      Elem<__nv_bfloat16>::unpack(x, fx);
-      Elem<__nv_bfloat16>::unpack(y, fy);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) d += fx[i] * fy[i];
+      for (int k = 0; k < 2; ++k) {
+        float fx[8], fy[8];
+        Elem<__nv_bfloat16>::unpack(xv[k], fx);
+        Elem<__nv_bfloat16>::unpack(yv[k], fy);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) d += fx[i] * fy[i];
+      }
     }
   }
 #pragma unroll
-  for (int o = 1; o < 8; o <<= 1) d += __shfl_xor_sync(kFullMask, d, o);
+  for (int o = 1; o < 4; o <<= 1) d += __shfl_xor_sync(kFullMask, d, o);
   if (v == 0) {
     float* stat = p.stats + static_cast<long long>(blockIdx.x) * kStatFloats;
     stat[row] = nl;
@@ -304,6 +308,53 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
       : "memory");
 }
 
+// The four K = 16 products of one 64-deep contraction, from one elected lane.
+// Descriptors step by 32 bytes of a swizzled row (SS, both operands) or by 16
+// rows of 128 bytes (TS, B).
+__device__ __forceinline__ void umma_ss_x4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc) {
+  asm volatile(
+      "{\n\t.reg .pred e, n, y;\n\t.reg .b64 a1, a2, a3, b1, b2, b3;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "setp.ne.b32 n, 0, 0;\n\tsetp.eq.b32 y, 0, 0;\n\t"
+      "add.s64 a1, %1, 2;\n\tadd.s64 a2, %1, 4;\n\tadd.s64 a3, %1, 6;\n\t"
+      "add.s64 b1, %2, 2;\n\tadd.s64 b2, %2, 4;\n\tadd.s64 b3, %2, 6;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, n;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a1, b1, %3, y;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a2, b2, %3, y;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a3, b3, %3, y;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc)
+      : "memory");
+}
+// A in TMEM at columns x + 0, 8, 32, 40; `acc` 0 starts a new sum; `on` 0
+// issues nothing.
+__device__ __forceinline__ void umma_ts_x4(uint32_t d, uint32_t x, uint64_t b, uint32_t idesc,
+                                           uint32_t acc, uint32_t on) {
+  asm volatile(
+      "{\n\t.reg .pred e, q, p, y;\n\t.reg .b32 x1, x2, x3;\n\t.reg .b64 b1, b2, b3;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "setp.ne.and.b32 q, %5, 0, e;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\tsetp.eq.b32 y, 0, 0;\n\t"
+      "add.s32 x1, %1, 8;\n\tadd.s32 x2, %1, 32;\n\tadd.s32 x3, %1, 40;\n\t"
+      "add.s64 b1, %2, 128;\n\tadd.s64 b2, %2, 256;\n\tadd.s64 b3, %2, 384;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [x1], b1, %3, y;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [x2], b2, %3, y;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [x3], b3, %3, y;\n\t}" ::"r"(d),
+      "r"(x), "l"(b), "r"(idesc), "r"(acc), "r"(on)
+      : "memory");
+}
+// A counter modulo n with the parity of its rounds.
+template <int n>
+struct Turn {
+  uint32_t i = 0, round = 0;
+  __device__ __forceinline__ void next() {
+    if (++i == n) {
+      i = 0;
+      round ^= 1;
+    }
+  }
+};
+
 template <int kMode>
 __global__ void __launch_bounds__(kThreads, 1) attn_bwd(const __grid_constant__ BwdParams p) {
   extern __shared__ uint8_t smem_raw[];
@@ -361,7 +412,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd(const __grid_constant__ 
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = bars->tmem_base;
+  // an allocation of all 512 columns starts at the first; as a constant, it keeps
+  // the issue warps' operands uniform
+  constexpr uint32_t tmem = 0;
 
   // The n-th item handed out (live < 0: no more); every warp but the producer
   // takes each once.
@@ -370,15 +423,18 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd(const __grid_constant__ 
     if (!__all_sync(kFullMask, bounded_wait<1>(&bars->it_full[q], (n / kQueue) & 1, abort_flag)))
       return false;
     const int4* src = reinterpret_cast<const int4*>(&bars->item[q]);
-    int4* dst = reinterpret_cast<int4*>(&it);
-#pragma unroll
-    for (int i = 0; i < 3; ++i) dst[i] = src[i];
+    const int4 x = src[0], y = src[1], z = src[2];
+    it.live = x.x; it.dkv = x.y; it.b = x.z; it.kvh = x.w;
+    it.L = y.x; it.k0 = y.y; it.s0 = y.z; it.n_here = y.w;
+    it.a1 = z.x; it.b0 = z.y; it.mt_lo = z.z; it.mt_hi = z.w;
     __syncwarp();
     mbar_arrive_elect(&bars->it_empty[q]);
     return true;
   };
 
   if (warp == kWarpProducer) {
+    // the statistics and the counter are those of the kernel before
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     uint32_t t = 0, live = 0;  // steps and live items issued
     bool ok = true;
     for (uint32_t n = 0; ok; ++n) {
@@ -461,50 +517,51 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd(const __grid_constant__ 
     // T0 = A0 B0^T and T1 = A1 B1^T of every step, up to kStages steps (and one
     // item, by the stationary tiles) ahead of the accumulating products.
     const uint32_t id_kk = idesc_bf16_f32(128, 64, false);
-    uint32_t t = 0, live = 0;
+    const uint64_t a_desc = sdesc_sw128(smem_u32(a_smem)), b_desc = sdesc_sw128(smem_u32(b_smem));
+    // streamed rows that meet X = 0 only, and may hold NaN, are cleared: keys
+    // that no query sees (dq), query rows past L (dkv)
+    const bool dead = kMode == kMaskLength || (kMode == kMaskAnalytic && p.ds < p.de);
+    Turn<2> ab;
+    Turn<kRing> s;
+    Turn<kStages> st;
     bool ok = true;
     for (uint32_t n = 0; ok; ++n) {
       Item it;
       if (!take_item(n, it) || it.live < 0) break;
       if (it.live == 0) continue;
-      const uint32_t ab = live & 1;
-      if (!__all_sync(kFullMask, bounded_wait<1>(&bars->a_full[ab], (live >> 1) & 1, abort_flag))) break;
-      ++live;
-      // descriptors step by 16 of the 64 columns: 32 bytes of a swizzled row
-      const uint64_t a0 = sdesc_sw128(smem_u32(a_smem + ab * 4 * kSubBytes));
-      const uint64_t a1 = a0 + 2 * kSubBytes / 16;
+      if (!__all_sync(kFullMask, bounded_wait<1>(&bars->a_full[ab.i], ab.round, abort_flag))) break;
+      const uint64_t a0 = a_desc + ab.i * (4 * kSubBytes / 16), a1 = a0 + 2 * kSubBytes / 16;
+      ab.next();
       Steps step;
       step.begin(it);
-      for (int j = 0; j < it.live; ++j, ++t, step.next(it)) {
-        const uint32_t s = t % kRing, st = t % kStages;
-        if (!__all_sync(kFullMask,
-                        bounded_wait<1>(&bars->t_empty[st], ((t / kStages) & 1) ^ 1, abort_flag) &&
-                            bounded_wait<1>(&bars->b_full[s], (t / kRing) & 1, abort_flag))) {
+      for (int j = 0; j < it.live; ++j) {
+        if (!__all_sync(kFullMask, bounded_wait<1>(&bars->t_empty[st.i], st.round ^ 1, abort_flag) &&
+                                       bounded_wait<1>(&bars->b_full[s.i], s.round, abort_flag))) {
           ok = false;
           break;
         }
-        uint8_t* bp = b_smem + s * 2 * kSubBytes;
-        // streamed rows that meet X = 0 only, and may hold NaN: keys that no
-        // query sees (dq), query rows past L (dkv)
-        if (kMode != kMaskBool && !it.dkv) {
-          const int c0 = step.pos * kChunk;
-          const int lo = kMode == kMaskLength ? it.L - c0 : p.ds - c0;
-          const int hi = kMode == kMaskLength ? kChunk : p.de - c0;
-          clear_rows(bp, max(lo, 0), min(hi, kChunk));
-        }
-        if (kMode == kMaskLength && it.dkv) {
-          const int lo = max(0, it.L - step.pos * p.MT) * p.Gb;
-          clear_rows(bp, lo, kSub);
-          clear_rows(bp + kSubBytes, lo, kSub);
+        if (dead) {
+          uint8_t* bp = b_smem + s.i * 2 * kSubBytes;
+          if (!it.dkv) {
+            const int c0 = step.pos * kChunk;
+            const int lo = kMode == kMaskLength ? it.L - c0 : p.ds - c0;
+            const int hi = kMode == kMaskLength ? kChunk : p.de - c0;
+            clear_rows(bp, max(lo, 0), min(hi, kChunk));
+          } else if (kMode == kMaskLength) {
+            const int lo = max(0, it.L - step.pos * p.MT) * p.Gb;
+            clear_rows(bp, lo, kSub);
+            clear_rows(bp + kSubBytes, lo, kSub);
+          }
+          step.next(it);
         }
         tc_fence_after();
-        const uint64_t b0 = sdesc_sw128(smem_u32(bp)), b1 = b0 + kSubBytes / 16;
-        const uint32_t d = tmem + kStage0 + st * kStageCols;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) umma_ss_elect(d, a0 + 2 * k, b0 + 2 * k, id_kk, k > 0);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) umma_ss_elect(d + kT1, a1 + 2 * k, b1 + 2 * k, id_kk, k > 0);
-        umma_commit_elect(&bars->s_full[st]);
+        const uint64_t b0 = b_desc + s.i * (2 * kSubBytes / 16);
+        const uint32_t d = tmem + kStage0 + st.i * kStageCols;
+        umma_ss_x4(d, a0, b0, id_kk);
+        umma_ss_x4(d + kT1, a1, b0 + kSubBytes / 16, id_kk);
+        umma_commit_elect(&bars->s_full[st.i]);
+        s.next();
+        st.next();
       }
     }
     // every issued product completes before TMEM is released
@@ -514,36 +571,33 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd(const __grid_constant__ 
   } else if (warp == kWarpAccum) {
     // acc1 += X1 B0, and acc0 += X0 B1 of a dkv item.
     const uint32_t id_kn = idesc_bf16_f32(128, 64, true);
-    uint32_t t = 0, live = 0;
+    const uint64_t b_desc = sdesc_sw128(smem_u32(b_smem));
+    Turn<kRing> s;
+    Turn<kStages> st;
+    uint32_t live = 0;
     bool ok = true;
     for (uint32_t n = 0; ok; ++n) {
       Item it;
       if (!take_item(n, it) || it.live < 0) break;
       if (it.live == 0) continue;
-      for (int j = 0; j < it.live; ++j, ++t) {
-        const uint32_t s = t % kRing, st = t % kStages;
-        // the step's X, and at an item's first step the previous item's
-        // accumulators read
-        if (!__all_sync(kFullMask,
-                        (j > 0 || live == 0 ||
-                         bounded_wait<1>(&bars->acc_empty, (live - 1) & 1, abort_flag)) &&
-                            bounded_wait<1>(&bars->x_full[st], (t / kStages) & 1, abort_flag))) {
+      // the previous item's accumulators have been read
+      if (live > 0 &&
+          !__all_sync(kFullMask, bounded_wait<1>(&bars->acc_empty, (live - 1) & 1, abort_flag)))
+        break;
+      for (int j = 0; j < it.live; ++j) {
+        if (!__all_sync(kFullMask, bounded_wait<1>(&bars->x_full[st.i], st.round, abort_flag))) {
           ok = false;
           break;
         }
         tc_fence_after();
-        const uint64_t b0 = sdesc_sw128(smem_u32(b_smem + s * 2 * kSubBytes)), b1 = b0 + kSubBytes / 16;
-        const uint32_t x = tmem + kStage0 + st * kStageCols;
-#pragma unroll
-        for (int k = 0; k < 4; ++k)  // dV += P^T dO: 16 rows are 2 KB
-          umma_ts_elect(tmem + kAcc0, x + packed_col(k), b1 + 128 * k, id_kn,
-                        (j > 0 || k > 0) ? 1u : 0u, it.dkv);
-#pragma unroll
-        for (int k = 0; k < 4; ++k)  // dK += dS^T Q, dQ += dS K
-          umma_ts_elect(tmem + kAcc1, x + kT1 + packed_col(k), b0 + 128 * k, id_kn,
-                        (j > 0 || k > 0) ? 1u : 0u);
-        umma_commit_elect(&bars->b_empty[s]);
-        umma_commit_elect(&bars->t_empty[st]);
+        const uint64_t b0 = b_desc + s.i * (2 * kSubBytes / 16);
+        const uint32_t x = tmem + kStage0 + st.i * kStageCols;
+        umma_ts_x4(tmem + kAcc0, x, b0 + kSubBytes / 16, id_kn, j > 0, it.dkv);  // dV += P^T dO
+        umma_ts_x4(tmem + kAcc1, x + kT1, b0, id_kn, j > 0, 1u);  // dK += dS^T Q, dQ += dS K
+        umma_commit_elect(&bars->t_empty[st.i]);
+        umma_commit_elect(&bars->b_empty[s.i]);
+        s.next();
+        st.next();
       }
       if (!ok) break;
       umma_commit_elect(&bars->out_full[live & 1]);
@@ -614,11 +668,17 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd(const __grid_constant__ 
         }
         if (kMode == kMaskBool && valid) mrow = p.mask + it.b * p.mask_sb + r.m * p.mask_sm;
       }
+      // the warp's extremes, to class a step's columns without looking at lanes
+      // (lanes without a key or row do not count)
+      const int from_hi = __reduce_max_sync(kFullMask, valid ? from : INT32_MIN / 2);
+      const int from_lo = __reduce_min_sync(kFullMask, valid ? from : INT32_MAX / 2);
+      const int to_lo = __reduce_min_sync(kFullMask, valid ? to : INT32_MAX / 2);
+      const int to_hi = __reduce_max_sync(kFullMask, valid ? to : INT32_MIN / 2);
       uint64_t nl2 = 0ull, nD2 = 0ull;
       bool first = !it.dkv;
       Steps step;
       step.begin(it);
-      for (int j = 0; ok && j < it.live; ++j, ++t, step.next(it)) {
+      for (int j = 0; j < it.live; ++j, ++t, step.next(it)) {
         if (static_cast<int>(t & 1) != group) continue;
         if (first) {
           // the row's statistics (only with a step to do: a group without one
@@ -633,34 +693,36 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd(const __grid_constant__ 
           first = false;
         }
         const uint32_t st = t % kStages, s = t % kRing;
-        // which of the warp's 32 columns this lane sees
+        // Which of the warp's 32 columns this lane sees. dkv: columns lo to hi
+        // see the key (rows past M or the box have -lse = -inf: their P is 0
+        // without a mask); dq: keys below `from` and from `mid` to `to`.
+        const int c0 = it.dkv ? step.pos * p.MT : step.pos * kChunk + 32 * gq;
         uint32_t vm = 0u;
-        if (it.dkv) {
-          // (rows past M or the box have -lse = -inf: their P is 0 unmasked)
-          const int m0 = step.pos * p.MT;
-          if (kMode == kMaskBool) {
-            if (valid) {
-              const uint64_t heads = ~0ull >> (64 - p.Gb);
-              const int rows = min(p.MT, p.M - m0);
-              for (int i = 0; i < rows; ++i)
-                if (__ldg(mrow + static_cast<long long>(m0 + i) * p.mask_sm) != 0)
-                  vm |= static_cast<uint32_t>((heads << (i * p.Gb)) >> (32 * gq));
-            }
-          } else {
-            const int lo = min(max(from - m0, 0), kSub) * p.Gb - 32 * gq;
-            const int hi = min(max(to - m0, 0), kSub) * p.Gb - 32 * gq;
-            vm = ~low_bits(lo) & (to >= p.M ? 0xffffffffu : low_bits(hi));
+        bool full, none;
+        if (kMode == kMaskBool) {
+          if (it.dkv && valid) {
+            const uint64_t heads = ~0ull >> (64 - p.Gb);
+            const int rows = min(p.MT, p.M - c0);
+            for (int i = 0; i < rows; ++i)
+              if (__ldg(mrow + static_cast<long long>(c0 + i) * p.mask_sm) != 0)
+                vm |= static_cast<uint32_t>((heads << (i * p.Gb)) >> (32 * gq));
+          } else if (!it.dkv && valid && c0 < p.N) {
+            vm = mask_bits32(mrow, c0, p.N, p.mask_words);
           }
+          full = __all_sync(kFullMask, !valid || vm == 0xffffffffu);
+          none = __all_sync(kFullMask, !valid || vm == 0u);
+        } else if (it.dkv) {
+          auto column = [&](int m) { return min(max(m - c0, 0), kSub) * p.Gb - 32 * gq; };
+          full = column(from_hi) <= 0 && (to_lo >= p.M || column(to_lo) >= 32);
+          none = column(from_lo) >= 32 || column(to_hi) <= 0;
+          if (!full && !none)
+            vm = ~low_bits(column(from)) & (to >= p.M ? 0xffffffffu : low_bits(column(to)));
         } else {
-          const int g0 = step.pos * kChunk + 32 * gq;
-          if (kMode == kMaskBool) {
-            if (mrow != nullptr && g0 < p.N) vm = mask_bits32(mrow, g0, p.N, p.mask_words);
-          } else {
-            vm = low_bits(from - g0) | (low_bits(to - g0) & ~low_bits(mid - g0));
-          }
+          full = c0 + 32 <= from || (c0 >= mid && c0 + 32 <= to_lo);
+          none = c0 >= from && (c0 + 32 <= mid || c0 >= to_hi);
+          if (!full && !none)
+            vm = low_bits(from - c0) | (low_bits(to - c0) & ~low_bits(mid - c0));
         }
-        const bool full = __all_sync(kFullMask, !valid || vm == 0xffffffffu);
-        const bool none = __all_sync(kFullMask, !valid || vm == 0u);
         // A group sees every phase of its ring slots (kRing is even), and a
         // stage's skipped phase completes before the step it sees in between.
         if ((it.dkv && !__all_sync(kFullMask, bounded_wait<1>(&bars->b_full[s], (t / kRing) & 1, abort_flag))) ||
@@ -791,7 +853,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd(const __grid_constant__ 
   if (threadIdx.x == 0 && *abort_flag) publish_device_error(p.host_err, VLAK_ERR_DEVICE_TIMEOUT);
   if (warp == kWarpAccum) {
     tc_fence_after();
-    tmem_dealloc(tmem, kTmemCols);
+    tmem_dealloc(bars->tmem_base, kTmemCols);
   }
 }
 
@@ -832,8 +894,18 @@ cudaError_t launch_both(const BwdParams& p, unsigned n_stats, unsigned grid, cud
   attn_bwd_stats<<<n_stats, kStatThreads, 0, cs>>>(p);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
-  attn_bwd<kMode><<<grid, kThreads, kSmem, cs>>>(p);
-  return cudaGetLastError();
+  // programmatic dependent launch: set up while the statistics are computed
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kSmem;
+  cfg.stream = cs;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, attn_bwd<kMode>, p);
 }
 
 int bwd_validate(const vlak_attn_train_args* a, int64_t* P, float* scale) {
