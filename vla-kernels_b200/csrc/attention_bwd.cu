@@ -79,7 +79,12 @@ constexpr int kComputeWarps = 2 * kGroupWarps;
 // took about 1.6K cycles per step for both, three times the products' own time.
 constexpr int kWarpProducer = kComputeWarps, kWarpScores = kComputeWarps + 1,
               kWarpAccum = kComputeWarps + 2;
-constexpr int kThreads = 32 * (kComputeWarps + 3);
+constexpr int kThreads = 32 * (kComputeWarps + 4);  // (the last warp has no role)
+// Registers: a compute thread wants more than an even share, the others less.
+constexpr int kRegsLaunch = 96, kRegsCompute = 104, kRegsOther = 64;
+static_assert(32 * kComputeWarps * kRegsCompute + (kThreads - 32 * kComputeWarps) * kRegsOther <=
+                  kThreads * kRegsLaunch,
+              "the split must fit the launch's registers");
 
 // TMEM columns: accumulators, then the stages; X0 and X1 (bf16 pairs) overwrite
 // parts of T0 and T1
@@ -355,6 +360,11 @@ struct Turn {
   }
 };
 
+// (each of the four warps of the last warpgroup)
+__device__ __forceinline__ void less_registers() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
+}
+
 template <int kMode>
 __global__ void __launch_bounds__(kThreads, 1) attn_bwd(const __grid_constant__ BwdParams p) {
   extern __shared__ uint8_t smem_raw[];
@@ -433,6 +443,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd(const __grid_constant__ 
   };
 
   if (warp == kWarpProducer) {
+    less_registers();
     // the statistics and the counter are those of the kernel before
     asm volatile("griddepcontrol.wait;" ::: "memory");
     uint32_t t = 0, live = 0;  // steps and live items issued
@@ -514,6 +525,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd(const __grid_constant__ 
       bounded_wait(&bars->b_full[k % kRing], (k / kRing) & 1, abort_flag, false);
     __syncwarp();
   } else if (warp == kWarpScores) {
+    less_registers();
     // T0 = A0 B0^T and T1 = A1 B1^T of every step, up to kStages steps (and one
     // item, by the stationary tiles) ahead of the accumulating products.
     const uint32_t id_kk = idesc_bf16_f32(128, 64, false);
@@ -569,6 +581,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd(const __grid_constant__ 
     bounded_wait(&bars->drain[0], 0, abort_flag, false);
     __syncwarp();
   } else if (warp == kWarpAccum) {
+    less_registers();
     // acc1 += X1 B0, and acc0 += X0 B1 of a dkv item.
     const uint32_t id_kn = idesc_bf16_f32(128, 64, true);
     const uint64_t b_desc = sdesc_sw128(smem_u32(b_smem));
@@ -606,7 +619,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd(const __grid_constant__ 
     umma_commit_elect(&bars->drain[1]);
     bounded_wait(&bars->drain[1], 0, abort_flag, false);
     __syncwarp();
-  } else {
+  } else if (warp < kComputeWarps) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsCompute));
     // Compute warps. A step belongs to the group of its parity, an item's
     // output to the group of the item's.
     const int group = warp >> 3, quarter = warp & 3, gq = (warp >> 2) & 1;
@@ -668,110 +682,140 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd(const __grid_constant__ 
         }
         if (kMode == kMaskBool && valid) mrow = p.mask + it.b * p.mask_sb + r.m * p.mask_sm;
       }
-      // the warp's extremes, to class a step's columns without looking at lanes
-      // (lanes without a key or row do not count)
-      const int from_hi = __reduce_max_sync(kFullMask, valid ? from : INT32_MIN / 2);
-      const int from_lo = __reduce_min_sync(kFullMask, valid ? from : INT32_MAX / 2);
-      const int to_lo = __reduce_min_sync(kFullMask, valid ? to : INT32_MAX / 2);
-      const int to_hi = __reduce_max_sync(kFullMask, valid ? to : INT32_MIN / 2);
-      uint64_t nl2 = 0ull, nD2 = 0ull;
-      bool first = !it.dkv;
-      Steps step;
-      step.begin(it);
-      for (int j = 0; j < it.live; ++j, ++t, step.next(it)) {
-        if (static_cast<int>(t & 1) != group) continue;
-        if (first) {
-          // the row's statistics (only with a step to do: a group without one
-          // may come here after the tiles have been replaced)
-          if (!__all_sync(kFullMask, bounded_wait<1>(&bars->a_full[ab], (live >> 1) & 1, abort_flag))) {
-            ok = false;
-            break;
-          }
-          const float* stat = a_stat + (ab * 2 + (quarter >> 1)) * kStatFloats + (quarter & 1) * 32 + lane;
-          nl2 = f2_pack(stat[0], stat[0]);
-          nD2 = f2_pack(stat[kSub], stat[kSub]);
-          first = false;
+      // A step's 32 columns of this warp, by their first key c (dq) or the
+      // sub-tile's first position c (dkv), are seen by all its lanes when
+      // c <= all_0 or all_1 <= c <= all_2, and by none when no_0 <= c <= no_1 or
+      // c >= no_2; lanes without a key or row do not count.
+      constexpr int kFar = INT32_MAX / 2;
+      int all_0 = -kFar, all_1 = 0, all_2 = 0, no_0 = -kFar, no_1 = 0, no_2 = 0;
+      if (kMode != kMaskBool) {
+        const int to_lo = __reduce_min_sync(kFullMask, valid ? to : kFar);
+        const int to_hi = __reduce_max_sync(kFullMask, valid ? to : -kFar);
+        if (it.dkv) {
+          // column of position m: (m - c) Gb - 32 gq
+          const int before = 32 * gq / p.Gb, past = (32 * gq + 32 + p.Gb - 1) / p.Gb;
+          all_1 = __reduce_max_sync(kFullMask, valid ? from : -kFar) - before;
+          all_2 = to_lo >= p.M ? kFar : to_lo - past;
+          no_1 = __reduce_min_sync(kFullMask, valid ? from : kFar) - past;
+          no_2 = to_hi - before;
+        } else {
+          all_0 = from - 32;
+          all_1 = mid;
+          all_2 = to_lo - 32;
+          no_0 = from;
+          no_1 = mid - 32;
+          no_2 = max(from, to_hi);
         }
-        const uint32_t st = t % kStages, s = t % kRing;
-        // Which of the warp's 32 columns this lane sees. dkv: columns lo to hi
-        // see the key (rows past M or the box have -lse = -inf: their P is 0
-        // without a mask); dq: keys below `from` and from `mid` to `to`.
-        const int c0 = it.dkv ? step.pos * p.MT : step.pos * kChunk + 32 * gq;
+      }
+      uint64_t nl2 = 0ull, nD2 = 0ull;
+      // this group's steps: every other one
+      const int j0 = static_cast<int>((t ^ group) & 1u);
+      if (!it.dkv && j0 < it.live) {
+        // the row's statistics (only with a step to do: a group without one may
+        // come here after the tiles have been replaced)
+        if (!__all_sync(kFullMask, bounded_wait<1>(&bars->a_full[ab], (live >> 1) & 1, abort_flag))) break;
+        const float* stat = a_stat + (ab * 2 + (quarter >> 1)) * kStatFloats + (quarter & 1) * 32 + lane;
+        nl2 = f2_pack(stat[0], stat[0]);
+        nD2 = f2_pack(stat[kSub], stat[kSub]);
+      }
+      const int per_head = it.mt_hi - it.mt_lo;  // position blocks of a head block (dkv)
+      int pos = it.mt_lo + j0;
+      for (int j = j0; j < it.live; j += 2, pos += 2) {
+        int c;
+        if (it.dkv) {
+          while (pos >= it.mt_hi) pos -= per_head;
+          c = pos * p.MT;
+        } else {
+          c = (j < it.a1 ? j : j - it.a1 + it.b0) * kChunk + 32 * gq;
+        }
+        // which of the columns this lane sees (dkv: rows past M or the box have
+        // -lse = -inf, so their P is 0 without a mask)
         uint32_t vm = 0u;
         bool full, none;
         if (kMode == kMaskBool) {
           if (it.dkv && valid) {
             const uint64_t heads = ~0ull >> (64 - p.Gb);
-            const int rows = min(p.MT, p.M - c0);
+            const int rows = min(p.MT, p.M - c);
             for (int i = 0; i < rows; ++i)
-              if (__ldg(mrow + static_cast<long long>(c0 + i) * p.mask_sm) != 0)
+              if (__ldg(mrow + static_cast<long long>(c + i) * p.mask_sm) != 0)
                 vm |= static_cast<uint32_t>((heads << (i * p.Gb)) >> (32 * gq));
-          } else if (!it.dkv && valid && c0 < p.N) {
-            vm = mask_bits32(mrow, c0, p.N, p.mask_words);
+          } else if (!it.dkv && valid && c < p.N) {
+            vm = mask_bits32(mrow, c, p.N, p.mask_words);
           }
           full = __all_sync(kFullMask, !valid || vm == 0xffffffffu);
           none = __all_sync(kFullMask, !valid || vm == 0u);
-        } else if (it.dkv) {
-          auto column = [&](int m) { return min(max(m - c0, 0), kSub) * p.Gb - 32 * gq; };
-          full = column(from_hi) <= 0 && (to_lo >= p.M || column(to_lo) >= 32);
-          none = column(from_lo) >= 32 || column(to_hi) <= 0;
-          if (!full && !none)
-            vm = ~low_bits(column(from)) & (to >= p.M ? 0xffffffffu : low_bits(column(to)));
         } else {
-          full = c0 + 32 <= from || (c0 >= mid && c0 + 32 <= to_lo);
-          none = c0 >= from && (c0 + 32 <= mid || c0 >= to_hi);
-          if (!full && !none)
-            vm = low_bits(from - c0) | (low_bits(to - c0) & ~low_bits(mid - c0));
+          full = c <= all_0 || (c >= all_1 && c <= all_2);
+          none = (c >= no_0 && c <= no_1) || c >= no_2;
+          if (!full && !none) {
+            if (it.dkv) {
+              auto column = [&](int m) { return min(max(m - c, 0), kSub) * p.Gb - 32 * gq; };
+              vm = ~low_bits(column(from)) & (to >= p.M ? 0xffffffffu : low_bits(column(to)));
+            } else {
+              vm = low_bits(from - c) | (low_bits(to - c) & ~low_bits(mid - c));
+            }
+          }
         }
+        const uint32_t tj = t + j, st = tj % kStages, s = tj % kRing;
         // A group sees every phase of its ring slots (kRing is even), and a
         // stage's skipped phase completes before the step it sees in between.
-        if ((it.dkv && !__all_sync(kFullMask, bounded_wait<1>(&bars->b_full[s], (t / kRing) & 1, abort_flag))) ||
-            !__all_sync(kFullMask, bounded_wait<1>(&bars->s_full[st], (t / kStages) & 1, abort_flag))) {
+        if (!__all_sync(kFullMask,
+                        (!it.dkv || bounded_wait<1>(&bars->b_full[s], (tj / kRing) & 1, abort_flag)) &&
+                            bounded_wait<1>(&bars->s_full[st], (tj / kStages) & 1, abort_flag))) {
           ok = false;
           break;
         }
         tc_fence_after();
         const uint32_t t0 = tbase + kStage0 + st * kStageCols + 32 * gq;
-        uint32_t pp[16], pd[16];
         if (none) {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) pp[i] = pd[i] = 0u;
+          const uint32_t zero[16] = {};
+          if (it.dkv) tmem_st16(t0, zero);
+          tmem_st16(t0 + kT1, zero);
         } else {
-          float sv[32], dp[32];
-          tmem_ld32(t0, sv);
-          tmem_ld32(t0 + kT1, dp);
-          tmem_wait_ld();
           const float4* stat = reinterpret_cast<const float4*>(b_stat + s * kStatFloats) + 8 * gq;
-          // four bodies: per-column or per-lane statistics, all shown or not
+          // Sixteen columns at a time, which keeps the step in registers. Four
+          // bodies: per-column or per-lane statistics, all shown or not.
           auto grads = [&](auto dkv, auto masked) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {  // four columns
-              uint64_t l2[2] = {nl2, nl2}, d2[2] = {nD2, nD2};
-              if (decltype(dkv)::value) {
-                const float4 l4 = stat[i], d4 = stat[16 + i];
-                l2[0] = f2_pack(l4.x, l4.y);
-                l2[1] = f2_pack(l4.z, l4.w);
-                d2[0] = f2_pack(d4.x, d4.y);
-                d2[1] = f2_pack(d4.z, d4.w);
-              }
+            for (int h = 0; h < 2; ++h) {
+              float sv[16], dp[16];
+              tmem_ld16(t0 + 16 * h, sv);
+              tmem_ld16(t0 + kT1 + 16 * h, dp);
+              tmem_wait_ld();
+              uint32_t pp[8], pd[8];
 #pragma unroll
-              for (int u = 0; u < 2; ++u) {
-                const int k = 2 * i + u;
-                float x0, x1, d0, d1;
-                f2_unpack(f2_fma(f2_pack(sv[2 * k], sv[2 * k + 1]), sl2, l2[u]), x0, x1);
-                float e0 = ex2(x0), e1 = ex2(x1);
-                f2_unpack(f2_mul(f2_pack(e0, e1),
-                                 f2_add(f2_pack(dp[2 * k], dp[2 * k + 1]), d2[u])), d0, d1);
-                if (decltype(masked)::value) {
-                  const bool see0 = (vm >> (2 * k)) & 1u, see1 = (vm >> (2 * k + 1)) & 1u;
-                  e0 = see0 ? e0 : 0.f;
-                  d0 = see0 ? d0 : 0.f;
-                  e1 = see1 ? e1 : 0.f;
-                  d1 = see1 ? d1 : 0.f;
+              for (int i = 0; i < 4; ++i) {  // four columns
+                uint64_t l2[2] = {nl2, nl2}, d2[2] = {nD2, nD2};
+                if (decltype(dkv)::value) {
+                  const float4 l4 = stat[4 * h + i], d4 = stat[16 + 4 * h + i];
+                  l2[0] = f2_pack(l4.x, l4.y);
+                  l2[1] = f2_pack(l4.z, l4.w);
+                  d2[0] = f2_pack(d4.x, d4.y);
+                  d2[1] = f2_pack(d4.z, d4.w);
                 }
-                if (decltype(dkv)::value) pp[k] = pack_bf16x2(e0, e1);
-                pd[k] = pack_bf16x2(d0, d1);
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                  const int k = 2 * i + u;
+                  float x0, x1, d0, d1;
+                  f2_unpack(f2_fma(f2_pack(sv[2 * k], sv[2 * k + 1]), sl2, l2[u]), x0, x1);
+                  float e0 = ex2(x0), e1 = ex2(x1);
+                  f2_unpack(f2_mul(f2_pack(e0, e1),
+                                   f2_add(f2_pack(dp[2 * k], dp[2 * k + 1]), d2[u])), d0, d1);
+                  if (decltype(masked)::value) {
+                    const uint32_t bits = vm >> (16 * h + 2 * k);
+                    e0 = bits & 1u ? e0 : 0.f;
+                    d0 = bits & 1u ? d0 : 0.f;
+                    e1 = bits & 2u ? e1 : 0.f;
+                    d1 = bits & 2u ? d1 : 0.f;
+                  }
+                  if (decltype(dkv)::value) pp[k] = pack_bf16x2(e0, e1);
+                  pd[k] = pack_bf16x2(d0, d1);
+                }
               }
+              // over the first half of the columns the warp has read: 8 of the
+              // 16 just loaded, then the next 8
+              if (decltype(dkv)::value) tmem_st8(t0 + 8 * h, pp);
+              tmem_st8(t0 + kT1 + 8 * h, pd);
             }
           };
           using Yes = std::true_type;
@@ -781,13 +825,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd(const __grid_constant__ 
           else
             full ? grads(No(), No()) : grads(No(), Yes());
         }
-        if (it.dkv) tmem_st16(t0, pp);
-        tmem_st16(t0 + kT1, pd);
         tmem_wait_st();
         tc_fence_before();
         mbar_arrive_elect(&bars->x_full[st]);
       }
       if (!ok) break;
+      t += it.live;
       if (static_cast<int>(ab) == group) {
         // Output: the accumulators, scaled, staged over the item's stationary
         // tiles in the swizzled layout of the maps, then TMA stores.
@@ -846,6 +889,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd(const __grid_constant__ 
     // the stores of this warp complete before the CTA exits
     if ((warp & 7) == 0 && lane == 0) bulk_wait_all0();
     __syncwarp();
+  } else {
+    less_registers();
   }
 
   tc_fence_before();
