@@ -66,8 +66,9 @@ constexpr int kSubBytes = kSub * kRowBytes;  // 8 KB
 constexpr int kChunk = 64;                   // keys of a dq step
 constexpr int kKeys = 128;                   // keys of a dkv item
 constexpr int kRing = 6;                     // streamed pairs in flight (even: see the compute warps)
+constexpr int kTiles = 3;                    // items whose stationary tiles are in shared memory
 constexpr int kStages = 3;                   // (T0, T1) pairs in TMEM
-constexpr int kQueue = 4;                    // items handed out and not yet seen by every warp
+constexpr int kQueue = 8;                    // items handed out and not yet seen by every warp
 constexpr int kStatFloats = 2 * kSub;        // -lse and -D of a sub-tile
 constexpr int kStatBytes = kStatFloats * 4;
 
@@ -77,11 +78,15 @@ constexpr int kGroupWarps = 8;
 constexpr int kComputeWarps = 2 * kGroupWarps;
 // One warp issues the scores, another the accumulating products: one alone
 // took about 1.6K cycles per step for both, three times the products' own time.
+// Four more, one per lane quarter, carry the outputs away, so that no compute
+// group pauses at an item's end (an item of three steps took twice as long
+// when the groups did it in turn).
 constexpr int kWarpProducer = kComputeWarps, kWarpScores = kComputeWarps + 1,
-              kWarpAccum = kComputeWarps + 2;
-constexpr int kThreads = 32 * (kComputeWarps + 4);  // (the last warp has no role)
+              kWarpAccum = kComputeWarps + 2;  // (kComputeWarps + 3 has no role)
+constexpr int kWarpOutput = kComputeWarps + 4, kOutputWarps = 4;
+constexpr int kThreads = 32 * (kWarpOutput + kOutputWarps);
 // Registers: a compute thread wants more than an even share, the others less.
-constexpr int kRegsLaunch = 96, kRegsCompute = 104, kRegsOther = 64;
+constexpr int kRegsLaunch = 80, kRegsCompute = 96, kRegsOther = 48;
 static_assert(32 * kComputeWarps * kRegsCompute + (kThreads - 32 * kComputeWarps) * kRegsOther <=
                   kThreads * kRegsLaunch,
               "the split must fit the launch's registers");
@@ -104,7 +109,7 @@ struct __align__(64) BwdParams {
   unsigned* counter;                         // next item
   int B, M, N, H, Hkv, G;
   int Gb, MT;                                // heads and positions of a sub-tile
-  int n_mt, n_sub, n_pair, n_kblk, n_chunks;
+  int n_mt, n_hblk, n_sub, n_pair, n_kblk, n_chunks;
   int n_bk, n_dkv, n_items;                  // B * Hkv; dkv items; all items
   int bk_inner;                              // items run over (b, kv head) first
   int P, ds, de;
@@ -115,6 +120,7 @@ struct __align__(64) BwdParams {
   const uint8_t* mask;
   long long mask_sb, mask_sm;
   int mask_words;
+  FastDiv by_bk, by_kblk, by_pair, by_hkv, by_mt_count, by_mt, by_gb;
 };
 
 __device__ __forceinline__ int length_of(const BwdParams& p, int b) {
@@ -144,8 +150,8 @@ struct SubRow {
   bool valid;
 };
 __device__ __forceinline__ SubRow sub_row(const BwdParams& p, int st, int row) {
-  const int hb = st / p.n_mt, mt = st - hb * p.n_mt;
-  const int local = row / p.Gb;
+  const int hb = fast_div(st, p.by_mt_count), mt = st - hb * p.n_mt;
+  const int local = fast_div(row, p.by_gb);
   SubRow r;
   r.m = mt * p.MT + local;
   r.g = hb * p.Gb + row - local * p.Gb;
@@ -164,7 +170,7 @@ __global__ void __launch_bounds__(kStatThreads) attn_bwd_stats(const __grid_cons
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (blockIdx.x == 0 && threadIdx.x == 0) *p.counter = 0u;
   const int bk = blockIdx.x / p.n_sub, st = blockIdx.x - bk * p.n_sub;
-  const int b = bk / p.Hkv, kvh = bk - b * p.Hkv;
+  const int b = fast_div(bk, p.by_hkv), kvh = bk - b * p.Hkv;
   const int row = threadIdx.x >> 2, v = threadIdx.x & 3;
   const SubRow r = sub_row(p, st, row);
   const int h = kvh * p.G + r.g;
@@ -233,19 +239,18 @@ struct Steps {
 };
 
 struct Barriers {
-  uint64_t a_full[2], a_empty[2];          // stationary tiles of an item
+  uint64_t a_full[kTiles], a_empty[kTiles];  // stationary tiles of an item
   uint64_t b_full[kRing], b_empty[kRing];  // streamed pairs
   uint64_t s_full[kStages], x_full[kStages], t_empty[kStages];
-  uint64_t out_full[2], staged[2];         // by the group that stores the item
-  uint64_t acc_empty, drain[2];
+  uint64_t out_full, staged, acc_empty, drain[2];
   uint64_t it_full[kQueue], it_empty[kQueue];
   Item item[kQueue];
   uint32_t tmem_base;
   int abort_flag;
 };
-constexpr int kBarrierBytes = 640;
+constexpr int kBarrierBytes = 896;
 static_assert(sizeof(Barriers) <= kBarrierBytes, "barrier block");
-constexpr int kSmem = 2 * 4 * kSubBytes + kRing * (2 * kSubBytes + kStatBytes) + 2 * 2 * kStatBytes +
+constexpr int kSmem = kTiles * 4 * kSubBytes + kRing * (2 * kSubBytes + kStatBytes) + kTiles * 2 * kStatBytes +
                       kBarrierBytes + 1024;
 static_assert(kSmem <= 227 * 1024, "shared memory");
 
@@ -254,12 +259,13 @@ __device__ __forceinline__ Item decode_item(const BwdParams& p, int id) {
   Item it{};
   it.dkv = id < p.n_dkv;
   const int i = it.dkv ? id : id - p.n_dkv;
-  const int inner = it.dkv ? p.n_kblk : p.n_pair;
   // blk: key block, or pair of sub-tiles counted from the last, whose rows see
   // the most keys under a staircase, as the first keys are seen by the most rows
-  const int blk = p.bk_inner ? i / p.n_bk : i % inner;
-  const int bk = p.bk_inner ? i - blk * p.n_bk : i / inner;
-  it.b = bk / p.Hkv;
+  const FastDiv& inner = it.dkv ? p.by_kblk : p.by_pair;
+  const int outer = fast_div(i, p.bk_inner ? p.by_bk : inner);
+  const int rest = i - outer * (p.bk_inner ? p.n_bk : static_cast<int>(inner.d));
+  const int blk = p.bk_inner ? outer : rest, bk = p.bk_inner ? rest : outer;
+  it.b = fast_div(bk, p.by_hkv);
   it.kvh = bk - it.b * p.Hkv;
   it.L = kMode == kMaskLength ? length_of(p, it.b) : 0;
   if (it.dkv) {
@@ -267,23 +273,27 @@ __device__ __forceinline__ Item decode_item(const BwdParams& p, int id) {
     it.k0 = blk * kKeys;
     int mt_lo = 0, mt_hi = p.n_mt;
     if (kMode == kMaskLength) {
-      mt_hi = it.k0 < it.L ? min(p.n_mt, (it.L + p.MT - 1) / p.MT) : 0;
+      mt_hi = it.k0 < it.L ? min(p.n_mt, static_cast<int>(fast_div(it.L + p.MT - 1, p.by_mt))) : 0;
     } else if (kMode == kMaskAnalytic) {
       const int pe = min(it.k0 + kKeys, p.P);  // prefix keys of the item: [k0, pe)
       const bool prefix = it.k0 < min(pe, p.ds) || max(it.k0, p.de) < pe;
       if (!prefix) {
         const int c = max(it.k0, p.P);  // the first staircase key: visible from row c - (N - M)
-        mt_lo = c < min(it.k0 + kKeys, p.N) ? min(p.n_mt, max(0, c - (p.N - p.M)) / p.MT) : p.n_mt;
+        mt_lo = c < min(it.k0 + kKeys, p.N)
+                    ? min(p.n_mt, static_cast<int>(fast_div(max(0, c - (p.N - p.M)), p.by_mt)))
+                    : p.n_mt;
       }
     }
     it.mt_lo = mt_lo;
     it.mt_hi = mt_hi;
-    it.live = p.n_sub / p.n_mt * max(0, mt_hi - mt_lo);
+    it.live = p.n_hblk * max(0, mt_hi - mt_lo);
   } else {
     it.s0 = 2 * (p.n_pair - 1 - blk);
     it.n_here = min(2, p.n_sub - it.s0);
     // first and last position of the rows
-    const int mt0 = it.s0 % p.n_mt, mt1 = (it.s0 + it.n_here - 1) % p.n_mt;
+    const int s1 = it.s0 + it.n_here - 1;
+    const int mt0 = it.s0 - fast_div(it.s0, p.by_mt_count) * p.n_mt;
+    const int mt1 = s1 - fast_div(s1, p.by_mt_count) * p.n_mt;
     const int m_lo = min(mt0, mt1) * p.MT;
     const int m_hi = min(p.M, (max(mt0, mt1) + 1) * p.MT) - 1;
     int b1 = 0;
@@ -360,7 +370,7 @@ struct Turn {
   }
 };
 
-// (each of the four warps of the last warpgroup)
+// (every warp of the warpgroups behind the compute warps)
 __device__ __forceinline__ void less_registers() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
 }
@@ -369,20 +379,18 @@ template <int kMode>
 __global__ void __launch_bounds__(kThreads, 1) attn_bwd(const __grid_constant__ BwdParams p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = aligned_smem(smem_raw);
-  uint8_t* a_smem = smem;                             // [2][A0 16 KB, A1 16 KB]; then the staged output
-  uint8_t* b_smem = a_smem + 2 * 4 * kSubBytes;       // [kRing][B0 8 KB, B1 8 KB]
+  uint8_t* a_smem = smem;                             // [kTiles][A0 16 KB, A1 16 KB]; then the staged output
+  uint8_t* b_smem = a_smem + kTiles * 4 * kSubBytes;       // [kRing][B0 8 KB, B1 8 KB]
   float* b_stat = reinterpret_cast<float*>(b_smem + kRing * 2 * kSubBytes);  // [kRing][128]: dkv
-  float* a_stat = b_stat + kRing * kStatFloats;       // [2][2 sub-tiles][128]: dq
-  Barriers* bars = reinterpret_cast<Barriers*>(a_stat + 2 * 2 * kStatFloats);
+  float* a_stat = b_stat + kRing * kStatFloats;       // [kTiles][2 sub-tiles][128]: dq
+  Barriers* bars = reinterpret_cast<Barriers*>(a_stat + kTiles * 2 * kStatFloats);
   volatile int* abort_flag = &bars->abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < kTiles; ++i) {
       mbar_init(&bars->a_full[i], 1);
       mbar_init(&bars->a_empty[i], 1);
-      mbar_init(&bars->out_full[i], 1);
-      mbar_init(&bars->staged[i], kGroupWarps);
     }
     for (int i = 0; i < kRing; ++i) {
       mbar_init(&bars->b_full[i], 1);
@@ -395,9 +403,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd(const __grid_constant__ 
     }
     for (int i = 0; i < kQueue; ++i) {
       mbar_init(&bars->it_full[i], 1);
-      mbar_init(&bars->it_empty[i], kComputeWarps + 2);
+      mbar_init(&bars->it_empty[i], kComputeWarps + 2 + kOutputWarps);
     }
-    mbar_init(&bars->acc_empty, kGroupWarps);
+    mbar_init(&bars->out_full, 1);
+    mbar_init(&bars->staged, kOutputWarps);
+    mbar_init(&bars->acc_empty, kOutputWarps);
     mbar_init(&bars->drain[0], 1);
     mbar_init(&bars->drain[1], 1);
     bars->abort_flag = 0;
@@ -447,14 +457,14 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd(const __grid_constant__ 
     // the statistics and the counter are those of the kernel before
     asm volatile("griddepcontrol.wait;" ::: "memory");
     uint32_t t = 0, live = 0;  // steps and live items issued
+    unsigned next = lane == 0 ? atomicAdd(p.counter, 1u) : 0u;  // taken one ahead: it is a round trip
     bool ok = true;
     for (uint32_t n = 0; ok; ++n) {
       const uint32_t q = n % kQueue;
       if (!__all_sync(kFullMask, bounded_wait(&bars->it_empty[q], ((n / kQueue) & 1) ^ 1, abort_flag)))
         break;
-      int id = 0;
-      if (lane == 0) id = static_cast<int>(min(atomicAdd(p.counter, 1u), static_cast<unsigned>(p.n_items)));
-      id = __shfl_sync(kFullMask, id, 0);
+      const int id = min(__shfl_sync(kFullMask, next, 0), static_cast<unsigned>(p.n_items));
+      if (lane == 0 && id < p.n_items) next = atomicAdd(p.counter, 1u);
       Item it{};
       if (id < p.n_items)
         it = decode_item<kMode>(p, id);
@@ -468,8 +478,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd(const __grid_constant__ 
       if (it.live < 0) break;
       if (it.live == 0) continue;
       const int bk = it.b * p.Hkv + it.kvh;
-      const uint32_t ab = live & 1;
-      if (!__all_sync(kFullMask, bounded_wait(&bars->a_empty[ab], ((live >> 1) & 1) ^ 1, abort_flag)))
+      const uint32_t ab = live % kTiles;
+      if (!__all_sync(kFullMask, bounded_wait(&bars->a_empty[ab], ((live / kTiles) & 1) ^ 1, abort_flag)))
         break;
       uint8_t* a0 = a_smem + ab * 4 * kSubBytes;
       uint8_t* a1 = a0 + 2 * kSubBytes;
@@ -482,7 +492,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd(const __grid_constant__ 
             &bars->a_full[ab],
             static_cast<uint32_t>(it.n_here * (2 * p.Gb * p.MT * kRowBytes + kStatBytes)));
         for (int i = 0; i < it.n_here; ++i) {
-          const int hb = (it.s0 + i) / p.n_mt, m0 = (it.s0 + i - hb * p.n_mt) * p.MT;
+          const int hb = fast_div(it.s0 + i, p.by_mt_count), m0 = (it.s0 + i - hb * p.n_mt) * p.MT;
           const int h = it.kvh * p.G + hb * p.Gb;
           tma_load_4d_elect(a0 + i * kSubBytes, &p.tm_q, &bars->a_full[ab], 0, h, m0, it.b);
           tma_load_4d_elect(a1 + i * kSubBytes, &p.tm_do, &bars->a_full[ab], 0, h, m0, it.b);
@@ -519,8 +529,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd(const __grid_constant__ 
       }
     }
     // never leave the CTA with copies in flight (bounded, abort or not)
-    for (uint32_t k = live > 2 ? live - 2 : 0; k < live; ++k)
-      bounded_wait(&bars->a_full[k & 1], (k >> 1) & 1, abort_flag, false);
+    for (uint32_t k = live > kTiles ? live - kTiles : 0; k < live; ++k)
+      bounded_wait(&bars->a_full[k % kTiles], (k / kTiles) & 1, abort_flag, false);
     for (uint32_t k = t > kRing ? t - kRing : 0; k < t; ++k)
       bounded_wait(&bars->b_full[k % kRing], (k / kRing) & 1, abort_flag, false);
     __syncwarp();
@@ -533,7 +543,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd(const __grid_constant__ 
     // streamed rows that meet X = 0 only, and may hold NaN, are cleared: keys
     // that no query sees (dq), query rows past L (dkv)
     const bool dead = kMode == kMaskLength || (kMode == kMaskAnalytic && p.ds < p.de);
-    Turn<2> ab;
+    Turn<kTiles> ab;
     Turn<kRing> s;
     Turn<kStages> st;
     bool ok = true;
@@ -613,7 +623,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd(const __grid_constant__ 
         st.next();
       }
       if (!ok) break;
-      umma_commit_elect(&bars->out_full[live & 1]);
+      umma_commit_elect(&bars->out_full);
       ++live;
     }
     umma_commit_elect(&bars->drain[1]);
@@ -621,8 +631,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd(const __grid_constant__ 
     __syncwarp();
   } else if (warp < kComputeWarps) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsCompute));
-    // Compute warps. A step belongs to the group of its parity, an item's
-    // output to the group of the item's.
+    // Compute warps. A step belongs to the group of its parity.
     const int group = warp >> 3, quarter = warp & 3, gq = (warp >> 2) & 1;
     const int tl = quarter * 32 + lane;  // TMEM lane: key of a dkv item, row of a dq item
     const uint32_t tbase = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
@@ -632,30 +641,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd(const __grid_constant__ 
     for (uint32_t n = 0; ok; ++n) {
       Item it;
       if (!take_item(n, it) || it.live < 0) break;
+      if (it.live == 0) continue;
       // this lane's key, or row
       const int key = it.k0 + tl;
       const SubRow r = sub_row(p, it.s0 + (quarter >> 1), (quarter & 1) * 32 + lane);
       const bool valid = it.dkv ? key < p.N : r.valid;
-      if (it.live == 0) {  // nothing seen: zeros
-        if (group == static_cast<int>(n & 1) && gq == 0 && valid) {
-          __nv_bfloat16* dst[2];
-          if (it.dkv) {
-            const long long at = ((static_cast<long long>(it.b) * p.N + key) * p.Hkv + it.kvh) * 64;
-            dst[0] = p.dk + at;
-            dst[1] = p.dv + at;
-          } else {
-            dst[0] = dst[1] = p.dq + ((static_cast<long long>(it.b) * p.M + r.m) * p.H +
-                                      it.kvh * p.G + r.g) * 64;
-          }
-#pragma unroll
-          for (int v = 0; v < 8; ++v) {
-            reinterpret_cast<uint4*>(dst[0])[v] = make_uint4(0, 0, 0, 0);
-            reinterpret_cast<uint4*>(dst[1])[v] = make_uint4(0, 0, 0, 0);
-          }
-        }
-        continue;
-      }
-      const uint32_t ab = live & 1;
+      const uint32_t ab = live % kTiles;
       // dkv: rows m in [from, to) see the key; dq: keys [0, from) and [mid, to)
       // are seen by the row
       int from = 0, mid = 0, to = 0;
@@ -713,7 +704,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd(const __grid_constant__ 
       if (!it.dkv && j0 < it.live) {
         // the row's statistics (only with a step to do: a group without one may
         // come here after the tiles have been replaced)
-        if (!__all_sync(kFullMask, bounded_wait<1>(&bars->a_full[ab], (live >> 1) & 1, abort_flag))) break;
+        if (!__all_sync(kFullMask, bounded_wait<1>(&bars->a_full[ab], (live / kTiles) & 1, abort_flag))) break;
         const float* stat = a_stat + (ab * 2 + (quarter >> 1)) * kStatFloats + (quarter & 1) * 32 + lane;
         nl2 = f2_pack(stat[0], stat[0]);
         nD2 = f2_pack(stat[kSub], stat[kSub]);
@@ -829,65 +820,87 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd(const __grid_constant__ 
         tc_fence_before();
         mbar_arrive_elect(&bars->x_full[st]);
       }
-      if (!ok) break;
       t += it.live;
-      if (static_cast<int>(ab) == group) {
-        // Output: the accumulators, scaled, staged over the item's stationary
-        // tiles in the swizzled layout of the maps, then TMA stores.
-        if (!__all_sync(kFullMask, bounded_wait(&bars->out_full[group], (live >> 1) & 1, abort_flag))) break;
-        tc_fence_after();
-        uint8_t* a0 = a_smem + ab * 4 * kSubBytes;
-        // dkv: dV (first warps of a quarter) over V, dK (second) over K, 64
-        // columns each; dq: 32 columns of dQ each, over Q
-        const float scale = it.dkv && gq == 0 ? 1.f : p.out_scale;
-        uint8_t* stage = a0 + (it.dkv && gq == 0 ? 2 * kSubBytes : 0) + tl * kRowBytes;
-        const uint32_t acc = tbase + (it.dkv && gq == 0 ? kAcc0 : kAcc1);
-        const int blocks = it.dkv ? 2 : 1;  // of 32 columns
-        for (int q = 0; q < blocks; ++q) {
-          const int col = it.dkv ? 32 * q : 32 * gq;
-          float o[32];
-          tmem_ld32(acc + col, o);
-          tmem_wait_ld();
-          if (q == blocks - 1) {  // read: the next item may accumulate
-            tc_fence_before();
-            mbar_arrive_elect(&bars->acc_empty);
-          }
-#pragma unroll
-          for (int v = 0; v < 4; ++v) {
-            uint32_t w[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              w[e] = pack_bf16x2(o[v * 8 + 2 * e] * scale, o[v * 8 + 2 * e + 1] * scale);
-            const uint32_t c = static_cast<uint32_t>(col / 8 + v) ^ static_cast<uint32_t>(tl & 7);
-            st_shared_v4(stage + c * 16, w[0], w[1], w[2], w[3]);
-          }
-        }
-        fence_proxy_async_smem();
-        __syncwarp();
-        mbar_arrive_elect(&bars->staged[group]);
-        if ((warp & 7) == 0) {
-          if (!__all_sync(kFullMask, bounded_wait(&bars->staged[group], (live >> 1) & 1, abort_flag))) break;
-          if (lane == 0) {
-            if (it.dkv) {
-              tma_store_4d(&p.tm_dk, a0, 0, it.kvh, it.k0, it.b);
-              tma_store_4d(&p.tm_dv, a0 + 2 * kSubBytes, 0, it.kvh, it.k0, it.b);
-            } else {
-              for (int i = 0; i < it.n_here; ++i) {
-                const int hb = (it.s0 + i) / p.n_mt, m0 = (it.s0 + i - hb * p.n_mt) * p.MT;
-                tma_store_4d(&p.tm_dq, a0 + i * kSubBytes, 0, it.kvh * p.G + hb * p.Gb, m0, it.b);
-              }
-            }
-            bulk_commit_group();
-            bulk_wait_read0();
-            mbar_arrive(&bars->a_empty[ab]);
-          }
-          __syncwarp();
-        }
-      }
       ++live;
     }
-    // the stores of this warp complete before the CTA exits
-    if ((warp & 7) == 0 && lane == 0) bulk_wait_all0();
+  } else if (warp >= kWarpOutput) {
+    less_registers();
+    // Outputs: the accumulators, scaled, staged over the item's stationary tiles
+    // in the swizzled layout of the maps, then TMA stores. One lane quarter of
+    // TMEM per warp.
+    const int quarter = warp & 3;
+    const int tl = quarter * 32 + lane;  // key of a dkv item, row of a dq item
+    const uint32_t tbase = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
+    uint32_t live = 0;
+    Turn<kTiles> ab;
+    for (uint32_t n = 0;; ++n) {
+      Item it;
+      if (!take_item(n, it) || it.live < 0) break;
+      if (it.live == 0) {  // nothing seen: zeros
+        const int key = it.k0 + tl;
+        const SubRow r = sub_row(p, it.s0 + (quarter >> 1), (quarter & 1) * 32 + lane);
+        if (it.dkv ? key < p.N : r.valid) {
+          const long long at =
+              it.dkv ? ((static_cast<long long>(it.b) * p.N + key) * p.Hkv + it.kvh) * 64
+                     : ((static_cast<long long>(it.b) * p.M + r.m) * p.H + it.kvh * p.G + r.g) * 64;
+          uint4* d0 = reinterpret_cast<uint4*>((it.dkv ? p.dk : p.dq) + at);
+          uint4* d1 = reinterpret_cast<uint4*>((it.dkv ? p.dv : p.dq) + at);
+#pragma unroll
+          for (int v = 0; v < 8; ++v) d0[v] = d1[v] = make_uint4(0, 0, 0, 0);
+        }
+        continue;
+      }
+      if (!__all_sync(kFullMask, bounded_wait<1>(&bars->out_full, live & 1, abort_flag))) break;
+      tc_fence_after();
+      uint8_t* a0 = a_smem + ab.i * 4 * kSubBytes;
+      // dK over K (dQ over Q), then dV over V
+      for (int q = 0; q < (it.dkv ? 8 : 4); ++q) {  // 16 columns at a time
+        const bool dv = q >= 4;
+        float o[16];
+        tmem_ld16(tbase + (dv ? kAcc0 - 64 : kAcc1) + 16 * q, o);
+        tmem_wait_ld();
+        if (q == (it.dkv ? 7 : 3)) {  // read: the next item may accumulate
+          tc_fence_before();
+          mbar_arrive_elect(&bars->acc_empty);
+        }
+        const float scale = dv ? 1.f : p.out_scale;
+        uint8_t* stage = a0 + (dv ? 2 * kSubBytes : 0) + tl * kRowBytes;
+#pragma unroll
+        for (int v = 0; v < 2; ++v) {
+          uint32_t w[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            w[e] = pack_bf16x2(o[v * 8 + 2 * e] * scale, o[v * 8 + 2 * e + 1] * scale);
+          const uint32_t c = static_cast<uint32_t>(2 * (q & 3) + v) ^ static_cast<uint32_t>(tl & 7);
+          st_shared_v4(stage + c * 16, w[0], w[1], w[2], w[3]);
+        }
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      mbar_arrive_elect(&bars->staged);
+      if (warp == kWarpOutput) {
+        if (!__all_sync(kFullMask, bounded_wait<1>(&bars->staged, live & 1, abort_flag))) break;
+        if (lane == 0) {
+          if (it.dkv) {
+            tma_store_4d(&p.tm_dk, a0, 0, it.kvh, it.k0, it.b);
+            tma_store_4d(&p.tm_dv, a0 + 2 * kSubBytes, 0, it.kvh, it.k0, it.b);
+          } else {
+            for (int i = 0; i < it.n_here; ++i) {
+              const int hb = fast_div(it.s0 + i, p.by_mt_count), m0 = (it.s0 + i - hb * p.n_mt) * p.MT;
+              tma_store_4d(&p.tm_dq, a0 + i * kSubBytes, 0, it.kvh * p.G + hb * p.Gb, m0, it.b);
+            }
+          }
+          bulk_commit_group();
+          bulk_wait_read0();
+          mbar_arrive(&bars->a_empty[ab.i]);
+        }
+        __syncwarp();
+      }
+      ab.next();
+      ++live;
+    }
+    // the stores complete before the CTA exits
+    if (warp == kWarpOutput && lane == 0) bulk_wait_all0();
     __syncwarp();
   } else {
     less_registers();
@@ -1032,6 +1045,7 @@ int run_bwd(const vlak_attn_train_args* t, void* workspace, int64_t ws_bytes, vo
   p.MT = tl.MT;
   p.n_mt = tl.n_mt;
   p.n_sub = tl.n_sub;
+  p.n_hblk = tl.n_sub / tl.n_mt;
   p.n_pair = (tl.n_sub + 1) / 2;
   p.n_kblk = (p.N + kKeys - 1) / kKeys;
   p.n_chunks = (p.N + kChunk - 1) / kChunk;
@@ -1045,6 +1059,13 @@ int run_bwd(const vlak_attn_train_args* t, void* workspace, int64_t ws_bytes, vo
   // Few heads: all their long items first, for balance, their tensors stay in
   // L2. Many: a head's items one after the other, while its tensors are there.
   p.bk_inner = n_bk <= 2 * dev.sm_count;
+  p.by_bk = fast_div_by(static_cast<unsigned>(n_bk));
+  p.by_kblk = fast_div_by(static_cast<unsigned>(p.n_kblk));
+  p.by_pair = fast_div_by(static_cast<unsigned>(p.n_pair));
+  p.by_hkv = fast_div_by(static_cast<unsigned>(p.Hkv));
+  p.by_mt_count = fast_div_by(static_cast<unsigned>(p.n_mt));
+  p.by_mt = fast_div_by(static_cast<unsigned>(p.MT));
+  p.by_gb = fast_div_by(static_cast<unsigned>(p.Gb));
   p.P = static_cast<int>(P);
   p.ds = static_cast<int>(a->dead_start);
   p.de = static_cast<int>(a->dead_end);

@@ -53,15 +53,6 @@ struct RotTensor {
   int H;
 };
 
-// n / d for n < 2^31 by a multiplication: m = ceil(2^(32 + l) / d) - 2^32 with
-// l = ceil(log2 d); (n m >> 32) + n is below 2^32 for n < 2^31.
-struct FastDiv {
-  unsigned d, m, l;
-};
-__device__ __forceinline__ unsigned fast_div(unsigned n, const FastDiv& f) {
-  return (__umulhi(n, f.m) + n) >> f.l;
-}
-
 struct RotParams {
   RotTensor t[2];      // blockIdx.y selects
   const void* pos;
@@ -542,11 +533,6 @@ int lg_ceil(int64_t n) {
   int lg = 0;
   while ((int64_t{1} << lg) < n) ++lg;
   return lg;
-}
-FastDiv fast_div_by(unsigned d) {
-  const unsigned l = static_cast<unsigned>(lg_ceil(d));
-  const uint64_t m = (((uint64_t{1} << l) - d) << 32) / d + 1;
-  return FastDiv{d, static_cast<unsigned>(m), l};
 }
 // The 16-byte path wants whole units (two vectors) in the rotated part and in
 // the rest, a head on at most one warp, and vectors on 16-byte boundaries.

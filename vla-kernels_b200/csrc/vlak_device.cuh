@@ -30,6 +30,22 @@ __device__ __forceinline__ float warp_sum(float v) {
 }
 
 // ---------------------------------------------------------------------------
+// n / d for n < 2^31 by a multiplication: m = ceil(2^(32 + l) / d) - 2^32 with
+// l = ceil(log2 d); (n m >> 32) + n is below 2^32 for n < 2^31.
+struct FastDiv {
+  unsigned d, m, l;
+};
+inline FastDiv fast_div_by(unsigned d) {
+  unsigned l = 0;
+  while ((uint64_t{1} << l) < d) ++l;
+  const uint64_t m = (((uint64_t{1} << l) - d) << 32) / d + 1;
+  return FastDiv{d, static_cast<unsigned>(m), l};
+}
+__device__ __forceinline__ unsigned fast_div(unsigned n, const FastDiv& f) {
+  return (__umulhi(n, f.m) + n) >> f.l;
+}
+
+// ---------------------------------------------------------------------------
 // 16-byte vectors of each element type
 template <typename T> struct Elem;
 template <> struct Elem<float> {
