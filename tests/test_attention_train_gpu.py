@@ -160,6 +160,27 @@ def test_many_samples(shape):
     run(*shape[:5], P, ds, de, seed=B)
 
 
+# few heads and one long side: an output's steps are shared out and joined
+@pytest.mark.parametrize("case", [(1, 2000, 1, 8, 1, None, 0, 0), (1, 2000, 70, 8, 1, 70, 5, 66),
+                                  (1, 1500, 1500, 1, 1, 0, 0, 0), (1, 1, 5000, 1, 1, None, 0, 0),
+                                  (1, 50, 4111, 3, 1, 4000, 100, 3900), (2, 2111, 9, 3, 1, 0, 0, 0),
+                                  (1, 7, 3000, 127, 1, 0, 0, 0), (1, 1300, 40, 67, 1, 0, 0, 0)], ids=str)
+def test_long_side_of_few_heads(case):
+    B, M, N, H, Hkv, P, ds, de = case
+    run(*case[:5], P, ds, de, seed=M)
+
+
+@pytest.mark.parametrize("shape", [(2, 1800, 1800, 2, 1), (1, 30, 3000, 3, 1), (1, 3000, 30, 3, 1)])
+def test_long_side_of_few_heads_other_masks(shape):
+    B, M, N, H, Hkv = shape
+    q, k, v, do = make(*shape, seed=M)
+    mask = random_mask(B, M, N, seed=N)
+    mask[:, :, N // 3: N // 2] = False
+    check(step(q, k, v, do, attn_mask=mask), orc.train(q, k, v, do, mask))
+    L = torch.tensor([N // 2, N][:B], device="cuda")
+    check(step(q, k, v, do, lengths=L), orc.train(q, k, v, do, orc.by_length(M, N, L)))
+
+
 def random_mask(B, M, N, seed, share=0.6):
     g = torch.Generator(device="cuda").manual_seed(seed)
     m = torch.rand(B, M, N, device="cuda", generator=g) < share

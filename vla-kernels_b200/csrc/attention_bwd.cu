@@ -52,18 +52,13 @@
 #include <type_traits>
 
 #include "attention_common.cuh"
+#include "attention_train.cuh"
 #include "vlak_device.cuh"
 #include "vlak_internal.h"
 
 namespace vlak {
 namespace {
 
-constexpr int kMaskAnalytic = 0, kMaskLength = 1, kMaskBool = 2;
-
-constexpr int kSub = 64;                     // rows of a streamed tile
-constexpr int kRowBytes = 128;               // 64 bf16
-constexpr int kSubBytes = kSub * kRowBytes;  // 8 KB
-constexpr int kChunk = 64;                   // keys of a dq step
 constexpr int kKeys = 128;                   // keys of a dkv item
 constexpr int kRing = 6;                     // streamed pairs in flight (even: see the compute warps)
 constexpr int kTiles = 3;                    // items whose stationary tiles are in shared memory
@@ -86,7 +81,7 @@ constexpr int kWarpProducer = kComputeWarps, kWarpScores = kComputeWarps + 1,
 constexpr int kWarpOutput = kComputeWarps + 4, kOutputWarps = 4;
 constexpr int kThreads = 32 * (kWarpOutput + kOutputWarps);
 // Registers: a compute thread wants more than an even share, the others less.
-constexpr int kRegsLaunch = 80, kRegsCompute = 96, kRegsOther = 48;
+constexpr int kRegsLaunch = 80, kRegsCompute = 88, kRegsOther = 64;
 static_assert(32 * kComputeWarps * kRegsCompute + (kThreads - 32 * kComputeWarps) * kRegsOther <=
                   kThreads * kRegsLaunch,
               "the split must fit the launch's registers");
@@ -97,7 +92,7 @@ constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kAcc0 = 0, kAcc1 = 64, kStage0 = 128, kStageCols = 128, kT1 = 64;
 static_assert(kStage0 + kStages * kStageCols <= kTmemCols, "TMEM");
 
-struct __align__(64) BwdParams {
+struct __align__(64) BwdParams : TrainShape {
   CUtensorMap tm_q, tm_do, tm_dq;            // dims (64, H, M, B), box (64, Gb, MT, 1)
   CUtensorMap tm_k64, tm_v64;                // dims (64, Hkv, N, B), box (64, 1, 64, 1)
   CUtensorMap tm_k, tm_v, tm_dk, tm_dv;      // the same, box (64, 1, 128, 1)
@@ -106,58 +101,14 @@ struct __align__(64) BwdParams {
   long long o_s[3], do_s[3];                 // (b, m, h) element strides
   const float* lse;                          // (B, M, H), log2 units
   float* stats;                              // [B * Hkv][n_sub][-lse 64, -D 64]
-  unsigned* counter;                         // next item
-  int B, M, N, H, Hkv, G;
-  int Gb, MT;                                // heads and positions of a sub-tile
-  int n_mt, n_hblk, n_sub, n_pair, n_kblk, n_chunks;
-  int n_bk, n_dkv, n_items;                  // B * Hkv; dkv items; all items
-  int bk_inner;                              // items run over (b, kv head) first
-  int P, ds, de;
-  float scale_log2, out_scale;
-  int* host_err;
-  const void* lengths;
-  int lengths_i64;
-  const uint8_t* mask;
-  long long mask_sb, mask_sm;
-  int mask_words;
-  FastDiv by_bk, by_kblk, by_pair, by_hkv, by_mt_count, by_mt, by_gb;
+  // Parts of a dkv and of a dq item's steps; with several, each leaves its sums
+  // in fp32: [part][item][128 keys][dK 64, dV 64] and [part][sub-tile][64][64].
+  int kv_parts, q_parts;
+  float *kv_sums, *q_sums;
+  int n_kblk, n_dkv, n_items;                // dkv parts; all parts
+  float out_scale;
+  FastDiv by_kblk, by_kv_parts, by_q_parts;
 };
-
-__device__ __forceinline__ int length_of(const BwdParams& p, int b) {
-  const long long len = p.lengths_i64 ? static_cast<const long long*>(p.lengths)[b]
-                                      : static_cast<const int*>(p.lengths)[b];
-  return static_cast<int>(min(max(len, 0LL), static_cast<long long>(p.N)));
-}
-
-// low n bits set, n clamped to [0, 32]
-__device__ __forceinline__ uint32_t low_bits(int n) {
-  return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : ((1u << n) - 1u);
-}
-
-// A step's 64 bf16 operand columns: each half of them is packed over the first
-// half of the 32 fp32 columns it was computed from, which the warp that packs
-// them has read; so they lie at columns 0-15 and 32-47 (see umma_ts_x4).
-
-// 1024-byte aligned start of the dynamic shared memory
-__device__ __forceinline__ uint8_t* aligned_smem(uint8_t* raw) {
-  return raw + (((smem_u32(raw) + 1023u) & ~1023u) - smem_u32(raw));
-}
-
-// Row `row` of sub-tile st of a (b, kv head): position m, head h within the kv
-// head, and whether it exists.
-struct SubRow {
-  int m, g;
-  bool valid;
-};
-__device__ __forceinline__ SubRow sub_row(const BwdParams& p, int st, int row) {
-  const int hb = fast_div(st, p.by_mt_count), mt = st - hb * p.n_mt;
-  const int local = fast_div(row, p.by_gb);
-  SubRow r;
-  r.m = mt * p.MT + local;
-  r.g = hb * p.Gb + row - local * p.Gb;
-  r.valid = st < p.n_sub && local < p.MT && r.m < p.M;
-  return r;
-}
 
 // ---------------------------------------------------------------------------
 // D = rowsum(dO * O) and -lse by sub-tile rows: four threads per row, two 16-byte
@@ -201,43 +152,6 @@ __global__ void __launch_bounds__(kStatThreads) attn_bwd_stats(const __grid_cons
   }
 }
 
-// ---------------------------------------------------------------------------
-// Items
-
-// An item as the producer hands it out through shared memory (16 bytes at a
-// time).
-struct __align__(16) Item {
-  int live;           // -1: no more items; else its steps
-  int dkv, b, kvh;
-  int L;              // length of the sample (lengths only)
-  int k0;             // dkv: first key
-  int s0, n_here;     // dq: first sub-tile and how many (1 or 2)
-  int a1, b0;         // dq: live chunks [0, a1) and [b0, ...)
-  int mt_lo, mt_hi;   // dkv: live position blocks of each head block
-};
-static_assert(sizeof(Item) == 48, "three vectors");
-
-// The steps of an item in order: chunk `pos` (dq), or position block `pos` of
-// head block `hb` (dkv).
-struct Steps {
-  int pos, hb;
-  __device__ __forceinline__ void begin(const Item& it) {
-    hb = 0;
-    pos = it.dkv ? it.mt_lo : it.a1 > 0 ? 0 : it.b0;
-  }
-  __device__ __forceinline__ void next(const Item& it) {
-    ++pos;
-    if (it.dkv) {
-      if (pos == it.mt_hi) {
-        pos = it.mt_lo;
-        ++hb;
-      }
-    } else if (pos == it.a1) {
-      pos = it.b0;
-    }
-  }
-};
-
 struct Barriers {
   uint64_t a_full[kTiles], a_empty[kTiles];  // stationary tiles of an item
   uint64_t b_full[kRing], b_empty[kRing];  // streamed pairs
@@ -248,7 +162,7 @@ struct Barriers {
   uint32_t tmem_base;
   int abort_flag;
 };
-constexpr int kBarrierBytes = 896;
+constexpr int kBarrierBytes = 1024;
 static_assert(sizeof(Barriers) <= kBarrierBytes, "barrier block");
 constexpr int kSmem = kTiles * 4 * kSubBytes + kRing * (2 * kSubBytes + kStatBytes) + kTiles * 2 * kStatBytes +
                       kBarrierBytes + 1024;
@@ -258,7 +172,8 @@ template <int kMode>
 __device__ __forceinline__ Item decode_item(const BwdParams& p, int id) {
   Item it{};
   it.dkv = id < p.n_dkv;
-  const int i = it.dkv ? id : id - p.n_dkv;
+  const int at = it.dkv ? id : id - p.n_dkv, parts = it.dkv ? p.kv_parts : p.q_parts;
+  const int i = fast_div(at, it.dkv ? p.by_kv_parts : p.by_q_parts);
   // blk: key block, or pair of sub-tiles counted from the last, whose rows see
   // the most keys under a staircase, as the first keys are seen by the most rows
   const FastDiv& inner = it.dkv ? p.by_kblk : p.by_pair;
@@ -288,87 +203,11 @@ __device__ __forceinline__ Item decode_item(const BwdParams& p, int id) {
     it.mt_hi = mt_hi;
     it.live = p.n_hblk * max(0, mt_hi - mt_lo);
   } else {
-    it.s0 = 2 * (p.n_pair - 1 - blk);
-    it.n_here = min(2, p.n_sub - it.s0);
-    // first and last position of the rows
-    const int s1 = it.s0 + it.n_here - 1;
-    const int mt0 = it.s0 - fast_div(it.s0, p.by_mt_count) * p.n_mt;
-    const int mt1 = s1 - fast_div(s1, p.by_mt_count) * p.n_mt;
-    const int m_lo = min(mt0, mt1) * p.MT;
-    const int m_hi = min(p.M, (max(mt0, mt1) + 1) * p.MT) - 1;
-    int b1 = 0;
-    if (kMode == kMaskBool) {
-      it.a1 = p.n_chunks;
-    } else if (kMode == kMaskLength) {
-      it.a1 = m_lo < it.L ? (it.L + kChunk - 1) / kChunk : 0;
-    } else {
-      it.a1 = (p.ds + kChunk - 1) / kChunk;
-      if (p.de < p.N) {
-        const int e2 = max(p.P, min(p.N, p.N - p.M + m_hi + 1));
-        it.b0 = max(p.de / kChunk, it.a1);
-        b1 = (e2 + kChunk - 1) / kChunk;
-      }
-    }
-    it.live = it.a1 + max(0, b1 - it.b0);
+    row_item<kMode>(p, blk, it);
   }
+  if (parts > 1) take_part(it, at - i * parts, parts);
   return it;
 }
-
-__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile(
-      "{\n\t.reg .pred e;\n\t"
-      "elect.sync _|e, 0xffffffff;\n\t"
-      "@e cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n\t}"
-      ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar))
-      : "memory");
-}
-
-// The four K = 16 products of one 64-deep contraction, from one elected lane.
-// Descriptors step by 32 bytes of a swizzled row (SS, both operands) or by 16
-// rows of 128 bytes (TS, B).
-__device__ __forceinline__ void umma_ss_x4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc) {
-  asm volatile(
-      "{\n\t.reg .pred e, n, y;\n\t.reg .b64 a1, a2, a3, b1, b2, b3;\n\t"
-      "elect.sync _|e, 0xffffffff;\n\t"
-      "setp.ne.b32 n, 0, 0;\n\tsetp.eq.b32 y, 0, 0;\n\t"
-      "add.s64 a1, %1, 2;\n\tadd.s64 a2, %1, 4;\n\tadd.s64 a3, %1, 6;\n\t"
-      "add.s64 b1, %2, 2;\n\tadd.s64 b2, %2, 4;\n\tadd.s64 b3, %2, 6;\n\t"
-      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, n;\n\t"
-      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a1, b1, %3, y;\n\t"
-      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a2, b2, %3, y;\n\t"
-      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a3, b3, %3, y;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc)
-      : "memory");
-}
-// A in TMEM at columns x + 0, 8, 32, 40; `acc` 0 starts a new sum; `on` 0
-// issues nothing.
-__device__ __forceinline__ void umma_ts_x4(uint32_t d, uint32_t x, uint64_t b, uint32_t idesc,
-                                           uint32_t acc, uint32_t on) {
-  asm volatile(
-      "{\n\t.reg .pred e, q, p, y;\n\t.reg .b32 x1, x2, x3;\n\t.reg .b64 b1, b2, b3;\n\t"
-      "elect.sync _|e, 0xffffffff;\n\t"
-      "setp.ne.and.b32 q, %5, 0, e;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\tsetp.eq.b32 y, 0, 0;\n\t"
-      "add.s32 x1, %1, 8;\n\tadd.s32 x2, %1, 32;\n\tadd.s32 x3, %1, 40;\n\t"
-      "add.s64 b1, %2, 128;\n\tadd.s64 b2, %2, 256;\n\tadd.s64 b3, %2, 384;\n\t"
-      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
-      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [x1], b1, %3, y;\n\t"
-      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [x2], b2, %3, y;\n\t"
-      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [x3], b3, %3, y;\n\t}" ::"r"(d),
-      "r"(x), "l"(b), "r"(idesc), "r"(acc), "r"(on)
-      : "memory");
-}
-// A counter modulo n with the parity of its rounds.
-template <int n>
-struct Turn {
-  uint32_t i = 0, round = 0;
-  __device__ __forceinline__ void next() {
-    if (++i == n) {
-      i = 0;
-      round ^= 1;
-    }
-  }
-};
 
 // (every warp of the warpgroups behind the compute warps)
 __device__ __forceinline__ void less_registers() {
@@ -442,11 +281,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd(const __grid_constant__ 
     const uint32_t q = n % kQueue;
     if (!__all_sync(kFullMask, bounded_wait<1>(&bars->it_full[q], (n / kQueue) & 1, abort_flag)))
       return false;
-    const int4* src = reinterpret_cast<const int4*>(&bars->item[q]);
-    const int4 x = src[0], y = src[1], z = src[2];
-    it.live = x.x; it.dkv = x.y; it.b = x.z; it.kvh = x.w;
-    it.L = y.x; it.k0 = y.y; it.s0 = y.z; it.n_here = y.w;
-    it.a1 = z.x; it.b0 = z.y; it.mt_lo = z.z; it.mt_hi = z.w;
+    it = load_item(&bars->item[q]);
     __syncwarp();
     mbar_arrive_elect(&bars->it_empty[q]);
     return true;
@@ -710,14 +545,15 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd(const __grid_constant__ 
         nD2 = f2_pack(stat[kSub], stat[kSub]);
       }
       const int per_head = it.mt_hi - it.mt_lo;  // position blocks of a head block (dkv)
-      int pos = it.mt_lo + j0;
+      int pos = it.mt_lo + j0 + (it.dkv && it.j0 > 0 ? it.j0 % per_head : 0);
       for (int j = j0; j < it.live; j += 2, pos += 2) {
         int c;
         if (it.dkv) {
           while (pos >= it.mt_hi) pos -= per_head;
           c = pos * p.MT;
         } else {
-          c = (j < it.a1 ? j : j - it.a1 + it.b0) * kChunk + 32 * gq;
+          const int k = it.j0 + j;
+          c = (k < it.a1 ? k : k - it.a1 + it.b0) * kChunk + 32 * gq;
         }
         // which of the columns this lane sees (dkv: rows past M or the box have
         // -lse = -inf, so their P is 0 without a mask)
@@ -836,10 +672,25 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd(const __grid_constant__ 
     for (uint32_t n = 0;; ++n) {
       Item it;
       if (!take_item(n, it) || it.live < 0) break;
+      const int parts = it.dkv ? p.kv_parts : p.q_parts;
+      // this lane's sums of a part: 128 (dK, dV) or 64 (dQ) of them
+      float* sums = nullptr;
+      if (parts > 1) {
+        const int bk = it.b * p.Hkv + it.kvh;
+        if (it.dkv)
+          sums = p.kv_sums + ((static_cast<long long>(it.part) * p.n_bk + bk) * p.n_kblk * kKeys +
+                              it.k0 + tl) * 128;
+        else if ((quarter >> 1) < it.n_here)
+          sums = p.q_sums + ((static_cast<long long>(it.part) * p.n_bk + bk) * p.n_sub * kSub +
+                             it.s0 * kSub + tl) * 64;
+      }
       if (it.live == 0) {  // nothing seen: zeros
         const int key = it.k0 + tl;
         const SubRow r = sub_row(p, it.s0 + (quarter >> 1), (quarter & 1) * 32 + lane);
-        if (it.dkv ? key < p.N : r.valid) {
+        if (sums != nullptr) {
+          for (int v = 0; v < (it.dkv ? 32 : 16); ++v)
+            reinterpret_cast<float4*>(sums)[v] = make_float4(0.f, 0.f, 0.f, 0.f);
+        } else if (parts == 1 && (it.dkv ? key < p.N : r.valid)) {
           const long long at =
               it.dkv ? ((static_cast<long long>(it.b) * p.N + key) * p.Hkv + it.kvh) * 64
                      : ((static_cast<long long>(it.b) * p.M + r.m) * p.H + it.kvh * p.G + r.g) * 64;
@@ -853,26 +704,39 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd(const __grid_constant__ 
       if (!__all_sync(kFullMask, bounded_wait<1>(&bars->out_full, live & 1, abort_flag))) break;
       tc_fence_after();
       uint8_t* a0 = a_smem + ab.i * 4 * kSubBytes;
-      // dK over K (dQ over Q), then dV over V
-      for (int q = 0; q < (it.dkv ? 8 : 4); ++q) {  // 16 columns at a time
-        const bool dv = q >= 4;
-        float o[16];
-        tmem_ld16(tbase + (dv ? kAcc0 - 64 : kAcc1) + 16 * q, o);
+      // dK over K (dQ over Q), then dV over V, 32 columns at a time
+      const int blocks = it.dkv ? 4 : 2;
+#pragma unroll 1
+      for (int q = 0; q < blocks; ++q) {
+        const bool dv = q >= 2;
+        float o[2][16];
+        tmem_ld16(tbase + (dv ? kAcc0 - 64 : kAcc1) + 32 * q, o[0]);
+        tmem_ld16(tbase + (dv ? kAcc0 - 64 : kAcc1) + 32 * q + 16, o[1]);
         tmem_wait_ld();
-        if (q == (it.dkv ? 7 : 3)) {  // read: the next item may accumulate
+        if (q == blocks - 1) {  // read: the next item may accumulate
           tc_fence_before();
           mbar_arrive_elect(&bars->acc_empty);
         }
-        const float scale = dv ? 1.f : p.out_scale;
-        uint8_t* stage = a0 + (dv ? 2 * kSubBytes : 0) + tl * kRowBytes;
+        if (parts > 1) {
+          if (sums != nullptr) {
 #pragma unroll
-        for (int v = 0; v < 2; ++v) {
-          uint32_t w[4];
+            for (int v = 0; v < 8; ++v)
+              reinterpret_cast<float4*>(sums)[8 * q + v] =
+                  make_float4(o[v / 4][v % 4 * 4], o[v / 4][v % 4 * 4 + 1], o[v / 4][v % 4 * 4 + 2],
+                              o[v / 4][v % 4 * 4 + 3]);
+          }
+        } else {
+          const float scale = dv ? 1.f : p.out_scale;
+          uint8_t* stage = a0 + (dv ? 2 * kSubBytes : 0) + tl * kRowBytes;
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            w[e] = pack_bf16x2(o[v * 8 + 2 * e] * scale, o[v * 8 + 2 * e + 1] * scale);
-          const uint32_t c = static_cast<uint32_t>(2 * (q & 3) + v) ^ static_cast<uint32_t>(tl & 7);
-          st_shared_v4(stage + c * 16, w[0], w[1], w[2], w[3]);
+          for (int v = 0; v < 4; ++v) {
+            uint32_t w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              w[e] = pack_bf16x2(o[v / 2][v % 2 * 8 + 2 * e] * scale, o[v / 2][v % 2 * 8 + 2 * e + 1] * scale);
+            const uint32_t c = static_cast<uint32_t>(4 * (q & 1) + v) ^ static_cast<uint32_t>(tl & 7);
+            st_shared_v4(stage + c * 16, w[0], w[1], w[2], w[3]);
+          }
         }
       }
       fence_proxy_async_smem();
@@ -881,7 +745,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd(const __grid_constant__ 
       if (warp == kWarpOutput) {
         if (!__all_sync(kFullMask, bounded_wait<1>(&bars->staged, live & 1, abort_flag))) break;
         if (lane == 0) {
-          if (it.dkv) {
+          if (parts > 1) {
+          } else if (it.dkv) {
             tma_store_4d(&p.tm_dk, a0, 0, it.kvh, it.k0, it.b);
             tma_store_4d(&p.tm_dv, a0 + 2 * kSubBytes, 0, it.kvh, it.k0, it.b);
           } else {
@@ -890,8 +755,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd(const __grid_constant__ 
               tma_store_4d(&p.tm_dq, a0 + i * kSubBytes, 0, it.kvh * p.G + hb * p.Gb, m0, it.b);
             }
           }
-          bulk_commit_group();
-          bulk_wait_read0();
+          if (parts == 1) {
+            bulk_commit_group();
+            bulk_wait_read0();
+          }
           mbar_arrive(&bars->a_empty[ab.i]);
         }
         __syncwarp();
@@ -916,29 +783,75 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd(const __grid_constant__ 
 }
 
 // ---------------------------------------------------------------------------
+// Joins of parts: the sums of an output, in the order of the parts, scaled and
+// rounded; four sums per thread. Bound: HBM, one read of the sums.
+__device__ __forceinline__ float4 sum_parts(const float* at, long long part_stride, int parts) {
+  float4 s = *reinterpret_cast<const float4*>(at);
+#pragma unroll 4
+  for (int k = 1; k < parts; ++k) {
+    const float4 x = *reinterpret_cast<const float4*>(at + k * part_stride);
+    s.x += x.x;
+    s.y += x.y;
+    s.z += x.z;
+    s.w += x.w;
+  }
+  return s;
+}
+__device__ __forceinline__ void store_4(__nv_bfloat16* dst, float4 s, float scale) {
+  *reinterpret_cast<uint2*>(dst) =
+      make_uint2(pack_bf16x2(s.x * scale, s.y * scale), pack_bf16x2(s.z * scale, s.w * scale));
+}
+// blockIdx.y: (b, kv head); 32 threads per key: dK, then dV
+__global__ void __launch_bounds__(256) attn_bwd_join_kv(const __grid_constant__ BwdParams p) {
+  const int key = blockIdx.x * 8 + (threadIdx.x >> 5), bk = blockIdx.y, v = threadIdx.x & 31;
+  if (key >= p.N) return;
+  const long long rows = static_cast<long long>(p.n_kblk) * kKeys;
+  const float4 s = sum_parts(p.kv_sums + (bk * rows + key) * 128 + 4 * v, p.n_bk * rows * 128, p.kv_parts);
+  const int b = fast_div(bk, p.by_hkv), kvh = bk - b * p.Hkv;
+  const long long at = ((static_cast<long long>(b) * p.N + key) * p.Hkv + kvh) * 64 + 4 * (v & 15);
+  store_4((v < 16 ? p.dk : p.dv) + at, s, v < 16 ? p.out_scale : 1.f);
+}
+// blockIdx.y: (b, kv head), blockIdx.x: quarter of a sub-tile; 16 threads per row
+__global__ void __launch_bounds__(256) attn_bwd_join_q(const __grid_constant__ BwdParams p) {
+  const int st = blockIdx.x >> 2, row = (blockIdx.x & 3) * 16 + (threadIdx.x >> 4);
+  const int bk = blockIdx.y, v = threadIdx.x & 15;
+  const SubRow r = sub_row(p, st, row);
+  if (!r.valid) return;
+  const long long rows = static_cast<long long>(p.n_sub) * kSub;
+  const float4 s = sum_parts(p.q_sums + (bk * rows + st * kSub + row) * 64 + 4 * v, p.n_bk * rows * 64,
+                             p.q_parts);
+  const int b = fast_div(bk, p.by_hkv), kvh = bk - b * p.Hkv;
+  store_4(p.dq + ((static_cast<long long>(b) * p.M + r.m) * p.H + kvh * p.G + r.g) * 64 + 4 * v, s,
+          p.out_scale);
+}
+
+// ---------------------------------------------------------------------------
 // host
 
-// Sub-tiles: the divisor Gb <= 64 of G whose boxes of Gb heads x MT positions
-// need the fewest, the larger one (longer contiguous reads) on a tie.
-struct SubTiling {
-  int Gb, MT, n_mt, n_sub;
+// Parts and workspace of a call: the sub-tiles' statistics, the item counter,
+// then the parts' sums.
+struct BwdPlan {
+  SubTiling tl;
+  int64_t n_bk, n_kblk, n_pair;
+  int kv_parts, q_parts;
+  int64_t counter, kv_sums, q_sums, bytes;  // offsets and size
 };
-SubTiling sub_tiling(int G, int M) {
-  SubTiling best{};
-  for (int d = 1; d <= std::min(G, kSub); ++d) {
-    if (G % d != 0) continue;
-    const int mt = std::min(kSub / d, M), n_mt = (M + mt - 1) / mt;
-    if (best.Gb == 0 || G / d * n_mt <= best.n_sub) best = SubTiling{d, mt, n_mt, G / d * n_mt};
-  }
-  return best;
+BwdPlan plan_bwd(const vlak_attn_gqa_args* a, bool keys_too) {
+  BwdPlan w{};
+  w.tl = sub_tiling(static_cast<int>(a->H / a->Hkv), static_cast<int>(a->M));
+  w.n_bk = a->B * a->Hkv;
+  w.n_kblk = (a->N + kKeys - 1) / kKeys;
+  w.n_pair = (w.tl.n_sub + 1) / 2;
+  const int64_t n_chunks = (a->N + kChunk - 1) / kChunk;
+  const int64_t total = w.n_bk * (w.n_pair * n_chunks + (keys_too ? w.n_kblk * w.tl.n_sub : 0));
+  w.kv_parts = keys_too ? item_parts(w.tl.n_sub, total) : 1;
+  w.q_parts = item_parts(n_chunks, total);
+  w.counter = w.n_bk * w.tl.n_sub * kStatBytes;
+  w.kv_sums = w.counter + 256;
+  w.q_sums = w.kv_sums + (w.kv_parts > 1 ? w.kv_parts * w.n_bk * w.n_kblk * kKeys * 128 * 4 : 0);
+  w.bytes = w.q_sums + (w.q_parts > 1 ? w.q_parts * w.n_bk * w.tl.n_sub * kSub * 64 * 4 : 0);
+  return w;
 }
-
-// workspace: statistics of the sub-tiles, then the item counter
-int64_t stats_bytes(const vlak_attn_gqa_args* a) {
-  const SubTiling t = sub_tiling(static_cast<int>(a->H / a->Hkv), static_cast<int>(a->M));
-  return a->B * a->Hkv * t.n_sub * kStatBytes;
-}
-constexpr int64_t kCounterBytes = 256;
 
 template <int kMode>
 cudaError_t launch_both(const BwdParams& p, unsigned n_stats, unsigned grid, cudaStream_t cs, int device) {
@@ -963,7 +876,16 @@ cudaError_t launch_both(const BwdParams& p, unsigned n_stats, unsigned grid, cud
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, attn_bwd<kMode>, p);
+  e = cudaLaunchKernelEx(&cfg, attn_bwd<kMode>, p);
+  if (e == cudaSuccess && p.kv_parts > 1) {
+    attn_bwd_join_kv<<<dim3((p.N + 7) / 8, p.n_bk), 256, 0, cs>>>(p);
+    e = cudaGetLastError();
+  }
+  if (e == cudaSuccess && p.q_parts > 1) {
+    attn_bwd_join_q<<<dim3(p.n_sub * 4, p.n_bk), 256, 0, cs>>>(p);
+    e = cudaGetLastError();
+  }
+  return e;
 }
 
 int bwd_validate(const vlak_attn_train_args* a, int64_t* P, float* scale) {
@@ -1019,7 +941,8 @@ int run_bwd(const vlak_attn_train_args* t, void* workspace, int64_t ws_bytes, vo
   }
   if (!a->q || !a->k || !a->v || !a->o || !args.grad_o || !args.lse)
     return set_error(VLAK_ERR_INVALID_ARGUMENT, "fused_attention_gqa_bwd: null tensor pointer");
-  if (!workspace || ws_bytes < stats_bytes(a) + kCounterBytes)
+  const BwdPlan plan = plan_bwd(a, keys_too);
+  if (!workspace || ws_bytes < plan.bytes)
     return set_error(VLAK_ERR_INVALID_ARGUMENT, "fused_attention_gqa_bwd: workspace missing or too small");
   if (reinterpret_cast<uintptr_t>(workspace) % 256 != 0)
     return set_error(VLAK_ERR_ALIGNMENT, "fused_attention_gqa_bwd: workspace must be 256-byte aligned");
@@ -1034,48 +957,30 @@ int run_bwd(const vlak_attn_train_args* t, void* workspace, int64_t ws_bytes, vo
 
   BwdParams p;
   memset(&p, 0, sizeof(p));
-  p.B = static_cast<int>(a->B);
-  p.M = static_cast<int>(a->M);
-  p.N = static_cast<int>(a->N);
-  p.H = static_cast<int>(a->H);
-  p.Hkv = static_cast<int>(a->Hkv);
-  p.G = p.H / p.Hkv;
-  const SubTiling tl = sub_tiling(p.G, p.M);
-  p.Gb = tl.Gb;
-  p.MT = tl.MT;
-  p.n_mt = tl.n_mt;
-  p.n_sub = tl.n_sub;
-  p.n_hblk = tl.n_sub / tl.n_mt;
-  p.n_pair = (tl.n_sub + 1) / 2;
-  p.n_kblk = (p.N + kKeys - 1) / kKeys;
-  p.n_chunks = (p.N + kChunk - 1) / kChunk;
-  const int64_t n_bk = a->B * a->Hkv, n_dq = n_bk * p.n_pair;
-  const int64_t n_dkv = keys_too ? n_bk * p.n_kblk : 0;
-  if (n_dq + n_dkv > INT32_MAX - 4096 || n_bk * p.n_sub > INT32_MAX)
+  const SubTiling& tl = plan.tl;
+  const int64_t n_bk = plan.n_bk, n_dq = n_bk * plan.n_pair * plan.q_parts;
+  const int64_t n_dkv = keys_too ? n_bk * plan.n_kblk * plan.kv_parts : 0;
+  if (n_dq + n_dkv > INT32_MAX - 4096 || n_bk * tl.n_sub > INT32_MAX)
     return set_error(VLAK_ERR_INVALID_ARGUMENT, "fused_attention_gqa_bwd: too many work items");
-  p.n_bk = static_cast<int>(n_bk);
+  static_cast<TrainShape&>(p) = train_shape(a, P, scale, tl);
+  set_masks(p, args);
+  p.n_kblk = static_cast<int>(plan.n_kblk);
   p.n_dkv = static_cast<int>(n_dkv);
   p.n_items = static_cast<int>(n_dkv + n_dq);
-  // Few heads: all their long items first, for balance, their tensors stay in
-  // L2. Many: a head's items one after the other, while its tensors are there.
-  p.bk_inner = n_bk <= 2 * dev.sm_count;
-  p.by_bk = fast_div_by(static_cast<unsigned>(n_bk));
+  p.kv_parts = plan.kv_parts;
+  p.q_parts = plan.q_parts;
   p.by_kblk = fast_div_by(static_cast<unsigned>(p.n_kblk));
-  p.by_pair = fast_div_by(static_cast<unsigned>(p.n_pair));
-  p.by_hkv = fast_div_by(static_cast<unsigned>(p.Hkv));
-  p.by_mt_count = fast_div_by(static_cast<unsigned>(p.n_mt));
-  p.by_mt = fast_div_by(static_cast<unsigned>(p.MT));
-  p.by_gb = fast_div_by(static_cast<unsigned>(p.Gb));
-  p.P = static_cast<int>(P);
-  p.ds = static_cast<int>(a->dead_start);
-  p.de = static_cast<int>(a->dead_end);
-  p.scale_log2 = scale * 1.4426950408889634f;
+  p.by_kv_parts = fast_div_by(static_cast<unsigned>(p.kv_parts));
+  p.by_q_parts = fast_div_by(static_cast<unsigned>(p.q_parts));
   // softmax over a single key is constant: its score's gradient is exactly zero
   p.out_scale = p.N == 1 ? 0.f : scale;
   p.host_err = host_error_word(cs);
   p.lse = args.lse;
   p.stats = static_cast<float*>(workspace);
-  p.counter = reinterpret_cast<unsigned*>(static_cast<uint8_t*>(workspace) + stats_bytes(a));
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  p.counter = reinterpret_cast<unsigned*>(ws + plan.counter);
+  p.kv_sums = reinterpret_cast<float*>(ws + plan.kv_sums);
+  p.q_sums = reinterpret_cast<float*>(ws + plan.q_sums);
   p.o = static_cast<const __nv_bfloat16*>(a->o);
   p.d_o = static_cast<const __nv_bfloat16*>(args.grad_o);
   for (int d = 0; d < 3; ++d) {
@@ -1085,14 +990,6 @@ int run_bwd(const vlak_attn_train_args* t, void* workspace, int64_t ws_bytes, vo
   p.dq = static_cast<__nv_bfloat16*>(args.dq);
   p.dk = static_cast<__nv_bfloat16*>(args.dk);
   p.dv = static_cast<__nv_bfloat16*>(args.dv);
-  p.lengths = args.lengths;
-  p.lengths_i64 = args.lengths_dtype == VLAK_I64;
-  p.mask = static_cast<const uint8_t*>(args.mask);
-  p.mask_sb = args.mask_stride_b;
-  p.mask_sm = args.mask_stride_m;
-  p.mask_words = reinterpret_cast<uintptr_t>(args.mask) % 4 == 0 && args.mask_stride_b % 4 == 0 &&
-                 args.mask_stride_m % 4 == 0;
-
   const uint32_t gb = static_cast<uint32_t>(tl.Gb), mt = static_cast<uint32_t>(tl.MT);
   auto rows = [&](CUtensorMap* m, const void* ptr, const int64_t* s, const char* name) {
     return encode_map(m, ptr, a->H, a->M, a->B, s[2], s[1], s[0], gb, mt, name);
@@ -1148,8 +1045,7 @@ extern "C" int vlak_attn_gqa_bwd_workspace_size(const vlak_attn_train_args* args
   }
   int st = vlak_attn_gqa_check(&a, nullptr, nullptr);
   if (st != VLAK_OK) return st;
-  if (args->attn.B > 0 && args->attn.M > 0 && args->attn.N > 0) 
-    *bytes = stats_bytes(&args->attn) + kCounterBytes;
+  if (a.B > 0 && a.M > 0 && a.N > 0) *bytes = plan_bwd(&a, args->dk || args->dv).bytes;
   return VLAK_OK;
 }
 

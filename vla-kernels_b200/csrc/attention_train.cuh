@@ -1,0 +1,302 @@
+// Shared by the training kernels of GQA attention (attention_train_fwd.cu,
+// attention_bwd.cu): how queries and keys are cut into items and steps, the
+// queue that hands items out, and the issue of tcgen05 products.
+//
+// Query rows are handled in sub-tiles of up to 64 rows, Gb heads x MT positions
+// with Gb a divisor of G, one TMA box each. A row item is two sub-tiles, the 128
+// lanes of a TMEM tile, and walks the keys in chunks of 64.
+#pragma once
+
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include <algorithm>
+
+#include "attention_common.cuh"
+#include "vlak_device.cuh"
+#include "vlak_internal.h"
+
+namespace vlak {
+namespace {
+
+constexpr int kMaskAnalytic = 0, kMaskLength = 1, kMaskBool = 2;
+
+constexpr int kSub = 64;                     // rows of a streamed tile
+constexpr int kRowBytes = 128;               // 64 bf16
+constexpr int kSubBytes = kSub * kRowBytes;  // 8 KB
+constexpr int kChunk = 64;                   // keys of a dq step
+
+// Shape, mask and cutting of a call, common to the kernels' parameters.
+struct TrainShape {
+  int B, M, N, H, Hkv, G;
+  int Gb, MT;                         // heads and positions of a sub-tile
+  int n_mt, n_hblk, n_sub, n_pair, n_chunks;
+  int n_bk;                           // B * Hkv
+  int bk_inner;                       // items run over (b, kv head) first
+  int P, ds, de;
+  float scale, scale_log2;
+  int* host_err;
+  unsigned* counter;                  // next item
+  const void* lengths;
+  int lengths_i64;
+  const uint8_t* mask;
+  long long mask_sb, mask_sm;
+  int mask_words;
+  FastDiv by_bk, by_pair, by_hkv, by_mt_count, by_mt, by_gb;
+};
+
+__device__ __forceinline__ int length_of(const TrainShape& p, int b) {
+  const long long len = p.lengths_i64 ? static_cast<const long long*>(p.lengths)[b]
+                                      : static_cast<const int*>(p.lengths)[b];
+  return static_cast<int>(min(max(len, 0LL), static_cast<long long>(p.N)));
+}
+
+// low n bits set, n clamped to [0, 32]
+__device__ __forceinline__ uint32_t low_bits(int n) {
+  return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : ((1u << n) - 1u);
+}
+
+// A step's 64 bf16 operand columns: each half of them is packed over the first
+// half of the 32 fp32 columns it was computed from, which the warp that packs
+// them has read; so they lie at columns 0-15 and 32-47 (see umma_ts_x4).
+
+// 1024-byte aligned start of the dynamic shared memory
+__device__ __forceinline__ uint8_t* aligned_smem(uint8_t* raw) {
+  return raw + (((smem_u32(raw) + 1023u) & ~1023u) - smem_u32(raw));
+}
+
+// Row `row` of sub-tile st of a (b, kv head): position m, head h within the kv
+// head, and whether it exists.
+struct SubRow {
+  int m, g;
+  bool valid;
+};
+__device__ __forceinline__ SubRow sub_row(const TrainShape& p, int st, int row) {
+  const int hb = fast_div(st, p.by_mt_count), mt = st - hb * p.n_mt;
+  const int local = fast_div(row, p.by_gb);
+  SubRow r;
+  r.m = mt * p.MT + local;
+  r.g = hb * p.Gb + row - local * p.Gb;
+  r.valid = st < p.n_sub && local < p.MT && r.m < p.M;
+  return r;
+}
+
+// ---------------------------------------------------------------------------
+// Items
+
+// An item as the producer hands it out through shared memory (16 bytes at a
+// time).
+struct __align__(16) Item {
+  int live;           // -1: no more items; else its steps
+  int dkv, b, kvh;
+  int L;              // length of the sample (lengths only)
+  int k0;             // dkv: first key
+  int s0, n_here;     // dq: first sub-tile and how many (1 or 2)
+  int a1, b0;         // dq: live chunks [0, a1) and [b0, ...)
+  int mt_lo, mt_hi;   // dkv: live position blocks of each head block
+  int j0, part;       // first of the item's steps, where several parts share them
+  int pad[2];
+};
+static_assert(sizeof(Item) == 64, "four vectors");
+__device__ __forceinline__ Item load_item(const Item* src) {
+  const int4* v = reinterpret_cast<const int4*>(src);
+  const int4 x = v[0], y = v[1], z = v[2], w = v[3];
+  Item it;
+  it.live = x.x; it.dkv = x.y; it.b = x.z; it.kvh = x.w;
+  it.L = y.x; it.k0 = y.y; it.s0 = y.z; it.n_here = y.w;
+  it.a1 = z.x; it.b0 = z.y; it.mt_lo = z.z; it.mt_hi = z.w;
+  it.j0 = w.x; it.part = w.y;
+  return it;
+}
+// Of an item's steps, those of its part: even shares in order.
+__device__ __forceinline__ void take_part(Item& it, int part, int parts) {
+  const int share = (it.live + parts - 1) / parts;
+  it.part = part;
+  it.j0 = min(part * share, it.live);
+  it.live = min(share, it.live - it.j0);
+}
+
+// The steps of an item in order: chunk `pos` (dq), or position block `pos` of
+// head block `hb` (dkv).
+struct Steps {
+  int pos, hb;
+  __device__ __forceinline__ void begin(const Item& it) {
+    hb = 0;
+    pos = it.j0 < it.a1 ? it.j0 : it.j0 - it.a1 + it.b0;
+    if (it.dkv) {
+      const int per_head = it.mt_hi - it.mt_lo;
+      hb = it.j0 > 0 ? it.j0 / per_head : 0;
+      pos = it.mt_lo + it.j0 - hb * per_head;
+    }
+  }
+  __device__ __forceinline__ void next(const Item& it) {
+    ++pos;
+    if (it.dkv) {
+      if (pos == it.mt_hi) {
+        pos = it.mt_lo;
+        ++hb;
+      }
+    } else if (pos == it.a1) {
+      pos = it.b0;
+    }
+  }
+};
+
+// Row item `blk` of a (b, kv head), counted from the last pair of sub-tiles,
+// whose rows see the most keys under a staircase: its rows and live chunks.
+template <int kMode>
+__device__ __forceinline__ void row_item(const TrainShape& p, int blk, Item& it) {
+  it.s0 = 2 * (p.n_pair - 1 - blk);
+  it.n_here = min(2, p.n_sub - it.s0);
+  // first and last position of the rows
+  const int s1 = it.s0 + it.n_here - 1;
+  const int mt0 = it.s0 - fast_div(it.s0, p.by_mt_count) * p.n_mt;
+  const int mt1 = s1 - fast_div(s1, p.by_mt_count) * p.n_mt;
+  const int m_lo = min(mt0, mt1) * p.MT;
+  const int m_hi = min(p.M, (max(mt0, mt1) + 1) * p.MT) - 1;
+  int b1 = 0;
+  if (kMode == kMaskBool) {
+    it.a1 = p.n_chunks;
+  } else if (kMode == kMaskLength) {
+    it.a1 = m_lo < it.L ? (it.L + kChunk - 1) / kChunk : 0;
+  } else {
+    it.a1 = (p.ds + kChunk - 1) / kChunk;
+    if (p.de < p.N) {
+      const int e2 = max(p.P, min(p.N, p.N - p.M + m_hi + 1));
+      it.b0 = max(p.de / kChunk, it.a1);
+      b1 = (e2 + kChunk - 1) / kChunk;
+    }
+  }
+  it.live = it.a1 + max(0, b1 - it.b0);
+}
+
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "@e cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n\t}"
+      ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar))
+      : "memory");
+}
+
+// The four K = 16 products of one 64-deep contraction, from one elected lane.
+// Descriptors step by 32 bytes of a swizzled row (SS, both operands) or by 16
+// rows of 128 bytes (TS, B).
+__device__ __forceinline__ void umma_ss_x4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc) {
+  asm volatile(
+      "{\n\t.reg .pred e, n, y;\n\t.reg .b64 a1, a2, a3, b1, b2, b3;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "setp.ne.b32 n, 0, 0;\n\tsetp.eq.b32 y, 0, 0;\n\t"
+      "add.s64 a1, %1, 2;\n\tadd.s64 a2, %1, 4;\n\tadd.s64 a3, %1, 6;\n\t"
+      "add.s64 b1, %2, 2;\n\tadd.s64 b2, %2, 4;\n\tadd.s64 b3, %2, 6;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, n;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a1, b1, %3, y;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a2, b2, %3, y;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a3, b3, %3, y;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc)
+      : "memory");
+}
+// A in TMEM at columns x + 0, 8, 32, 40; `acc` 0 starts a new sum; `on` 0
+// issues nothing.
+__device__ __forceinline__ void umma_ts_x4(uint32_t d, uint32_t x, uint64_t b, uint32_t idesc,
+                                           uint32_t acc, uint32_t on) {
+  asm volatile(
+      "{\n\t.reg .pred e, q, p, y;\n\t.reg .b32 x1, x2, x3;\n\t.reg .b64 b1, b2, b3;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "setp.ne.and.b32 q, %5, 0, e;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\tsetp.eq.b32 y, 0, 0;\n\t"
+      "add.s32 x1, %1, 8;\n\tadd.s32 x2, %1, 32;\n\tadd.s32 x3, %1, 40;\n\t"
+      "add.s64 b1, %2, 128;\n\tadd.s64 b2, %2, 256;\n\tadd.s64 b3, %2, 384;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [x1], b1, %3, y;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [x2], b2, %3, y;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [x3], b3, %3, y;\n\t}" ::"r"(d),
+      "r"(x), "l"(b), "r"(idesc), "r"(acc), "r"(on)
+      : "memory");
+}
+// A counter modulo n with the parity of its rounds.
+template <int n>
+struct Turn {
+  uint32_t i = 0, round = 0;
+  __device__ __forceinline__ void next() {
+    if (++i == n) {
+      i = 0;
+      round ^= 1;
+    }
+  }
+};
+
+// ---------------------------------------------------------------------------
+// host
+
+// Sub-tiles: the divisor Gb <= 64 of G whose boxes of Gb heads x MT positions
+// need the fewest, the larger one (longer contiguous reads) on a tie.
+struct SubTiling {
+  int Gb, MT, n_mt, n_sub;
+};
+SubTiling sub_tiling(int G, int M) {
+  SubTiling best{};
+  for (int d = 1; d <= std::min(G, kSub); ++d) {
+    if (G % d != 0) continue;
+    const int mt = std::min(kSub / d, M), n_mt = (M + mt - 1) / mt;
+    if (best.Gb == 0 || G / d * n_mt <= best.n_sub) best = SubTiling{d, mt, n_mt, G / d * n_mt};
+  }
+  return best;
+}
+
+// Plans are made for a B200's SMs whatever device is current, so that sizes can
+// be asked without one and results do not depend on it.
+constexpr int kPlanSms = 148;
+inline TrainShape train_shape(const vlak_attn_gqa_args* a, int64_t P, float scale, const SubTiling& t) {
+  TrainShape s{};
+  s.B = static_cast<int>(a->B);
+  s.M = static_cast<int>(a->M);
+  s.N = static_cast<int>(a->N);
+  s.H = static_cast<int>(a->H);
+  s.Hkv = static_cast<int>(a->Hkv);
+  s.G = s.H / s.Hkv;
+  s.Gb = t.Gb;
+  s.MT = t.MT;
+  s.n_mt = t.n_mt;
+  s.n_hblk = t.n_sub / t.n_mt;
+  s.n_sub = t.n_sub;
+  s.n_pair = (t.n_sub + 1) / 2;
+  s.n_chunks = (s.N + kChunk - 1) / kChunk;
+  s.n_bk = static_cast<int>(a->B * a->Hkv);
+  // Few heads: all their long items first, for balance, their tensors stay in
+  // L2. Many: a head's items one after the other, while its tensors are there.
+  s.bk_inner = s.n_bk <= 2 * kPlanSms;
+  s.P = static_cast<int>(P);
+  s.ds = static_cast<int>(a->dead_start);
+  s.de = static_cast<int>(a->dead_end);
+  s.scale = scale;
+  s.scale_log2 = scale * 1.4426950408889634f;
+  s.by_bk = fast_div_by(static_cast<unsigned>(s.n_bk));
+  s.by_pair = fast_div_by(static_cast<unsigned>(s.n_pair));
+  s.by_hkv = fast_div_by(static_cast<unsigned>(s.Hkv));
+  s.by_mt_count = fast_div_by(static_cast<unsigned>(s.n_mt));
+  s.by_mt = fast_div_by(static_cast<unsigned>(s.MT));
+  s.by_gb = fast_div_by(static_cast<unsigned>(s.Gb));
+  return s;
+}
+inline void set_masks(TrainShape& s, const vlak_attn_train_args& a) {
+  s.lengths = a.lengths;
+  s.lengths_i64 = a.lengths_dtype == VLAK_I64;
+  s.mask = static_cast<const uint8_t*>(a.mask);
+  s.mask_sb = a.mask_stride_b;
+  s.mask_sm = a.mask_stride_m;
+  s.mask_words = reinterpret_cast<uintptr_t>(a.mask) % 4 == 0 && a.mask_stride_b % 4 == 0 &&
+                 a.mask_stride_m % 4 == 0;
+}
+// Parts of an item of `steps` steps, in a call of `total` steps: none longer
+// than an SM's even share, but no shorter than eight steps (joining costs
+// about that much), and at most 32.
+inline int item_parts(int64_t steps, int64_t total) {
+  const int64_t most = std::max<int64_t>(8, (total + kPlanSms - 1) / kPlanSms);
+  return static_cast<int>(std::min<int64_t>(32, std::max<int64_t>(1, (steps + most - 1) / most)));
+}
+
+}  // namespace
+}  // namespace vlak
