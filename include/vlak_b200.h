@@ -258,9 +258,9 @@ VLAK_API int vlak_attn_fwd(const void* q, const void* k, const void* v, void* o,
  * that is seen spreads as in the formulas. Results repeat bit for bit.
  *
  * Workspaces: device, 256-byte aligned, owned by the caller and unused by
- * anything else until the work on `stream` has finished. The forward one is
- * optional and sized by vlak_attn_gqa_workspace_size (key splits of small
- * batches); the backward one is required, vlak_attn_gqa_bwd_workspace_size.
+ * anything else until the work on `stream` has finished; sized by the two
+ * functions below (the forward one is 0 bytes, and may be NULL, unless few
+ * heads have many keys).
  * ---------------------------------------------------------------------- */
 typedef struct {
   vlak_attn_gqa_args attn;
@@ -276,6 +276,7 @@ typedef struct {
   int lengths_dtype; /* VLAK_I32 or VLAK_I64 */
 } vlak_attn_train_args;
 
+VLAK_API int vlak_attn_gqa_train_workspace_size(const vlak_attn_train_args* args, int64_t* bytes);
 VLAK_API int vlak_attn_gqa_train_fwd(const vlak_attn_train_args* args, void* workspace,
                                      int64_t workspace_bytes, void* stream);
 VLAK_API int vlak_attn_gqa_bwd_workspace_size(const vlak_attn_train_args* args, int64_t* bytes);

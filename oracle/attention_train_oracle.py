@@ -3,7 +3,7 @@ bf16 kernels may differ by.
 
 Bounds, u = 2^-8 (half a bf16 step) and f = 2^-13 (what the 32-bit parts may
 add relative to a term: scores of 64 products, the exponential, sums):
-  o   u |o| + (2 u + f) sum P |v|      output; P and, in split calls, a part's O
+  o   u |o| + (u + f) sum P |v|        output; P
   D   sum |do| err(o) + f sum |do| |o|
   dS  u |dS| + P err(D) + f P (sum |do| |v| + |D|)
   dv  u |dv| + (u + f) sum P |do|
@@ -44,7 +44,7 @@ def train(q, k, v, do, seen, scale=0.125):
     p = torch.exp(s - lse.clamp_min(-1e300)[..., None])
     p = torch.where(seen[:, None], p, 0.0)
     o = p @ v
-    err_o = U * o.abs() + (2 * U + F) * (p @ v.abs())
+    err_o = U * o.abs() + (U + F) * (p @ v.abs())
     dv, err_dv = p.transpose(2, 3) @ do, p.transpose(2, 3) @ do.abs()
     dp = do @ v.transpose(2, 3)
     D = (do * o).sum(-1, keepdim=True)

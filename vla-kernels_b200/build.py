@@ -33,7 +33,7 @@ TORCH_LIB = os.path.join(LIB_DIR, "libvlak_torch.so")
 CMP_LIB = os.path.join(LIB_DIR, "libvlak_comparators.so")
 
 CU_SOURCES = ["capi.cu", "softmax.cu", "attention_gqa.cu", "attention_simt.cu",
-              "attention_bwd.cu", "rotary.cu"]
+              "attention_train_fwd.cu", "attention_bwd.cu", "rotary.cu"]
 HEADERS = ["vlak_device.cuh", "vlak_internal.h", "attention_common.cuh",
            "attention_train.cuh"]
 SHIM_SOURCES = ["torch_ops.cpp", "torch_rotary.cpp", "torch_attention_train.cpp"]

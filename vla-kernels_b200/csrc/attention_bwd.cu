@@ -901,15 +901,7 @@ int bwd_validate(const vlak_attn_train_args* a, int64_t* P, float* scale) {
       return set_error(VLAK_ERR_ALIGNMENT, "fused_attention_gqa_bwd: grad_o strides must be multiples of 8");
   if (reinterpret_cast<uintptr_t>(a->lse) % 4 != 0)
     return set_error(VLAK_ERR_ALIGNMENT, "fused_attention_gqa_bwd: lse must be 4-byte aligned");
-  if (a->lengths && a->mask)
-    return set_error(VLAK_ERR_INVALID_ARGUMENT, "fused_attention_gqa_bwd: lengths or a mask, not both");
-  if (a->lengths && a->lengths_dtype != VLAK_I32 && a->lengths_dtype != VLAK_I64)
-    return set_error(VLAK_ERR_UNSUPPORTED_DTYPE, "lengths must be int32 or int64");
-  if (reinterpret_cast<uintptr_t>(a->lengths) % (a->lengths_dtype == VLAK_I64 ? 8 : 4) != 0)
-    return set_error(VLAK_ERR_ALIGNMENT, "lengths must be aligned to its element size");
-  if (a->mask && (a->mask_stride_b < 0 || a->mask_stride_m < 0))
-    return set_error(VLAK_ERR_INVALID_ARGUMENT, "attn_mask strides must be non-negative");
-  return VLAK_OK;
+  return check_train_masks(*a, "fused_attention_gqa_bwd");
 }
 
 int run_bwd(const vlak_attn_train_args* t, void* workspace, int64_t ws_bytes, void* stream) {

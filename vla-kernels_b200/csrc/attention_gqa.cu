@@ -62,7 +62,6 @@
 #include <atomic>
 #include <cstring>
 #include <mutex>
-#include <type_traits>
 
 #include "attention_common.cuh"
 #include "vlak_device.cuh"
@@ -171,7 +170,6 @@ struct __align__(64) Params {
   const uint8_t* mask;
   long long mask_sb, mask_sm;  // byte strides of dims b and m
   int mask_words;              // rows start 4-byte aligned: four keys per load
-  float* lse;                  // (B, M, H) log2 of each row's sum of 2^x (kLse)
 };
 
 // Mask modes (a template parameter of the kernel, uniform per launch):
@@ -282,9 +280,7 @@ __device__ __forceinline__ int chunk_cols(const Params& p, int c) {
   return (width + 15) & ~15;  // MMA N must be a multiple of 16
 }
 
-// kLse (the training forward) also stores each row's log2-sum-exp2, and keeps
-// V rows that no query sees out of the products (0 times a NaN there is NaN).
-template <int kMode, bool kSplit, bool kNarrow, bool kLse>
+template <int kMode, bool kSplit, bool kNarrow>
 __global__ void __launch_bounds__(WarpLayout<kNarrow>::kThreads, kCtasPerSm)
 gqa_attention_sm100(const __grid_constant__ Params p) {
   using WL = WarpLayout<kNarrow>;
@@ -491,13 +487,6 @@ gqa_attention_sm100(const __grid_constant__ Params p) {
           // over the S/P columns (in issue order after the product reading P)
           if (!wait_p(0)) { ok = false; break; }
           if (kSplit && !wait_kv(bars->v_full, j)) { ok = false; break; }
-          if (kLse && kMode != kMaskBool) {
-            // keys of the chunk that no row sees: the dead band, or past L
-            const int c0 = cur * kChunk;
-            const int lo = kMode == kMaskLength ? it.L - c0 : p.ds - c0;
-            const int hi = kMode == kMaskLength ? kChunk : p.de - c0;
-            clear_rows(v_smem + (kv + j) % kStages * kChunkBytes, max(lo, 0), min(hi, kChunk));
-          }
           issue_pv(0, cur, j);
           if (nxt >= 0) {
             if (!wait_kv(bars->k_full, j + 1)) { ok = false; break; }
@@ -590,9 +579,6 @@ gqa_attention_sm100(const __grid_constant__ Params p) {
       auto part_row = [&]() {
         return ((static_cast<long long>(it.split) * p.B + it.b) * p.M + m) * p.H + it.kvh * p.G + g;
       };
-      auto lse_row = [&]() {
-        return (static_cast<long long>(it.b) * p.M + m) * p.H + it.kvh * p.G + g;
-      };
       if (!live) {
         // no key visible to any row of the item: zeros, no barrier phase (a
         // split records an empty partial, which the combine skips)
@@ -604,7 +590,6 @@ gqa_attention_sm100(const __grid_constant__ Params p) {
                                 static_cast<long long>(it.kvh * p.G + g) * p.o_sh;
 #pragma unroll
           for (int v = 0; v < 8; ++v) reinterpret_cast<uint4*>(orow)[v] = make_uint4(0, 0, 0, 0);
-          if (kLse) p.lse[lse_row()] = -INFINITY;
         }
         continue;
       }
@@ -792,8 +777,7 @@ gqa_attention_sm100(const __grid_constant__ Params p) {
       tc_fence_after();
       uint8_t* stage = q_smem + qb * kQBytes + t * kTileBytes;
       if (warp_active) {
-        // (the training forward lets a NaN row through, the other writes zeros)
-        const bool any = (j > 0) && (kLse ? l_run != 0.f : l_run > 0.f);
+        const bool any = (j > 0) && (l_run > 0.f);
         const float inv = any ? 1.f / l_run : 0.f;
 #pragma unroll 1
         for (int q4 = 0; q4 < 4; ++q4) {  // 16 columns of O at a time
@@ -816,7 +800,6 @@ gqa_attention_sm100(const __grid_constant__ Params p) {
         }
       }
       if (kSplit && valid) p.part_ml[part_row()] = make_float2(m_run, l_run);
-      if (kLse && !kSplit && valid) p.lse[lse_row()] = l_run != 0.f ? m_run + log2f(l_run) : -INFINITY;
       fence_proxy_async_smem();
       mbar_arrive_elect(&bars->o_staged[t], 1u);
       if (leader) {
@@ -854,9 +837,9 @@ gqa_attention_sm100(const __grid_constant__ Params p) {
   }
 }
 
-// Zero-fill of o for N == 0 (every row fully masked), and of lse with -inf.
+// Zero-fill of o for N == 0 (every row fully masked).
 __global__ void zero_rows(__nv_bfloat16* o, long long o_sb, long long o_sm, long long o_sh, int B,
-                          int M, int H, float* lse) {
+                          int M, int H) {
   const long long rows = static_cast<long long>(B) * M * H;
   for (long long r = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x; r < rows;
        r += static_cast<long long>(gridDim.x) * blockDim.x) {
@@ -864,7 +847,6 @@ __global__ void zero_rows(__nv_bfloat16* o, long long o_sb, long long o_sm, long
     uint4* row = reinterpret_cast<uint4*>(o + b * o_sb + m * o_sm + h * o_sh);
 #pragma unroll
     for (int v = 0; v < 8; ++v) row[v] = make_uint4(0, 0, 0, 0);
-    if (lse != nullptr) lse[r] = -INFINITY;
   }
 }
 
@@ -883,8 +865,7 @@ constexpr int kCombineBatch = 8;
 __global__ void __launch_bounds__(256) combine_splits(const __nv_bfloat16* __restrict__ part,
                                                       const float2* __restrict__ ml,
                                                       __nv_bfloat16* o, long long o_sb, long long o_sm,
-                                                      long long o_sh, int B, int M, int H, int splits,
-                                                      float* lse) {
+                                                      long long o_sh, int B, int M, int H, int splits) {
   // launched as a programmatic dependent of the attention kernel: wait for
   // that grid to complete and its partials to be visible
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -918,7 +899,7 @@ __global__ void __launch_bounds__(256) combine_splits(const __nv_bfloat16* __res
   auto accumulate = [&]() {
 #pragma unroll
     for (int i = 0; i < kCombineBatch; ++i) {
-      if (lse != nullptr ? v[i].y == 0.f : !(v[i].y > 0.f)) continue;
+      if (!(v[i].y > 0.f)) continue;
       const float w = exp2f(v[i].x - mx) * v[i].y;
       wsum += w;
       const uint32_t uw[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
@@ -945,7 +926,6 @@ __global__ void __launch_bounds__(256) combine_splits(const __nv_bfloat16* __res
       accumulate();
     }
   }
-  if (lse != nullptr && q == 0) lse[r] = wsum != 0.f ? mx + log2f(wsum) : -INFINITY;
   const float inv = wsum > 0.f ? 1.f / wsum : 0.f;
   const long long h = r % H, bm = r / H, m = bm % M, b = bm / M;
   uint32_t w[4];
@@ -999,7 +979,6 @@ struct MaskSpec {
   void* workspace = nullptr;  // key-split partials (nullptr: never split)
   int64_t workspace_bytes = 0;
   bool no_alloc = false;      // never set up the host error word here
-  float* lse = nullptr;       // (B, M, H): the training forward
 };
 
 // Query tiling of an item: MT query positions per M-tile, 1 or 2 M-tiles per
@@ -1050,31 +1029,31 @@ static SplitPlan plan_splits(const vlak_attn_gqa_args* a, const Tiling& t, int s
   return sp;
 }
 
-template <int kMode, bool kSplit, bool kNarrow, bool kLse>
+template <int kMode, bool kSplit, bool kNarrow>
 static cudaError_t launch_variant(const Params& prm, int grid, cudaStream_t cs, int device) {
   // one-time per (device, variant) opt-in to the large dynamic shared-memory carve-out
   static std::atomic<int> ready[64];
   if (ready[device].load() == 0) {
-    cudaError_t e = cudaFuncSetAttribute(gqa_attention_sm100<kMode, kSplit, kNarrow, kLse>,
+    cudaError_t e = cudaFuncSetAttribute(gqa_attention_sm100<kMode, kSplit, kNarrow>,
                                          cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
     if (e != cudaSuccess) return e;
     ready[device].store(1);
   }
-  gqa_attention_sm100<kMode, kSplit, kNarrow, kLse>
+  gqa_attention_sm100<kMode, kSplit, kNarrow>
       <<<grid, WarpLayout<kNarrow>::kThreads, kSmemBytes, cs>>>(prm);
   return cudaGetLastError();
 }
-template <int kMode, bool kLse>
+template <int kMode>
 static cudaError_t launch_mode(const Params& prm, int grid, cudaStream_t cs, int device) {
   // the narrow warp layout when the second M-tile holds at most 32 rows
   // (analytic mask only: the sites of the other modes never qualify)
   if constexpr (kMode == kMaskAnalytic) {
     if (prm.tiles == 2 && prm.n_mblk == 1 && (prm.M - prm.MT) * prm.G <= 32)
-      return prm.splits > 1 ? launch_variant<kMode, true, true, kLse>(prm, grid, cs, device)
-                            : launch_variant<kMode, false, true, kLse>(prm, grid, cs, device);
+      return prm.splits > 1 ? launch_variant<kMode, true, true>(prm, grid, cs, device)
+                            : launch_variant<kMode, false, true>(prm, grid, cs, device);
   }
-  return prm.splits > 1 ? launch_variant<kMode, true, false, kLse>(prm, grid, cs, device)
-                        : launch_variant<kMode, false, false, kLse>(prm, grid, cs, device);
+  return prm.splits > 1 ? launch_variant<kMode, true, false>(prm, grid, cs, device)
+                        : launch_variant<kMode, false, false>(prm, grid, cs, device);
 }
 
 static int launch_gqa(const vlak_attn_gqa_args* a_in, void* stream, const MaskSpec& ms = MaskSpec()) {
@@ -1121,7 +1100,7 @@ static int launch_gqa(const vlak_attn_gqa_args* a_in, void* stream, const MaskSp
     const int blocks = static_cast<int>(std::min<long long>((rows + 255) / 256, 4096));
     zero_rows<<<blocks, 256, 0, cs>>>(o, a->o_stride[0], a->o_stride[1], a->o_stride[2],
                                       static_cast<int>(a->B), static_cast<int>(a->M),
-                                      static_cast<int>(a->H), ms.lse);
+                                      static_cast<int>(a->H));
     cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? VLAK_OK : set_cuda_error("fused_attention_gqa zero fill", e);
   }
@@ -1157,7 +1136,6 @@ static int launch_gqa(const vlak_attn_gqa_args* a_in, void* stream, const MaskSp
   prm.de = static_cast<int>(a->dead_end);
   prm.scale_log2 = scale * 1.4426950408889634f;
   prm.host_err = host_error_word(cs, !ms.no_alloc);
-  prm.lse = ms.lse;
   prm.o = o;
   prm.o_sb = a->o_stride[0];
   prm.o_sm = a->o_stride[1];
@@ -1210,13 +1188,9 @@ static int launch_gqa(const vlak_attn_gqa_args* a_in, void* stream, const MaskSp
   if (dev.device >= 64) return set_error(VLAK_ERR_CUDA, "device ordinal out of range");
   const int grid = static_cast<int>(std::min<long long>(items, static_cast<long long>(dev.sm_count) * kCtasPerSm));
 
-  auto launch = [&](auto with_lse) {
-    constexpr bool kLse = decltype(with_lse)::value;
-    return ms.mode == kMaskLength ? launch_mode<kMaskLength, kLse>(prm, grid, cs, dev.device)
-           : ms.mode == kMaskBool ? launch_mode<kMaskBool, kLse>(prm, grid, cs, dev.device)
-                                  : launch_mode<kMaskAnalytic, kLse>(prm, grid, cs, dev.device);
-  };
-  cudaError_t e = ms.lse ? launch(std::true_type()) : launch(std::false_type());
+  cudaError_t e = ms.mode == kMaskLength ? launch_mode<kMaskLength>(prm, grid, cs, dev.device)
+                  : ms.mode == kMaskBool ? launch_mode<kMaskBool>(prm, grid, cs, dev.device)
+                                         : launch_mode<kMaskAnalytic>(prm, grid, cs, dev.device);
   if (e != cudaSuccess) return set_cuda_error("fused_attention_gqa launch failed", e);
   if (sp.splits > 1) {
     const long long threads = static_cast<long long>(a->B) * a->M * a->H * 8;
@@ -1235,8 +1209,7 @@ static int launch_gqa(const vlak_attn_gqa_args* a_in, void* stream, const MaskSp
                            static_cast<const float2*>(prm.part_ml), o,
                            static_cast<long long>(a->o_stride[0]),
                            static_cast<long long>(a->o_stride[1]),
-                           static_cast<long long>(a->o_stride[2]), prm.B, prm.M, prm.H, sp.splits,
-                           ms.lse);
+                           static_cast<long long>(a->o_stride[2]), prm.B, prm.M, prm.H, sp.splits);
     if (e != cudaSuccess) return set_cuda_error("fused_attention_gqa split combine failed", e);
   }
   return VLAK_OK;
@@ -1324,34 +1297,6 @@ extern "C" int vlak_attn_gqa_masked_fwd(const vlak_attn_gqa_args* args, const vo
   ms.mask_sb = mask_stride_b;
   ms.mask_sm = mask_stride_m;
   return vlak::launch_gqa(args, stream, ms);
-}
-
-extern "C" int vlak_attn_gqa_train_fwd(const vlak_attn_train_args* args, void* workspace,
-                                       int64_t workspace_bytes, void* stream) {
-  using namespace vlak;
-  clear_error();
-  if (!args) return set_error(VLAK_ERR_INVALID_ARGUMENT, "fused_attention_gqa_train: null arguments");
-  if (args->lengths && args->mask)
-    return set_error(VLAK_ERR_INVALID_ARGUMENT, "fused_attention_gqa_train: lengths or a mask, not both");
-  if (!args->lse && args->attn.B > 0 && args->attn.M > 0)
-    return set_error(VLAK_ERR_INVALID_ARGUMENT, "fused_attention_gqa_train: lse must not be null");
-  if (reinterpret_cast<uintptr_t>(args->lse) % 4 != 0)
-    return set_error(VLAK_ERR_ALIGNMENT, "fused_attention_gqa_train: lse must be 4-byte aligned");
-  MaskSpec ms;
-  if (args->lengths) {
-    ms.mode = kMaskLength;
-    ms.lengths = args->lengths;
-    ms.lengths_dtype = args->lengths_dtype;
-  } else if (args->mask) {
-    ms.mode = kMaskBool;
-    ms.mask = args->mask;
-    ms.mask_sb = args->mask_stride_b;
-    ms.mask_sm = args->mask_stride_m;
-  }
-  ms.lse = args->lse;
-  ms.workspace = workspace;
-  ms.workspace_bytes = workspace_bytes;
-  return launch_gqa(&args->attn, stream, ms);
 }
 
 extern "C" int vlak_attn_gqa_workspace_size(const vlak_attn_gqa_args* args, int64_t* bytes) {
@@ -1459,10 +1404,13 @@ extern "C" int vlak_device_error_read(int* code) {
   const int zero = 0;
   e = cudaMemcpyToSymbol(vlak::g_device_error, &zero, sizeof(int));
   if (e != cudaSuccess) return vlak::set_cuda_error("vlak_device_error_read", e);
-  int bwd = 0;
-  const int st = vlak::take_bwd_device_error(&bwd);
-  if (st != VLAK_OK) return st;
-  if (v == 0) v = bwd;
+  // the training kernels' words
+  for (int (*take)(int*) : {vlak::take_train_fwd_device_error, vlak::take_bwd_device_error}) {
+    int more = 0;
+    const int st = take(&more);
+    if (st != VLAK_OK) return st;
+    if (v == 0) v = more;
+  }
   // the host-mapped word of the process (cleared as well)
   int h = 0;
   vlak_device_error_poll(&h);

@@ -216,6 +216,18 @@ __device__ __forceinline__ void umma_ts_x4(uint32_t d, uint32_t x, uint64_t b, u
       "r"(x), "l"(b), "r"(idesc), "r"(acc), "r"(on)
       : "memory");
 }
+// Two of them: a 32-deep contraction, A at columns x and x + 8.
+__device__ __forceinline__ void umma_ts_x2(uint32_t d, uint32_t x, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred e, p, y;\n\t.reg .b32 x1;\n\t.reg .b64 b1;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\tsetp.eq.b32 y, 0, 0;\n\t"
+      "add.s32 x1, %1, 8;\n\tadd.s64 b1, %2, 128;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [x1], b1, %3, y;\n\t}" ::"r"(d),
+      "r"(x), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
 // A counter modulo n with the parity of its rounds.
 template <int n>
 struct Turn {
@@ -236,7 +248,7 @@ struct Turn {
 struct SubTiling {
   int Gb, MT, n_mt, n_sub;
 };
-SubTiling sub_tiling(int G, int M) {
+inline SubTiling sub_tiling(int G, int M) {
   SubTiling best{};
   for (int d = 1; d <= std::min(G, kSub); ++d) {
     if (G % d != 0) continue;
@@ -280,6 +292,18 @@ inline TrainShape train_shape(const vlak_attn_gqa_args* a, int64_t P, float scal
   s.by_mt = fast_div_by(static_cast<unsigned>(s.MT));
   s.by_gb = fast_div_by(static_cast<unsigned>(s.Gb));
   return s;
+}
+// The masks of a call beyond the analytic one.
+inline int check_train_masks(const vlak_attn_train_args& a, const char* op) {
+  if (a.lengths && a.mask)
+    return set_errorf(VLAK_ERR_INVALID_ARGUMENT, "%s: lengths or a mask, not both", op);
+  if (a.lengths && a.lengths_dtype != VLAK_I32 && a.lengths_dtype != VLAK_I64)
+    return set_errorf(VLAK_ERR_UNSUPPORTED_DTYPE, "%s: lengths must be int32 or int64", op);
+  if (reinterpret_cast<uintptr_t>(a.lengths) % (a.lengths_dtype == VLAK_I64 ? 8 : 4) != 0)
+    return set_errorf(VLAK_ERR_ALIGNMENT, "%s: lengths must be aligned to its element size", op);
+  if (a.mask && (a.mask_stride_b < 0 || a.mask_stride_m < 0))
+    return set_errorf(VLAK_ERR_INVALID_ARGUMENT, "%s: attn_mask strides must be non-negative", op);
+  return VLAK_OK;
 }
 inline void set_masks(TrainShape& s, const vlak_attn_train_args& a) {
   s.lengths = a.lengths;

@@ -101,9 +101,13 @@ std::tuple<Tensor, Tensor> fwd_lse(const Tensor& q_in, const Tensor& k_in, const
   set_o(a, o);
   vlak_attn_train_args t = train_args(a, m);
   t.lse = lse.data_ptr<float>();
-  const Tensor ws = vlak_torch::split_workspace(a, q);
-  check_status(vlak_attn_gqa_train_fwd(&t, vlak_torch::ws_ptr(ws), vlak_torch::ws_bytes(ws), stream()),
-               op);
+  // workspaces: from the caching allocator on the current stream, so reused only
+  // by work queued behind this call there, and a captured graph's own while it lives
+  int64_t bytes = 0;
+  check_status(vlak_attn_gqa_train_workspace_size(&t, &bytes), op);
+  Tensor ws;
+  if (bytes > 0) ws = at::empty({bytes}, q.options().dtype(at::kByte));
+  check_status(vlak_attn_gqa_train_fwd(&t, bytes > 0 ? ws.data_ptr() : nullptr, bytes, stream()), op);
   return {o, lse};
 }
 
@@ -150,8 +154,6 @@ std::vector<Tensor> bwd(const Tensor& grad_o_in, const Tensor& q_in, const Tenso
   }
   int64_t bytes = 0;
   check_status(vlak_attn_gqa_bwd_workspace_size(&t, &bytes), op);
-  // from the caching allocator on the current stream: reused only by work
-  // queued behind this call there, and a captured graph's own while it lives
   const Tensor ws = at::empty({bytes}, q.options().dtype(at::kByte));
   check_status(vlak_attn_gqa_bwd(&t, ws.data_ptr(), bytes, stream()), op);
   return out;

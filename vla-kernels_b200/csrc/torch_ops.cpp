@@ -61,19 +61,6 @@ vlak_attn_gqa_args gqa_args(const at::Tensor& q, const at::Tensor& k, const at::
   return a;
 }
 
-// Key-split workspace for small batches, from the caching allocator on the
-// current stream (its memory is reused only by work queued after this call
-// on that stream). Undefined when the launch will not split.
-at::Tensor split_workspace(const vlak_attn_gqa_args& a, const at::Tensor& like) {
-  int64_t bytes = 0;
-  check_status(vlak_attn_gqa_workspace_size(&a, &bytes), "fused_attention workspace size");
-  if (bytes == 0) return at::Tensor();
-  return at::empty({bytes}, like.options().dtype(at::kByte));
-}
-// workspace pointer and bytes as the C ABI wants them
-void* ws_ptr(const at::Tensor& ws) { return ws.defined() ? ws.data_ptr() : nullptr; }
-int64_t ws_bytes(const at::Tensor& ws) { return ws.defined() ? ws.numel() : 0; }
-
 }  // namespace vlak_torch
 
 namespace {
@@ -82,9 +69,6 @@ using vlak_torch::check_status;
 using vlak_torch::dtype_code;
 using vlak_torch::gqa_args;
 using vlak_torch::raise_pending_device_error;
-using vlak_torch::split_workspace;
-using vlak_torch::ws_bytes;
-using vlak_torch::ws_ptr;
 
 // vlak::device_error(): the synchronous check. Waits for the device, then
 // reads and clears the error words; returns the status found (0 = none).
@@ -111,6 +95,18 @@ at::Tensor softmax_lastdim(const at::Tensor& x_in, int64_t version) {
   check_status(st, "softmax kernel launch failed");
   return y;
 }
+
+// Key-split workspace for small batches, from the caching allocator on the
+// current stream (its memory is reused only by work queued after this call
+// on that stream). Undefined when the launch will not split.
+at::Tensor split_workspace(const vlak_attn_gqa_args& a, const at::Tensor& like) {
+  int64_t bytes = 0;
+  check_status(vlak_attn_gqa_workspace_size(&a, &bytes), "fused_attention workspace size");
+  if (bytes == 0) return at::Tensor();
+  return at::empty({bytes}, like.options().dtype(at::kByte));
+}
+void* ws_ptr(const at::Tensor& ws) { return ws.defined() ? ws.data_ptr() : nullptr; }
+int64_t ws_bytes(const at::Tensor& ws) { return ws.defined() ? ws.numel() : 0; }
 
 at::Tensor run_gqa(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, double scale,
                    int64_t prefix_len, int64_t dead_start, int64_t dead_end, bool v4) {

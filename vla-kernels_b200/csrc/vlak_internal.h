@@ -40,8 +40,9 @@ int current_device_info(DeviceInfo* out);
 // may_allocate false it only returns a word set up earlier (or nullptr).
 int* host_error_word(cudaStream_t stream, bool may_allocate = true);
 
-// Reads and clears the backward kernels' per-device error word (part of
+// Read and clear the training kernels' per-device error words (part of
 // vlak_device_error_read).
+int take_train_fwd_device_error(int* code);
 int take_bwd_device_error(int* code);
 
 }  // namespace vlak

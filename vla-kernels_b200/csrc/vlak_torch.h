@@ -34,13 +34,9 @@ inline int dtype_code(at::ScalarType t) {
   }
 }
 
-// Checks and arguments of the GQA attention ops (torch_ops.cpp), and the
-// key-split workspace of a forward call, undefined when it will not split.
+// Checks and arguments of the GQA attention ops (torch_ops.cpp).
 vlak_attn_gqa_args gqa_args(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
                             double scale, int64_t prefix_len, int64_t dead_start,
                             int64_t dead_end, const char* op);
-at::Tensor split_workspace(const vlak_attn_gqa_args& a, const at::Tensor& like);
-void* ws_ptr(const at::Tensor& ws);
-int64_t ws_bytes(const at::Tensor& ws);
 
 }  // namespace vlak_torch
