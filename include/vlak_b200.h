@@ -247,6 +247,10 @@ VLAK_API int vlak_attn_fwd(const void* q, const void* k, const void* v, void* o,
  *   lse      : contiguous (B, M, H) fp32: log2 of the sum of 2^(scale log2(e)
  *              q.k) over the keys a row sees, -inf for a row that sees none;
  *              written by the forward call and read by the backward call
+ *   o_low    : NULL, or contiguous (B, M, H, 64) bytes, 16-byte aligned: eight
+ *              more bits of each entry of o, written by the forward call for the
+ *              backward one. Without it dq and dk lose precision where a row's
+ *              weight lies on few keys (D = rowsum(grad_o * o) takes o's rounding)
  *   grad_o   : gradient of o, bf16, strides as q (backward only)
  *   dq       : contiguous (B, M, H, 64) bf16 (backward only)
  *   dk, dv   : contiguous (B, N, Hkv, 64) bf16, summed over the G query heads
@@ -268,6 +272,7 @@ typedef struct {
   const void* mask;
   int64_t mask_stride_b, mask_stride_m;
   float* lse;
+  void* o_low;
   const void* grad_o;
   int64_t grad_o_stride[3];
   void* dq;

@@ -4,7 +4,7 @@ bf16 kernels may differ by.
 Bounds, u = 2^-8 (half a bf16 step) and f = 2^-13 (what the 32-bit parts may
 add relative to a term: scores of 64 products, the exponential, sums):
   o   u |o| + (u + f) sum P |v|        output; P
-  D   sum |do| err(o) + f sum |do| |o|
+  D   f sum |do| (|o| + sum P |v|) + u sum |do| sum P |v|: of o only the rounding of P
   dS  u |dS| + P err(D) + f P (sum |do| |v| + |D|)
   dv  u |dv| + (u + f) sum P |do|
   dq  u |dq| + scale sum err(dS) |k|
@@ -48,7 +48,7 @@ def train(q, k, v, do, seen, scale=0.125):
     dv, err_dv = p.transpose(2, 3) @ do, p.transpose(2, 3) @ do.abs()
     dp = do @ v.transpose(2, 3)
     D = (do * o).sum(-1, keepdim=True)
-    err_D = (do.abs() * (err_o + F * o.abs())).sum(-1, keepdim=True)
+    err_D = (do.abs() * (F * o.abs() + (U + F) * (p @ v.abs()))).sum(-1, keepdim=True)
     ds = p * (dp - D)
     err_ds = U * ds.abs() + p * (err_D + F * (do.abs() @ v.abs().transpose(2, 3) + D.abs()))
     dq, dk = scale * ds @ k, scale * ds.transpose(2, 3) @ q

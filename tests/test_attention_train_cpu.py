@@ -13,7 +13,7 @@ from tests import capi
 class TrainArgs(ctypes.Structure):
     _fields_ = [("attn", capi.GqaArgs), ("lengths", ctypes.c_void_p), ("mask", ctypes.c_void_p),
                 ("mask_stride_b", ctypes.c_int64), ("mask_stride_m", ctypes.c_int64),
-                ("lse", ctypes.c_void_p), ("grad_o", ctypes.c_void_p),
+                ("lse", ctypes.c_void_p), ("o_low", ctypes.c_void_p), ("grad_o", ctypes.c_void_p),
                 ("grad_o_stride", ctypes.c_int64 * 3), ("dq", ctypes.c_void_p),
                 ("dk", ctypes.c_void_p), ("dv", ctypes.c_void_p), ("lengths_dtype", ctypes.c_int)]
 
@@ -45,7 +45,7 @@ def args(attn=(), **kw):
 
 BAD_ATTN = [dict(H=16), dict(Hkv=0), dict(B=-1), dict(prefix_len=292), dict(q=0x1008),
             dict(dead_start=5, dead_end=4), dict(dead_end=242), dict(H=645)]
-BAD = [dict(lse=0x1002), dict(lengths=0x1000, mask=0x1000), dict(lengths=0x1004),
+BAD = [dict(lse=0x1002), dict(o_low=0x1008), dict(lengths=0x1000, mask=0x1000), dict(lengths=0x1004),
        dict(lengths=0x1000, lengths_dtype=2), dict(mask=0x1000, mask_stride_b=-1), dict(lse=None)]
 
 
@@ -107,9 +107,10 @@ def test_fakes():
         q, k, v = x[:, :, :15], x[:, :, 15:20], x[:, :, 20:]
         o = attention.fused_attention_gqa_train(q, k, v)
         assert o.shape == q.shape and o.is_contiguous()
-        o, lse = torch.ops.vlak.fused_attention_gqa_fwd_lse(q, k, v)
+        o, lse, low = torch.ops.vlak.fused_attention_gqa_fwd_lse(q, k, v)
         assert lse.shape == (2, 50, 15) and lse.dtype == torch.float32
-        d = torch.ops.vlak.fused_attention_gqa_bwd(o, q, k, v, o, lse)
+        assert low.shape == q.shape and low.dtype == torch.int8
+        d = torch.ops.vlak.fused_attention_gqa_bwd(o, q, k, v, o, lse, low)
         assert [t.shape for t in d] == [q.shape, k.shape, v.shape]
         assert all(t.is_contiguous() for t in d)
-        assert len(torch.ops.vlak.fused_attention_gqa_bwd(o, q, k, v, o, lse, with_kv=False)) == 1
+        assert len(torch.ops.vlak.fused_attention_gqa_bwd(o, q, k, v, o, lse, low, with_kv=False)) == 1

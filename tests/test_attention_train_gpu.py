@@ -114,6 +114,21 @@ def test_large_scores_and_scale():
     run(1, 70, 150, 4, 2, 40, 0, 0, scale=1e-3)
 
 
+@pytest.mark.parametrize("N", [2, 3, 5, 9])
+def test_few_keys_keep_their_precision(N):
+    # where a row's weight lies on few keys, D = rowsum(do * o) is as large as dP:
+    # with o rounded to bf16, its error would be that of dS once more. The
+    # gradients' roundings here: P, dS, and the result's, so 2^-8 of the norm
+    # (three times 2^-8 / sqrt(3) in the mean square)
+    q, k, v, do = make(4, 400, N, 8, 4, seed=N)
+    got = step(q, k, v, do)
+    ref = orc.train(q, k, v, do, orc.analytic(400, N, N))
+    check(got, ref)
+    for name, x in zip(("dq", "dk"), got[1:]):
+        want = ref[name][0]
+        assert (x.double() - want).norm() <= 2.0 ** -8 * want.norm()
+
+
 def test_one_key_has_no_score_gradient():
     for kw in ({}, dict(P=0)):
         got = run(2, 9, 1, 6, 2, **kw)
@@ -240,7 +255,7 @@ def test_log_sums():
     attention._ensure_registered_train()
     for B, M, N, P in ((2, 90, 40, 0), (1, 50, 700, 600), (40, 50, 291, 241)):
         q, k, v, do = make(B, M, N, H, Hkv)
-        _, lse = torch.ops.vlak.fused_attention_gqa_fwd_lse(q, k, v, -1.0, P, 0, 0)
+        _, lse, _ = torch.ops.vlak.fused_attention_gqa_fwd_lse(q, k, v, -1.0, P, 0, 0)
         want = orc.train(q, k, v, do, orc.analytic(M, N, P))["lse"][0]
         empty = want.isinf()
         assert torch.equal(lse.double()[empty], want[empty])
@@ -461,10 +476,11 @@ def test_refusals():
         with pytest.raises((RuntimeError, NotImplementedError)):
             call()
             pytest.fail(f"case {i} was accepted")
-    o, lse = torch.ops.vlak.fused_attention_gqa_fwd_lse(q, k, v)
-    for args in ((do.float(), q, k, v, o, lse), (do[:1], q, k, v, o, lse),
-                 (do, q, k, v, o[:, :5], lse), (do, q, k, v, o, lse[:1]),
-                 (do, q, k, v, o, lse.double())):
+    o, lse, low = torch.ops.vlak.fused_attention_gqa_fwd_lse(q, k, v)
+    for args in ((do.float(), q, k, v, o, lse, low), (do[:1], q, k, v, o, lse, low),
+                 (do, q, k, v, o[:, :5], lse, low), (do, q, k, v, o, lse[:1], low),
+                 (do, q, k, v, o, lse.double(), low), (do, q, k, v, o, lse, low[:1]),
+                 (do, q, k, v, o, lse, low.float())):
         with pytest.raises(RuntimeError):
             torch.ops.vlak.fused_attention_gqa_bwd(*args)
     # differentiable once

@@ -98,6 +98,7 @@ struct __align__(64) BwdParams : TrainShape {
   CUtensorMap tm_k, tm_v, tm_dk, tm_dv;      // the same, box (64, 1, 128, 1)
   __nv_bfloat16 *dq, *dk, *dv;               // contiguous
   const __nv_bfloat16 *o, *d_o;
+  const int8_t* o_low;                       // contiguous (B, M, H, 64), or null
   long long o_s[3], do_s[3];                 // (b, m, h) element strides
   const float* lse;                          // (B, M, H), log2 units
   float* stats;                              // [B * Hkv][n_sub][-lse 64, -D 64]
@@ -111,8 +112,8 @@ struct __align__(64) BwdParams : TrainShape {
 };
 
 // ---------------------------------------------------------------------------
-// D = rowsum(dO * O) and -lse by sub-tile rows: four threads per row, two 16-byte
-// vectors of each tensor per thread. Rows that do not exist or see no key get
+// D = rowsum(dO * O), O with its low bytes, and -lse by sub-tile rows: four
+// threads per row, two 16-byte vectors of each tensor per thread. Rows that do not exist or see no key get
 // -lse = -inf (every P is 0) and D = 0, whatever memory holds there. Bound: HBM,
 // one read of O and dO.
 constexpr int kStatThreads = 4 * kSub;
@@ -127,10 +128,17 @@ __global__ void __launch_bounds__(kStatThreads) attn_bwd_stats(const __grid_cons
   const int h = kvh * p.G + r.g;
   float nl = -INFINITY, d = 0.f;
   if (r.valid) {
-    const float lse = p.lse[(static_cast<long long>(b) * p.M + r.m) * p.H + h];
+    const long long at = (static_cast<long long>(b) * p.M + r.m) * p.H + h;
+    const float lse = p.lse[at];
     const uint4* x = reinterpret_cast<const uint4*>(p.o + b * p.o_s[0] + r.m * p.o_s[1] + h * p.o_s[2]);
     const uint4* y = reinterpret_cast<const uint4*>(p.d_o + b * p.do_s[0] + r.m * p.do_s[1] + h * p.do_s[2]);
     const uint4 xv[2] = {x[v], x[v + 4]}, yv[2] = {y[v], y[v + 4]};
+    uint2 low[2] = {make_uint2(0u, 0u), make_uint2(0u, 0u)};
+    if (p.o_low != nullptr) {
+      const uint2* l = reinterpret_cast<const uint2*>(p.o_low + at * 64);
+      low[0] = l[v];
+      low[1] = l[v + 4];
+    }
     if (lse != -INFINITY) {
       nl = -lse;
 #pragma unroll
@@ -138,6 +146,8 @@ __global__ void __launch_bounds__(kStatThreads) attn_bwd_stats(const __grid_cons
         float fx[8], fy[8];
         Elem<__nv_bfloat16>::unpack(xv[k], fx);
         Elem<__nv_bfloat16>::unpack(yv[k], fy);
+        with_low_bytes(fx, low[k].x);
+        with_low_bytes(fx + 4, low[k].y);
 #pragma unroll
         for (int i = 0; i < 8; ++i) d += fx[i] * fy[i];
       }
@@ -899,8 +909,9 @@ int bwd_validate(const vlak_attn_train_args* a, int64_t* P, float* scale) {
   for (int d = 0; d < 3; ++d)
     if (a->grad_o_stride[d] % 8 != 0)
       return set_error(VLAK_ERR_ALIGNMENT, "fused_attention_gqa_bwd: grad_o strides must be multiples of 8");
-  if (reinterpret_cast<uintptr_t>(a->lse) % 4 != 0)
-    return set_error(VLAK_ERR_ALIGNMENT, "fused_attention_gqa_bwd: lse must be 4-byte aligned");
+  if (reinterpret_cast<uintptr_t>(a->lse) % 4 != 0 || reinterpret_cast<uintptr_t>(a->o_low) % 16 != 0)
+    return set_error(VLAK_ERR_ALIGNMENT,
+                     "fused_attention_gqa_bwd: lse must be 4-byte, o_low 16-byte aligned");
   return check_train_masks(*a, "fused_attention_gqa_bwd");
 }
 
@@ -975,6 +986,7 @@ int run_bwd(const vlak_attn_train_args* t, void* workspace, int64_t ws_bytes, vo
   p.q_sums = reinterpret_cast<float*>(ws + plan.q_sums);
   p.o = static_cast<const __nv_bfloat16*>(a->o);
   p.d_o = static_cast<const __nv_bfloat16*>(args.grad_o);
+  p.o_low = static_cast<const int8_t*>(args.o_low);
   for (int d = 0; d < 3; ++d) {
     p.o_s[d] = a->o_stride[d];
     p.do_s[d] = args.grad_o_stride[d];

@@ -240,6 +240,27 @@ struct Turn {
   }
 };
 
+// O beyond its bf16 rounding. D = rowsum(dO * O) is a sum in which the bf16
+// rounding of O would weigh as much as that of dS where a row's weight lies on
+// few keys, so the forward pass keeps the next eight bits of each entry of O: the
+// distance of the 32-bit value from its bf16 one, as integers, in units of 2^8.
+__device__ __forceinline__ uint32_t low_bytes(const float* x, const uint32_t* hi) {  // of four entries
+  uint32_t w = 0u;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int top = static_cast<int>(i & 1 ? hi[i >> 1] & 0xffff0000u : hi[i >> 1] << 16);
+    const int d = (__float_as_int(x[i]) - top + 128) >> 8;
+    w |= (static_cast<uint32_t>(max(-128, min(127, d))) & 0xffu) << (8 * i);
+  }
+  return w;
+}
+// the four entries again, from their bf16 values and the word of low_bytes
+__device__ __forceinline__ void with_low_bytes(float* x, uint32_t w) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    x[i] = __int_as_float(__float_as_int(x[i]) + (static_cast<int>(w << (24 - 8 * i)) >> 24 << 8));
+}
+
 // ---------------------------------------------------------------------------
 // host
 

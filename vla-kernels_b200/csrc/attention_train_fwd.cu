@@ -72,6 +72,7 @@ struct __align__(64) FwdParams : TrainShape {
   CUtensorMap tm_k, tm_v;                    // dims (64, Hkv, N, B), box (64, 1, 64, 1)
   float* lse;                                // (B, M, H), log2 units
   __nv_bfloat16* o;
+  int8_t* o_low;                             // contiguous (B, M, H, 64), or null
   long long o_s[3];                          // (b, m, h) element strides
   int parts;                                 // of an item's steps; with several:
   float* sums;                               // [part][B * Hkv][n_sub * 64][64] O
@@ -508,6 +509,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_train_fwd(const __grid_const
       tc_fence_after();
       uint8_t* a0 = a_smem + ab.i * kTileBytes;
       float* sums = p.parts > 1 ? p.sums + part_row * 64 : nullptr;
+      uint4 low = make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll 1
       for (int q = 0; q < 4; ++q) {  // 16 columns at a time
         float o[16];
@@ -536,6 +538,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_train_fwd(const __grid_const
           }
         } else {
           uint8_t* stage = a0 + tl * kRowBytes;
+          uint32_t lo[4];
 #pragma unroll
           for (int v = 0; v < 2; ++v) {
             uint32_t pk[4];
@@ -544,6 +547,17 @@ __global__ void __launch_bounds__(kThreads, 1) attn_train_fwd(const __grid_const
               pk[e] = L == 0.f ? 0u : pack_bf16x2(o[v * 8 + 2 * e], o[v * 8 + 2 * e + 1]);
             const uint32_t c = static_cast<uint32_t>(2 * q + v) ^ static_cast<uint32_t>(tl & 7);
             st_shared_v4(stage + c * 16, pk[0], pk[1], pk[2], pk[3]);
+            lo[2 * v] = low_bytes(o + 8 * v, pk);
+            lo[2 * v + 1] = low_bytes(o + 8 * v + 4, pk + 2);
+          }
+          if (p.o_low != nullptr && r.valid) {  // whole 32-byte sectors
+            const uint4 now = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+            if (q & 1) {
+              uint4* dst = reinterpret_cast<uint4*>(p.o_low + row * 64 + 16 * (q - 1));
+              dst[0] = low;
+              dst[1] = now;
+            }
+            low = now;
           }
         }
       }
@@ -612,10 +626,14 @@ __global__ void __launch_bounds__(256) attn_train_fwd_join(const __grid_constant
   }
   const int b = fast_div(bk, p.by_hkv), kvh = bk - b * p.Hkv, h = kvh * p.G + r.g;
   const float inv = L == 0.f ? 0.f : 1.f / L;
+  const long long row = (static_cast<long long>(b) * p.M + r.m) * p.H + h;
+  const float x[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
+  const uint32_t hi[2] = {pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3])};
   *reinterpret_cast<uint2*>(p.o + b * p.o_s[0] + r.m * p.o_s[1] + h * p.o_s[2] + 4 * v) =
-      make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
+      make_uint2(hi[0], hi[1]);
+  if (p.o_low != nullptr) *reinterpret_cast<uint32_t*>(p.o_low + row * 64 + 4 * v) = low_bytes(x, hi);
   if (v == 0)
-    p.lse[(static_cast<long long>(b) * p.M + r.m) * p.H + h] = L == 0.f ? -INFINITY : m + log2f(L);
+    p.lse[row] = L == 0.f ? -INFINITY : m + log2f(L);
 }
 
 // N == 0: zeros, and log-sums of -inf.
@@ -692,6 +710,8 @@ int run_fwd(const vlak_attn_train_args* t, void* workspace, int64_t ws_bytes, vo
     return set_errorf(VLAK_ERR_ALIGNMENT, "%s: lse must be 4-byte aligned", op);
   const int64_t rows = a->B * a->M * a->H;
   if (rows == 0) return VLAK_OK;
+  if (reinterpret_cast<uintptr_t>(args.o_low) % 16 != 0)
+    return set_errorf(VLAK_ERR_ALIGNMENT, "%s: o_low must be 16-byte aligned", op);
   if (!a->o || !args.lse || (a->N > 0 && (!a->q || !a->k || !a->v)))
     return set_errorf(VLAK_ERR_INVALID_ARGUMENT, "%s: null tensor pointer", op);
   cudaStream_t cs = static_cast<cudaStream_t>(stream);
@@ -726,6 +746,7 @@ int run_fwd(const vlak_attn_train_args* t, void* workspace, int64_t ws_bytes, vo
   p.host_err = host_error_word(cs);
   p.lse = args.lse;
   p.o = o;
+  p.o_low = static_cast<int8_t*>(args.o_low);
   for (int d = 0; d < 3; ++d) p.o_s[d] = a->o_stride[d];
   p.parts = plan.parts;
   p.sums = static_cast<float*>(workspace);

@@ -85,10 +85,11 @@ void set_o(vlak_attn_gqa_args& a, const Tensor& o) {
 
 void* stream() { return c10::cuda::getCurrentCUDAStream().stream(); }
 
-std::tuple<Tensor, Tensor> fwd_lse(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in,
-                                   double scale, int64_t prefix_len, int64_t dead_start,
-                                   int64_t dead_end, const OptTensor& lengths,
-                                   const OptTensor& attn_mask) {
+// o, its rows' log-sums, and (for a backward pass) its low bytes
+std::tuple<Tensor, Tensor, Tensor> forward(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in,
+                                           double scale, int64_t prefix_len, int64_t dead_start,
+                                           int64_t dead_end, const OptTensor& lengths,
+                                           const OptTensor& attn_mask, bool for_backward) {
   const char* op = "fused_attention_gqa_train";
   raise_pending_device_error(op);
   const Tensor q = stepped(q_in), k = stepped(k_in), v = stepped(v_in);
@@ -98,9 +99,14 @@ std::tuple<Tensor, Tensor> fwd_lse(const Tensor& q_in, const Tensor& k_in, const
   check_status(vlak_attn_gqa_check(&a, nullptr, nullptr), op);
   Tensor o = at::empty({a.B, a.M, a.H, 64}, q.options());
   Tensor lse = at::empty({a.B, a.M, a.H}, q.options().dtype(at::kFloat));
+  Tensor o_low;
   set_o(a, o);
   vlak_attn_train_args t = train_args(a, m);
   t.lse = lse.data_ptr<float>();
+  if (for_backward) {
+    o_low = at::empty({a.B, a.M, a.H, 64}, q.options().dtype(at::kChar));
+    t.o_low = o_low.data_ptr();
+  }
   // workspaces: from the caching allocator on the current stream, so reused only
   // by work queued behind this call there, and a captured graph's own while it lives
   int64_t bytes = 0;
@@ -108,12 +114,20 @@ std::tuple<Tensor, Tensor> fwd_lse(const Tensor& q_in, const Tensor& k_in, const
   Tensor ws;
   if (bytes > 0) ws = at::empty({bytes}, q.options().dtype(at::kByte));
   check_status(vlak_attn_gqa_train_fwd(&t, bytes > 0 ? ws.data_ptr() : nullptr, bytes, stream()), op);
-  return {o, lse};
+  return {o, lse, o_low};
+}
+
+std::tuple<Tensor, Tensor, Tensor> fwd_lse(const Tensor& q, const Tensor& k, const Tensor& v,
+                                           double scale, int64_t prefix_len, int64_t dead_start,
+                                           int64_t dead_end, const OptTensor& lengths,
+                                           const OptTensor& attn_mask) {
+  return forward(q, k, v, scale, prefix_len, dead_start, dead_end, lengths, attn_mask, true);
 }
 
 // [dq, dk, dv], or [dq] without with_kv
 std::vector<Tensor> bwd(const Tensor& grad_o_in, const Tensor& q_in, const Tensor& k_in,
-                        const Tensor& v_in, const Tensor& o_in, const Tensor& lse, double scale,
+                        const Tensor& v_in, const Tensor& o_in, const Tensor& lse,
+                        const Tensor& o_low, double scale,
                         int64_t prefix_len, int64_t dead_start, int64_t dead_end,
                         const OptTensor& lengths, const OptTensor& attn_mask, bool with_kv) {
   const char* op = "fused_attention_gqa_bwd";
@@ -129,6 +143,9 @@ std::vector<Tensor> bwd(const Tensor& grad_o_in, const Tensor& q_in, const Tenso
                   lse.size(0) == a.B && lse.size(1) == a.M && lse.size(2) == a.H &&
                   lse.is_contiguous(),
               op, ": lse must be the contiguous float32 (B, M, H) of the forward call");
+  TORCH_CHECK(o_low.device() == q.device() && o_low.scalar_type() == at::kChar &&
+                  o_low.sizes() == q.sizes() && o_low.is_contiguous(),
+              op, ": o_low must be the contiguous int8 tensor of the forward call");
   c10::cuda::CUDAGuard guard(q.device());
   // a gradient arrives in whatever layout its consumer left it in
   auto tma_ready = [](const Tensor& t) {
@@ -143,6 +160,7 @@ std::vector<Tensor> bwd(const Tensor& grad_o_in, const Tensor& q_in, const Tenso
   std::vector<Tensor> out{at::empty({a.B, a.M, a.H, 64}, q.options())};
   vlak_attn_train_args t = train_args(a, m);
   t.lse = lse.data_ptr<float>();
+  t.o_low = o_low.data_ptr();
   t.grad_o = grad_o.data_ptr();
   for (int d = 0; d < 3; ++d) t.grad_o_stride[d] = grad_o.stride(d);
   t.dq = out[0].data_ptr();
@@ -162,7 +180,8 @@ std::vector<Tensor> bwd(const Tensor& grad_o_in, const Tensor& q_in, const Tenso
 Tensor train(const Tensor& q, const Tensor& k, const Tensor& v, double scale, int64_t prefix_len,
              int64_t dead_start, int64_t dead_end, const OptTensor& lengths,
              const OptTensor& attn_mask) {
-  return std::get<0>(fwd_lse(q, k, v, scale, prefix_len, dead_start, dead_end, lengths, attn_mask));
+  return std::get<0>(
+      forward(q, k, v, scale, prefix_len, dead_start, dead_end, lengths, attn_mask, false));
 }
 
 // ---------------------------------------------------------------------------
@@ -184,8 +203,8 @@ struct TrainFunction : torch::autograd::Function<TrainFunction> {
                           const std::optional<Variable>& attn_mask) {
     static auto op = typed_op<decltype(fwd_lse)>("vlak::fused_attention_gqa_fwd_lse");
     at::AutoDispatchBelowADInplaceOrView below;
-    auto [o, lse] = op.call(q, k, v, scale, prefix_len, dead_start, dead_end, lengths, attn_mask);
-    ctx->save_for_backward({q, k, v, o, lse, lengths.value_or(Variable()),
+    auto [o, lse, o_low] = op.call(q, k, v, scale, prefix_len, dead_start, dead_end, lengths, attn_mask);
+    ctx->save_for_backward({q, k, v, o, lse, o_low, lengths.value_or(Variable()),
                             attn_mask.value_or(Variable())});
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["prefix_len"] = prefix_len;
@@ -199,9 +218,9 @@ struct TrainFunction : torch::autograd::Function<TrainFunction> {
     auto optional = [](const Variable& t) { return t.defined() ? OptTensor(t) : std::nullopt; };
     const bool with_kv = ctx->needs_input_grad(1) || ctx->needs_input_grad(2);
     const std::vector<Tensor> d =
-        op.call(g[0], s[0], s[1], s[2], s[3], s[4], ctx->saved_data["scale"].toDouble(),
+        op.call(g[0], s[0], s[1], s[2], s[3], s[4], s[5], ctx->saved_data["scale"].toDouble(),
                 ctx->saved_data["prefix_len"].toInt(), ctx->saved_data["dead_start"].toInt(),
-                ctx->saved_data["dead_end"].toInt(), optional(s[5]), optional(s[6]), with_kv);
+                ctx->saved_data["dead_end"].toInt(), optional(s[6]), optional(s[7]), with_kv);
     variable_list out(9);
     out[0] = d[0];
     if (with_kv) {
@@ -232,9 +251,10 @@ TORCH_LIBRARY_FRAGMENT(vlak, m) {
   m.def(
       "fused_attention_gqa_fwd_lse(Tensor q, Tensor k, Tensor v, float scale=-1., "
       "int prefix_len=-1, int dead_start=0, int dead_end=0, Tensor? lengths=None, "
-      "Tensor? attn_mask=None) -> (Tensor, Tensor)");
+      "Tensor? attn_mask=None) -> (Tensor, Tensor, Tensor)");
   m.def(
       "fused_attention_gqa_bwd(Tensor grad_o, Tensor q, Tensor k, Tensor v, Tensor o, Tensor lse, "
+      "Tensor o_low, "
       "float scale=-1., int prefix_len=-1, int dead_start=0, int dead_end=0, "
       "Tensor? lengths=None, Tensor? attn_mask=None, bool with_kv=True) -> Tensor[]");
 }

@@ -63,9 +63,10 @@ def _ext_train():
     torch.library.register_fake("vlak::fused_attention_gqa_fwd_lse")(
         lambda q, k, v, scale=-1.0, prefix_len=-1, dead_start=0, dead_end=0, lengths=None,
         attn_mask=None:
-            (o_like(q), torch.empty(q.shape[:3], dtype=torch.float32, device=q.device)))
+            (o_like(q), torch.empty(q.shape[:3], dtype=torch.float32, device=q.device),
+             torch.empty(q.shape, dtype=torch.int8, device=q.device)))
     torch.library.register_fake("vlak::fused_attention_gqa_bwd")(
-        lambda grad_o, q, k, v, o, lse, scale=-1.0, prefix_len=-1, dead_start=0, dead_end=0,
+        lambda grad_o, q, k, v, o, lse, o_low, scale=-1.0, prefix_len=-1, dead_start=0, dead_end=0,
         lengths=None, attn_mask=None, with_kv=True:
             [o_like(t) for t in ((q, k, v) if with_kv else (q,))])
     return torch.ops.vlak
@@ -180,8 +181,8 @@ def fused_attention_gqa_train(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     gradient goes to kv head h // (H // H_kv), summed over its query heads.
 
     The backward pass (vla-kernels_b200/csrc/attention_bwd.cu) recomputes the
-    probabilities; between the passes only q, k, v, the output and one float
-    per row are kept. Sums are 32-bit in a fixed order, so gradients repeat bit
+    probabilities; between the passes only q, k, v, the output (with eight
+    more bits of each entry) and one float per row are kept. Sums are 32-bit in a fixed order, so gradients repeat bit
     for bit. A row that sees no key is zeros and has a zero gradient. Values
     that no row may see (a dead band, positions past a sample's length) may be
     anything, NaN included; behind ``attn_mask`` all values must be finite.
