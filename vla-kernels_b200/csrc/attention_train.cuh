@@ -243,22 +243,27 @@ struct Turn {
 // O beyond its bf16 rounding. D = rowsum(dO * O) is a sum in which the bf16
 // rounding of O would weigh as much as that of dS where a row's weight lies on
 // few keys, so the forward pass keeps the next eight bits of each entry of O: the
-// distance of the 32-bit value from its bf16 one, as integers, in units of 2^8.
+// distance of the 32-bit value from its bf16 one, as integers, -2^15 to 2^15,
+// without its low byte (whose middle is taken in its place).
 __device__ __forceinline__ uint32_t low_bytes(const float* x, const uint32_t* hi) {  // of four entries
-  uint32_t w = 0u;
+  int d[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int top = static_cast<int>(i & 1 ? hi[i >> 1] & 0xffff0000u : hi[i >> 1] << 16);
-    const int d = (__float_as_int(x[i]) - top + 128) >> 8;
-    w |= (static_cast<uint32_t>(max(-128, min(127, d))) & 0xffu) << (8 * i);
+    d[i] = min(__float_as_int(x[i]) - top, 0x7fff);  // (a tie may be 2^15)
   }
-  return w;
+  // the second byte of each
+  return __byte_perm(__byte_perm(d[0], d[1], 0x0051), __byte_perm(d[2], d[3], 0x0051), 0x5410);
 }
 // the four entries again, from their bf16 values and the word of low_bytes
 __device__ __forceinline__ void with_low_bytes(float* x, uint32_t w) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    x[i] = __int_as_float(__float_as_int(x[i]) + (static_cast<int>(w << (24 - 8 * i)) >> 24 << 8));
+  for (int i = 0; i < 4; ++i) {
+    // byte i, its sign above it, zero below
+    int d;
+    asm("prmt.b32 %0, %1, 0, %2;" : "=r"(d) : "r"(w), "r"(0x0004 | i << 4 | (8 + i) << 8 | (8 + i) << 12));
+    x[i] = __int_as_float(__float_as_int(x[i]) + d + 128);
+  }
 }
 
 // ---------------------------------------------------------------------------

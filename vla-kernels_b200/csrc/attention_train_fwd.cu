@@ -55,8 +55,9 @@ constexpr int kWarpProducer = kComputeWarps, kWarpScores = kComputeWarps + 1,
               kWarpAccum = kComputeWarps + 2;  // (kComputeWarps + 3 has no role)
 constexpr int kWarpOutput = kComputeWarps + 4, kOutputWarps = 4;
 constexpr int kThreads = 32 * (kWarpOutput + kOutputWarps);
-constexpr int kRegsLaunch = 80, kRegsCompute = 88, kRegsOther = 64;
-static_assert(32 * kComputeWarps * kRegsCompute + (kThreads - 32 * kComputeWarps) * kRegsOther <=
+// Registers by warpgroup: compute, issue, output.
+constexpr int kRegsLaunch = 80, kRegsCompute = 88, kRegsIssue = 48, kRegsOutput = 80;
+static_assert(32 * kComputeWarps * kRegsCompute + 128 * kRegsIssue + 32 * kOutputWarps * kRegsOutput <=
                   kThreads * kRegsLaunch,
               "the split must fit the launch's registers");
 
@@ -116,7 +117,7 @@ __device__ __forceinline__ Item decode_item(const FwdParams& p, int id) {
 }
 
 __device__ __forceinline__ void less_registers() {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsIssue));
 }
 
 template <int kMode>
@@ -447,7 +448,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_train_fwd(const __grid_const
       ++live;
     }
   } else if (warp >= kWarpOutput) {
-    less_registers();
+    // (kRegsOutput is the launch's count: nothing to set)
+    static_assert(kRegsOutput == kRegsLaunch, "output warps keep the launch's registers");
     // Outputs: the streams joined, staged over the item's Q tile in the swizzled
     // layout of the map, then TMA stores; or a part's sums. One lane quarter of
     // TMEM per warp.
@@ -509,12 +511,15 @@ __global__ void __launch_bounds__(kThreads, 1) attn_train_fwd(const __grid_const
       tc_fence_after();
       uint8_t* a0 = a_smem + ab.i * kTileBytes;
       float* sums = p.parts > 1 ? p.sums + part_row * 64 : nullptr;
-      uint4 low = make_uint4(0u, 0u, 0u, 0u);
-#pragma unroll 1
-      for (int q = 0; q < 4; ++q) {  // 16 columns at a time
-        float o[16];
+      // Join and round all 64 columns first, so that the next item may soon
+      // accumulate; then stage them.
+      uint32_t hi[32], lo[16];
+      uint64_t w2[4];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) o[i] = 0.f;
+      for (int i = 0; i < 4; ++i) w2[i] = f2_pack(w[i], w[i]);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {  // 16 columns at a time
+        uint64_t o2[8] = {};
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
           if (!has[g]) continue;
@@ -523,12 +528,17 @@ __global__ void __launch_bounds__(kThreads, 1) attn_train_fwd(const __grid_const
           tmem_ld16(tbase + kAcc + 128 * g + 64 + 16 * q, x[1]);
           tmem_wait_ld();
 #pragma unroll
-          for (int i = 0; i < 16; ++i) o[i] += w[2 * g] * x[0][i] + w[2 * g + 1] * x[1][i];
+          for (int i = 0; i < 8; ++i)
+            o2[i] = f2_fma(f2_pack(x[1][2 * i], x[1][2 * i + 1]), w2[2 * g + 1],
+                           f2_fma(f2_pack(x[0][2 * i], x[0][2 * i + 1]), w2[2 * g], o2[i]));
         }
         if (q == 3) {  // read: the next item may accumulate
           tc_fence_before();
           mbar_arrive_elect(&bars->acc_empty);
         }
+        float o[16];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f2_unpack(o2[i], o[2 * i], o[2 * i + 1]);
         if (p.parts > 1) {
           if (r.valid) {
 #pragma unroll
@@ -537,29 +547,19 @@ __global__ void __launch_bounds__(kThreads, 1) attn_train_fwd(const __grid_const
                   make_float4(o[4 * v], o[4 * v + 1], o[4 * v + 2], o[4 * v + 3]);
           }
         } else {
-          uint8_t* stage = a0 + tl * kRowBytes;
-          uint32_t lo[4];
 #pragma unroll
-          for (int v = 0; v < 2; ++v) {
-            uint32_t pk[4];
+          for (int i = 0; i < 8; ++i)
+            hi[8 * q + i] = L == 0.f ? 0u : pack_bf16x2(o[2 * i], o[2 * i + 1]);
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              pk[e] = L == 0.f ? 0u : pack_bf16x2(o[v * 8 + 2 * e], o[v * 8 + 2 * e + 1]);
-            const uint32_t c = static_cast<uint32_t>(2 * q + v) ^ static_cast<uint32_t>(tl & 7);
-            st_shared_v4(stage + c * 16, pk[0], pk[1], pk[2], pk[3]);
-            lo[2 * v] = low_bytes(o + 8 * v, pk);
-            lo[2 * v + 1] = low_bytes(o + 8 * v + 4, pk + 2);
-          }
-          if (p.o_low != nullptr && r.valid) {  // whole 32-byte sectors
-            const uint4 now = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-            if (q & 1) {
-              uint4* dst = reinterpret_cast<uint4*>(p.o_low + row * 64 + 16 * (q - 1));
-              dst[0] = low;
-              dst[1] = now;
-            }
-            low = now;
-          }
+          for (int i = 0; i < 4; ++i) lo[4 * q + i] = low_bytes(o + 4 * i, hi + 8 * q + 2 * i);
         }
+      }
+      if (p.parts == 1) {
+        uint8_t* stage = a0 + tl * kRowBytes;
+#pragma unroll
+        for (int v = 0; v < 8; ++v)
+          st_shared_v4(stage + (static_cast<uint32_t>(v) ^ static_cast<uint32_t>(tl & 7)) * 16, hi[4 * v],
+                       hi[4 * v + 1], hi[4 * v + 2], hi[4 * v + 3]);
       }
       fence_proxy_async_smem();
       __syncwarp();
@@ -578,6 +578,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_train_fwd(const __grid_const
           mbar_arrive(&bars->a_empty[ab.i]);
         }
         __syncwarp();
+      }
+      if (p.parts == 1 && p.o_low != nullptr && r.valid) {
+        uint4* dst = reinterpret_cast<uint4*>(p.o_low + row * 64);
+#pragma unroll
+        for (int v = 0; v < 4; ++v) dst[v] = make_uint4(lo[4 * v], lo[4 * v + 1], lo[4 * v + 2], lo[4 * v + 3]);
       }
       ab.next();
       t += it.live;
