@@ -263,8 +263,8 @@ VLAK_API int vlak_attn_fwd(const void* q, const void* k, const void* v, void* o,
  *
  * Workspaces: device, 256-byte aligned, owned by the caller and unused by
  * anything else until the work on `stream` has finished; sized by the two
- * functions below (the forward one is 0 bytes, and may be NULL, unless few
- * heads have many keys).
+ * functions below (the forward one is 0 bytes, and may be NULL, unless there is
+ * a mask or few heads have many keys).
  * ---------------------------------------------------------------------- */
 typedef struct {
   vlak_attn_gqa_args attn;

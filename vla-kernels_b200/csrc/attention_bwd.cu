@@ -495,7 +495,6 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd(const __grid_constant__ 
       // dkv: rows m in [from, to) see the key; dq: keys [0, from) and [mid, to)
       // are seen by the row
       int from = 0, mid = 0, to = 0;
-      const uint8_t* mrow = nullptr;
       if (it.dkv) {
         to = p.M;
         if (kMode == kMaskAnalytic) {
@@ -507,7 +506,6 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd(const __grid_constant__ 
           to = key < it.L ? it.L : 0;
         }
         if (!valid) to = 0;
-        if (kMode == kMaskBool && valid) mrow = p.mask + it.b * p.mask_sb + key;
       } else {
         if (kMode == kMaskAnalytic) {
           from = p.ds;
@@ -516,7 +514,6 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd(const __grid_constant__ 
         } else if (kMode == kMaskLength) {
           to = r.m < it.L ? it.L : 0;
         }
-        if (kMode == kMaskBool && valid) mrow = p.mask + it.b * p.mask_sb + r.m * p.mask_sm;
       }
       // A step's 32 columns of this warp, by their first key c (dq) or the
       // sub-tile's first position c (dkv), are seen by all its lanes when
@@ -571,13 +568,22 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd(const __grid_constant__ 
         bool full, none;
         if (kMode == kMaskBool) {
           if (it.dkv && valid) {
-            const uint64_t heads = ~0ull >> (64 - p.Gb);
-            const int rows = min(p.MT, p.M - c);
-            for (int i = 0; i < rows; ++i)
-              if (__ldg(mrow + static_cast<long long>(c + i) * p.mask_sm) != 0)
-                vm |= static_cast<uint32_t>((heads << (i * p.Gb)) >> (32 * gq));
+            // the positions of the warp's columns, each spread over Gb of them
+            // (the first may have begun in the columns before)
+            const int first = 32 * gq / p.Gb, begun = 32 * gq - first * p.Gb;
+            if (first < p.MT && c + first < p.M) {
+              const uint32_t seen = col_bits_at(p, it.b, key, c + first);
+              if (p.Gb == 1) {
+                vm = seen;
+              } else {
+                const uint64_t heads = ~0ull >> (64 - p.Gb);
+                const int last = min(p.MT - first, (32 + begun + p.Gb - 1) / p.Gb);
+                for (int i = 0; i < last; ++i)
+                  if ((seen >> i) & 1u) vm |= static_cast<uint32_t>((heads << (i * p.Gb)) >> begun);
+              }
+            }
           } else if (!it.dkv && valid && c < p.N) {
-            vm = mask_bits32(mrow, c, p.N, p.mask_words);
+            vm = row_bits_at(p, it.b, r.m, c);
           }
           full = __all_sync(kFullMask, !valid || vm == 0xffffffffu);
           none = __all_sync(kFullMask, !valid || vm == 0u);
@@ -838,15 +844,15 @@ __global__ void __launch_bounds__(256) attn_bwd_join_q(const __grid_constant__ B
 // ---------------------------------------------------------------------------
 // host
 
-// Parts and workspace of a call: the sub-tiles' statistics, the item counter,
-// then the parts' sums.
+// Parts and workspace of a call: the sub-tiles' statistics, the item counter, the
+// parts' sums, and the packed mask.
 struct BwdPlan {
   SubTiling tl;
   int64_t n_bk, n_kblk, n_pair;
   int kv_parts, q_parts;
-  int64_t counter, kv_sums, q_sums, bytes;  // offsets and size
+  int64_t counter, kv_sums, q_sums, row_bits, col_bits, bytes;  // offsets and size
 };
-BwdPlan plan_bwd(const vlak_attn_gqa_args* a, bool keys_too) {
+BwdPlan plan_bwd(const vlak_attn_gqa_args* a, bool keys_too, bool masked) {
   BwdPlan w{};
   w.tl = sub_tiling(static_cast<int>(a->H / a->Hkv), static_cast<int>(a->M));
   w.n_bk = a->B * a->Hkv;
@@ -859,7 +865,9 @@ BwdPlan plan_bwd(const vlak_attn_gqa_args* a, bool keys_too) {
   w.counter = w.n_bk * w.tl.n_sub * kStatBytes;
   w.kv_sums = w.counter + 256;
   w.q_sums = w.kv_sums + (w.kv_parts > 1 ? w.kv_parts * w.n_bk * w.n_kblk * kKeys * 128 * 4 : 0);
-  w.bytes = w.q_sums + (w.q_parts > 1 ? w.q_parts * w.n_bk * w.tl.n_sub * kSub * 64 * 4 : 0);
+  w.row_bits = w.q_sums + (w.q_parts > 1 ? w.q_parts * w.n_bk * w.tl.n_sub * kSub * 64 * 4 : 0);
+  w.col_bits = w.row_bits + (masked ? row_bits_bytes(*a) : 0);
+  w.bytes = w.col_bits + (masked && keys_too ? col_bits_bytes(*a) : 0);
   return w;
 }
 
@@ -944,7 +952,7 @@ int run_bwd(const vlak_attn_train_args* t, void* workspace, int64_t ws_bytes, vo
   }
   if (!a->q || !a->k || !a->v || !a->o || !args.grad_o || !args.lse)
     return set_error(VLAK_ERR_INVALID_ARGUMENT, "fused_attention_gqa_bwd: null tensor pointer");
-  const BwdPlan plan = plan_bwd(a, keys_too);
+  const BwdPlan plan = plan_bwd(a, keys_too, args.mask != nullptr);
   if (!workspace || ws_bytes < plan.bytes)
     return set_error(VLAK_ERR_INVALID_ARGUMENT, "fused_attention_gqa_bwd: workspace missing or too small");
   if (reinterpret_cast<uintptr_t>(workspace) % 256 != 0)
@@ -984,6 +992,8 @@ int run_bwd(const vlak_attn_train_args* t, void* workspace, int64_t ws_bytes, vo
   p.counter = reinterpret_cast<unsigned*>(ws + plan.counter);
   p.kv_sums = reinterpret_cast<float*>(ws + plan.kv_sums);
   p.q_sums = reinterpret_cast<float*>(ws + plan.q_sums);
+  p.row_bits = reinterpret_cast<uint32_t*>(ws + plan.row_bits);
+  p.col_bits = keys_too ? reinterpret_cast<uint32_t*>(ws + plan.col_bits) : nullptr;
   p.o = static_cast<const __nv_bfloat16*>(a->o);
   p.d_o = static_cast<const __nv_bfloat16*>(args.grad_o);
   p.o_low = static_cast<const int8_t*>(args.o_low);
@@ -1016,9 +1026,11 @@ int run_bwd(const vlak_attn_train_args* t, void* workspace, int64_t ws_bytes, vo
 
   const unsigned n_stats = static_cast<unsigned>(n_bk * p.n_sub);
   const unsigned grid = static_cast<unsigned>(std::min(p.n_items, dev.sm_count));
-  cudaError_t e = args.lengths ? launch_both<kMaskLength>(p, n_stats, grid, cs, dev.device)
-                  : args.mask  ? launch_both<kMaskBool>(p, n_stats, grid, cs, dev.device)
-                               : launch_both<kMaskAnalytic>(p, n_stats, grid, cs, dev.device);
+  cudaError_t e = args.mask ? launch_pack(args, p, cs) : cudaSuccess;
+  if (e != cudaSuccess) return set_cuda_error("fused_attention_gqa_bwd mask", e);
+  e = args.lengths ? launch_both<kMaskLength>(p, n_stats, grid, cs, dev.device)
+      : args.mask  ? launch_both<kMaskBool>(p, n_stats, grid, cs, dev.device)
+                   : launch_both<kMaskAnalytic>(p, n_stats, grid, cs, dev.device);
   if (e != cudaSuccess) return set_cuda_error("fused_attention_gqa_bwd launch failed", e);
   return VLAK_OK;
 }
@@ -1049,7 +1061,8 @@ extern "C" int vlak_attn_gqa_bwd_workspace_size(const vlak_attn_train_args* args
   }
   int st = vlak_attn_gqa_check(&a, nullptr, nullptr);
   if (st != VLAK_OK) return st;
-  if (a.B > 0 && a.M > 0 && a.N > 0) *bytes = plan_bwd(&a, args->dk || args->dv).bytes;
+  if (a.B > 0 && a.M > 0 && a.N > 0) 
+    *bytes = plan_bwd(&a, args->dk || args->dv, args->mask != nullptr).bytes;
   return VLAK_OK;
 }
 

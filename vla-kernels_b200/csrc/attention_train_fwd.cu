@@ -337,15 +337,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_train_fwd(const __grid_const
       const SubRow r = sub_row(p, it.s0 + (quarter >> 1), (quarter & 1) * 32 + lane);
       // keys [0, from) and [mid, to) are seen by the row
       int from = 0, mid = 0, to = 0;
-      const uint8_t* mrow = nullptr;
       if (kMode == kMaskAnalytic) {
         from = p.ds;
         mid = p.de;
         to = max(p.P, min(p.N, p.N - p.M + r.m + 1));
       } else if (kMode == kMaskLength) {
         to = r.m < it.L ? it.L : 0;
-      } else if (r.valid) {
-        mrow = p.mask + it.b * p.mask_sb + r.m * p.mask_sm;
       }
       constexpr int kFar = INT32_MAX / 2;
       const int to_lo = __reduce_min_sync(kFullMask, r.valid ? to : kFar);
@@ -361,7 +358,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_train_fwd(const __grid_const
         uint32_t vm = 0u;
         bool full, none;
         if (kMode == kMaskBool) {
-          if (r.valid && c < p.N) vm = mask_bits32(mrow, c, p.N, p.mask_words);
+          if (r.valid && c < p.N) vm = row_bits_at(p, it.b, r.m, c);
           full = __all_sync(kFullMask, !r.valid || vm == 0xffffffffu);
           none = __all_sync(kFullMask, !r.valid || vm == 0u);
         } else {
@@ -657,14 +654,15 @@ __global__ void no_keys(__nv_bfloat16* o, long long o_sb, long long o_sm, long l
 // ---------------------------------------------------------------------------
 // host
 
-// Parts and workspace of a call: the parts' sums, then their maxima and sums.
+// Parts and workspace of a call: the parts' sums, their maxima and sums, and the
+// packed mask.
 struct FwdPlan {
   SubTiling tl;
   int64_t n_bk, n_pair;
   int parts;
-  int64_t ml, bytes;
+  int64_t ml, bits, bytes;
 };
-FwdPlan plan_fwd(const vlak_attn_gqa_args* a) {
+FwdPlan plan_fwd(const vlak_attn_gqa_args* a, bool masked) {
   FwdPlan w{};
   w.tl = sub_tiling(static_cast<int>(a->H / a->Hkv), static_cast<int>(a->M));
   w.n_bk = a->B * a->Hkv;
@@ -674,8 +672,9 @@ FwdPlan plan_fwd(const vlak_attn_gqa_args* a) {
   if (w.parts > 1) {
     const int64_t rows = w.parts * w.n_bk * w.tl.n_sub * kSub;
     w.ml = rows * 64 * 4;
-    w.bytes = w.ml + rows * 8;
+    w.bits = w.ml + rows * 8;
   }
+  w.bytes = w.bits + (masked ? row_bits_bytes(*a) : 0);
   return w;
 }
 
@@ -720,8 +719,8 @@ int run_fwd(const vlak_attn_train_args* t, void* workspace, int64_t ws_bytes, vo
   if (!a->o || !args.lse || (a->N > 0 && (!a->q || !a->k || !a->v)))
     return set_errorf(VLAK_ERR_INVALID_ARGUMENT, "%s: null tensor pointer", op);
   cudaStream_t cs = static_cast<cudaStream_t>(stream);
-  const FwdPlan plan = plan_fwd(a);
-  if (plan.parts > 1 && (!workspace || ws_bytes < plan.bytes))
+  const FwdPlan plan = plan_fwd(a, args.mask != nullptr);
+  if (a->N > 0 && plan.bytes > 0 && (!workspace || ws_bytes < plan.bytes))
     return set_errorf(VLAK_ERR_INVALID_ARGUMENT, "%s: workspace missing or too small", op);
   if (reinterpret_cast<uintptr_t>(workspace) % 256 != 0)
     return set_errorf(VLAK_ERR_ALIGNMENT, "%s: workspace must be 256-byte aligned", op);
@@ -756,6 +755,7 @@ int run_fwd(const vlak_attn_train_args* t, void* workspace, int64_t ws_bytes, vo
   p.parts = plan.parts;
   p.sums = static_cast<float*>(workspace);
   p.ml = reinterpret_cast<float2*>(static_cast<uint8_t*>(workspace) + plan.ml);
+  p.row_bits = reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(workspace) + plan.bits);
   p.n_items = static_cast<int>(n_items);
   p.by_parts = fast_div_by(static_cast<unsigned>(p.parts));
   const uint32_t gb = static_cast<uint32_t>(plan.tl.Gb), mt = static_cast<uint32_t>(plan.tl.MT);
@@ -770,9 +770,11 @@ int run_fwd(const vlak_attn_train_args* t, void* workspace, int64_t ws_bytes, vo
                     kChunk, "v");
   if (st != VLAK_OK) return st;
   const unsigned grid = static_cast<unsigned>(std::min(p.n_items, dev.sm_count));
-  const cudaError_t e = args.lengths ? launch_fwd<kMaskLength>(p, grid, cs, dev.device)
-                        : args.mask  ? launch_fwd<kMaskBool>(p, grid, cs, dev.device)
-                                     : launch_fwd<kMaskAnalytic>(p, grid, cs, dev.device);
+  cudaError_t e = args.mask ? launch_pack(args, p, cs) : cudaSuccess;
+  if (e == cudaSuccess)
+    e = args.lengths ? launch_fwd<kMaskLength>(p, grid, cs, dev.device)
+        : args.mask  ? launch_fwd<kMaskBool>(p, grid, cs, dev.device)
+                     : launch_fwd<kMaskAnalytic>(p, grid, cs, dev.device);
   return e == cudaSuccess ? VLAK_OK : set_cuda_error("fused_attention_gqa_train launch failed", e);
 }
 
@@ -806,6 +808,6 @@ extern "C" int vlak_attn_gqa_train_workspace_size(const vlak_attn_train_args* ar
   }
   const int st = vlak_attn_gqa_check(&a, nullptr, nullptr);
   if (st != VLAK_OK) return st;
-  if (a.B > 0 && a.M > 0 && a.N > 0) *bytes = plan_fwd(&a).bytes;
+  if (a.B > 0 && a.M > 0 && a.N > 0) *bytes = plan_fwd(&a, args->mask != nullptr).bytes;
   return VLAK_OK;
 }
