@@ -114,6 +114,12 @@ def test_large_scores_and_scale():
     run(1, 70, 150, 4, 2, 40, 0, 0, scale=1e-3)
 
 
+def test_scale_below_the_smallest_float():
+    # zero in 32 bits, which must not meet the -inf of masked scores
+    run(1, 70, 150, 4, 2, 40, 0, 0, scale=1e-60)
+    run(2, 60, 60, 2, 1, 0, 0, 0, scale=1e-300)
+
+
 @pytest.mark.parametrize("N", [2, 3, 5, 9])
 def test_few_keys_keep_their_precision(N):
     # where a row's weight lies on few keys, D = rowsum(do * o) is as large as dP:

@@ -8,8 +8,8 @@
 // the exp2 domain: P = 2^(scale log2(e) s - lse), lse from the forward pass.
 //
 // A first small kernel (attn_bwd_stats) computes D and lays (-lse, -D) out by
-// sub-tiles. The second, persistent, one works through two kinds of items, in
-// no shared sums, so without atomics on results, which repeat bit for bit:
+// sub-tiles. The second, persistent, one works through two kinds of items that
+// share no sums, so without atomics on results, which repeat bit for bit:
 //   dkv  128 keys of a kv head, stationary K and V; walks the query rows of all
 //        G heads: S^T = K Q^T, dP^T = V dO^T, then dV += P^T dO, dK += dS^T Q
 //        with P^T and dS^T as TMEM operands (keys along the lanes, so nothing is
@@ -25,18 +25,20 @@
 // Pipeline. One CTA per SM with all 512 columns of TMEM: two accumulators and
 // three stages of (T0, T1), so the products of the next steps, also those of the
 // next item, are issued while the current one's elementwise part runs. Sixteen
-// compute warps in two groups take the steps in turn. Items come from a counter,
-// the long ones first.
+// compute warps in two groups take the steps in turn, one warp issues the score
+// products and another the accumulating ones, four carry the outputs away. Items
+// come from a counter, the long ones first; long items of few heads are cut into
+// parts, whose fp32 sums another kernel joins in their order.
 //
 // Bound: by the products' shared-memory reads and issue. A step (128 x 64) is
 // 8 SS products of about 49 cycles and 4 (dq) or 8 (dkv) TS products of about 43.
 //
-// Rounding: P and dS are rounded to bf16 as operands of the second products,
-// as the forward pass rounds P; all sums, D and the statistics are fp32.
+// Rounding: P and dS are rounded to bf16 as operands of the second products, as
+// the forward pass rounds P, or to twice that in fine calls (see kFineShare);
+// all sums, D and the statistics are fp32.
 //
-// Query rows are handled in sub-tiles of up to 64 rows, Gb heads x MT
-// positions with Gb a divisor of G, one TMA box each. Two sub-tiles make the
-// 128 rows of a dq item; one is the 64 columns of a dkv step.
+// Rows are cut into sub-tiles as attention_train.cuh says: two are the 128 rows
+// of a dq item, one is the 64 columns of a dkv step.
 //
 // Every mbarrier wait is bounded as in the forward kernel.
 
@@ -60,7 +62,7 @@ namespace vlak {
 namespace {
 
 constexpr int kKeys = 128;                   // keys of a dkv item
-constexpr int kRing = 6;                     // streamed pairs in flight (even: see the compute warps)
+constexpr int kRing = 6;                     // streamed pairs in flight (even: see the compute warps' waits)
 constexpr int kTiles = 3;                    // items whose stationary tiles are in shared memory
 constexpr int kStages = 3;                   // (T0, T1) pairs in TMEM
 constexpr int kQueue = 8;                    // items handed out and not yet seen by every warp
@@ -113,9 +115,9 @@ struct __align__(64) BwdParams : TrainShape {
 
 // ---------------------------------------------------------------------------
 // D = rowsum(dO * O), O with its low bytes, and -lse by sub-tile rows: four
-// threads per row, two 16-byte vectors of each tensor per thread. Rows that do not exist or see no key get
-// -lse = -inf (every P is 0) and D = 0, whatever memory holds there. Bound: HBM,
-// one read of O and dO.
+// threads per row, two 16-byte vectors of each tensor per thread. Rows that do not
+// exist or see no key get -lse = -inf (every P is 0) and D = 0, whatever memory
+// holds there. Bound: HBM, one read of O and dO.
 constexpr int kStatThreads = 4 * kSub;
 __global__ void __launch_bounds__(kStatThreads) attn_bwd_stats(const __grid_constant__ BwdParams p) {
   // the main kernel may set itself up meanwhile; it waits for this grid's end
@@ -224,7 +226,7 @@ __device__ __forceinline__ void less_registers() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
 }
 
-template <int kMode>
+template <int kMode, bool kFine>
 __global__ void __launch_bounds__(kThreads, 1) attn_bwd(const __grid_constant__ BwdParams p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = aligned_smem(smem_raw);
@@ -462,6 +464,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd(const __grid_constant__ 
         const uint32_t x = tmem + kStage0 + st.i * kStageCols;
         umma_ts_x4(tmem + kAcc0, x, b0 + kSubBytes / 16, id_kn, j > 0, it.dkv);  // dV += P^T dO
         umma_ts_x4(tmem + kAcc1, x + kT1, b0, id_kn, j > 0, 1u);  // dK += dS^T Q, dQ += dS K
+        if (kFine) {  // the rests of P and dS
+          umma_ts_x4(tmem + kAcc0, x + 8, b0 + kSubBytes / 16, id_kn, 1u, it.dkv);
+          umma_ts_x4(tmem + kAcc1, x + kT1 + 8, b0, id_kn, 1u, 1u);
+        }
         umma_commit_elect(&bars->t_empty[st.i]);
         umma_commit_elect(&bars->b_empty[s.i]);
         s.next();
@@ -611,9 +617,16 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd(const __grid_constant__ 
         tc_fence_after();
         const uint32_t t0 = tbase + kStage0 + st * kStageCols + 32 * gq;
         if (none) {
-          const uint32_t zero[16] = {};
-          if (it.dkv) tmem_st16(t0, zero);
-          tmem_st16(t0 + kT1, zero);
+          const uint32_t zero[8] = {};
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            if (it.dkv) tmem_st8(t0 + 16 * h, zero);
+            tmem_st8(t0 + kT1 + 16 * h, zero);
+            if (kFine) {
+              if (it.dkv) tmem_st8(t0 + 16 * h + 8, zero);
+              tmem_st8(t0 + kT1 + 16 * h + 8, zero);
+            }
+          }
         } else {
           const float4* stat = reinterpret_cast<const float4*>(b_stat + s * kStatFloats) + 8 * gq;
           // Sixteen columns at a time, which keeps the step in registers. Four
@@ -625,7 +638,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd(const __grid_constant__ 
               tmem_ld16(t0 + 16 * h, sv);
               tmem_ld16(t0 + kT1 + 16 * h, dp);
               tmem_wait_ld();
-              uint32_t pp[8], pd[8];
+              uint32_t pp[8], pd[8], rp[4], rd[4];
 #pragma unroll
               for (int i = 0; i < 4; ++i) {  // four columns
                 uint64_t l2[2] = {nl2, nl2}, d2[2] = {nD2, nD2};
@@ -653,12 +666,24 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd(const __grid_constant__ 
                   }
                   if (decltype(dkv)::value) pp[k] = pack_bf16x2(e0, e1);
                   pd[k] = pack_bf16x2(d0, d1);
+                  if (kFine) {
+                    if (decltype(dkv)::value) rp[k % 4] = rest_of_pair(e0, e1, pp[k]);
+                    rd[k % 4] = rest_of_pair(d0, d1, pd[k]);
+                  }
+                }
+                if (kFine && i % 2 == 1) {
+                  // over the columns just read, the rests behind
+                  const uint32_t at = t0 + 16 * h + 4 * (i / 2);
+                  if (decltype(dkv)::value) tmem_st4(at, pp + 2 * i - 2);
+                  if (decltype(dkv)::value) tmem_st4(at + 8, rp);
+                  tmem_st4(at + kT1, pd + 2 * i - 2);
+                  tmem_st4(at + kT1 + 8, rd);
                 }
               }
-              // over the first half of the columns the warp has read: 8 of the
-              // 16 just loaded, then the next 8
-              if (decltype(dkv)::value) tmem_st8(t0 + 8 * h, pp);
-              tmem_st8(t0 + kT1 + 8 * h, pd);
+              if (!kFine) {
+                if (decltype(dkv)::value) tmem_st8(t0 + 16 * h, pp);
+                tmem_st8(t0 + kT1 + 16 * h, pd);
+              }
             }
           };
           using Yes = std::true_type;
@@ -850,6 +875,7 @@ struct BwdPlan {
   SubTiling tl;
   int64_t n_bk, n_kblk, n_pair;
   int kv_parts, q_parts;
+  bool fine;
   int64_t counter, kv_sums, q_sums, row_bits, col_bits, bytes;  // offsets and size
 };
 BwdPlan plan_bwd(const vlak_attn_gqa_args* a, bool keys_too, bool masked) {
@@ -862,6 +888,7 @@ BwdPlan plan_bwd(const vlak_attn_gqa_args* a, bool keys_too, bool masked) {
   const int64_t total = w.n_bk * (w.n_pair * n_chunks + (keys_too ? w.n_kblk * w.tl.n_sub : 0));
   w.kv_parts = keys_too ? item_parts(w.tl.n_sub, total) : 1;
   w.q_parts = item_parts(n_chunks, total);
+  w.fine = fine_call(*a, total);
   w.counter = w.n_bk * w.tl.n_sub * kStatBytes;
   w.kv_sums = w.counter + 256;
   w.q_sums = w.kv_sums + (w.kv_parts > 1 ? w.kv_parts * w.n_bk * w.n_kblk * kKeys * 128 * 4 : 0);
@@ -871,11 +898,11 @@ BwdPlan plan_bwd(const vlak_attn_gqa_args* a, bool keys_too, bool masked) {
   return w;
 }
 
-template <int kMode>
+template <int kMode, bool kFine>
 cudaError_t launch_both(const BwdParams& p, unsigned n_stats, unsigned grid, cudaStream_t cs, int device) {
   static std::atomic<int> ready[64];
   if (ready[device].load() == 0) {
-    cudaError_t e = cudaFuncSetAttribute(attn_bwd<kMode>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    cudaError_t e = cudaFuncSetAttribute(attn_bwd<kMode, kFine>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          kSmem);
     if (e != cudaSuccess) return e;
     ready[device].store(1);
@@ -894,7 +921,7 @@ cudaError_t launch_both(const BwdParams& p, unsigned n_stats, unsigned grid, cud
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, attn_bwd<kMode>, p);
+  e = cudaLaunchKernelEx(&cfg, attn_bwd<kMode, kFine>, p);
   if (e == cudaSuccess && p.kv_parts > 1) {
     attn_bwd_join_kv<<<dim3((p.N + 7) / 8, p.n_bk), 256, 0, cs>>>(p);
     e = cudaGetLastError();
@@ -984,7 +1011,7 @@ int run_bwd(const vlak_attn_train_args* t, void* workspace, int64_t ws_bytes, vo
   p.by_kv_parts = fast_div_by(static_cast<unsigned>(p.kv_parts));
   p.by_q_parts = fast_div_by(static_cast<unsigned>(p.q_parts));
   // softmax over a single key is constant: its score's gradient is exactly zero
-  p.out_scale = p.N == 1 ? 0.f : scale;
+  p.out_scale = p.N == 1 ? 0.f : p.scale;
   p.host_err = host_error_word(cs);
   p.lse = args.lse;
   p.stats = static_cast<float*>(workspace);
@@ -1028,9 +1055,13 @@ int run_bwd(const vlak_attn_train_args* t, void* workspace, int64_t ws_bytes, vo
   const unsigned grid = static_cast<unsigned>(std::min(p.n_items, dev.sm_count));
   cudaError_t e = args.mask ? launch_pack(args, p, cs) : cudaSuccess;
   if (e != cudaSuccess) return set_cuda_error("fused_attention_gqa_bwd mask", e);
-  e = args.lengths ? launch_both<kMaskLength>(p, n_stats, grid, cs, dev.device)
-      : args.mask  ? launch_both<kMaskBool>(p, n_stats, grid, cs, dev.device)
-                   : launch_both<kMaskAnalytic>(p, n_stats, grid, cs, dev.device);
+  auto launch = [&](auto fine) {
+    constexpr bool kFine = decltype(fine)::value;
+    return args.lengths ? launch_both<kMaskLength, kFine>(p, n_stats, grid, cs, dev.device)
+           : args.mask  ? launch_both<kMaskBool, kFine>(p, n_stats, grid, cs, dev.device)
+                        : launch_both<kMaskAnalytic, kFine>(p, n_stats, grid, cs, dev.device);
+  };
+  e = plan.fine ? launch(std::true_type()) : launch(std::false_type());
   if (e != cudaSuccess) return set_cuda_error("fused_attention_gqa_bwd launch failed", e);
   return VLAK_OK;
 }
@@ -1061,7 +1092,7 @@ extern "C" int vlak_attn_gqa_bwd_workspace_size(const vlak_attn_train_args* args
   }
   int st = vlak_attn_gqa_check(&a, nullptr, nullptr);
   if (st != VLAK_OK) return st;
-  if (a.B > 0 && a.M > 0 && a.N > 0) 
+  if (a.B > 0 && a.M > 0 && a.N > 0)
     *bytes = plan_bwd(&a, args->dk || args->dv, args->mask != nullptr).bytes;
   return VLAK_OK;
 }

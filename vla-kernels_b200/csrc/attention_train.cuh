@@ -62,9 +62,21 @@ __device__ __forceinline__ uint32_t low_bits(int n) {
   return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : ((1u << n) - 1u);
 }
 
-// A step's 64 bf16 operand columns: each half of them is packed over the first
-// half of the 32 fp32 columns it was computed from, which the warp that packs
-// them has read; so they lie at columns 0-15 and 32-47 (see umma_ts_x4).
+// P and dS as TMEM operands are bf16 pairs packed over the fp32 columns they were
+// computed from: half as many, so beside each lies room for what the rounding
+// left, again as bf16. In fine calls that is a second operand of the same product,
+// which brings P and dS to 16 bits. Without it their rounding is as large as the
+// result's own, so errors are sqrt(2) of the least possible, and on rows of few
+// keys, where D carries the rounding of P as well, up to 1.7 times. Twice the
+// accumulating products cost a long call a third more time; so calls are fine
+// whose time goes to launches or to starting and ending items: of at most
+// kFineShare steps per SM, or kFineSteps per row item.
+constexpr int kFineShare = 8, kFineSteps = 2;
+
+// What a rounded pair leaves, rounded in turn.
+__device__ __forceinline__ uint32_t rest_of_pair(float x0, float x1, uint32_t pair) {
+  return pack_bf16x2(x0 - __uint_as_float(pair << 16), x1 - __uint_as_float(pair & 0xffff0000u));
+}
 
 // 1024-byte aligned start of the dynamic shared memory
 __device__ __forceinline__ uint8_t* aligned_smem(uint8_t* raw) {
@@ -243,7 +255,7 @@ __device__ __forceinline__ void umma_ss_x4(uint32_t d, uint64_t a, uint64_t b, u
       "l"(a), "l"(b), "r"(idesc)
       : "memory");
 }
-// A in TMEM at columns x + 0, 8, 32, 40; `acc` 0 starts a new sum; `on` 0
+// A in TMEM at columns x + 0, 16, 32, 48; `acc` 0 starts a new sum; `on` 0
 // issues nothing.
 __device__ __forceinline__ void umma_ts_x4(uint32_t d, uint32_t x, uint64_t b, uint32_t idesc,
                                            uint32_t acc, uint32_t on) {
@@ -252,7 +264,7 @@ __device__ __forceinline__ void umma_ts_x4(uint32_t d, uint32_t x, uint64_t b, u
       "elect.sync _|e, 0xffffffff;\n\t"
       "setp.ne.and.b32 q, %5, 0, e;\n\t"
       "setp.ne.b32 p, %4, 0;\n\tsetp.eq.b32 y, 0, 0;\n\t"
-      "add.s32 x1, %1, 8;\n\tadd.s32 x2, %1, 32;\n\tadd.s32 x3, %1, 40;\n\t"
+      "add.s32 x1, %1, 16;\n\tadd.s32 x2, %1, 32;\n\tadd.s32 x3, %1, 48;\n\t"
       "add.s64 b1, %2, 128;\n\tadd.s64 b2, %2, 256;\n\tadd.s64 b3, %2, 384;\n\t"
       "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
       "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [x1], b1, %3, y;\n\t"
@@ -351,8 +363,9 @@ inline TrainShape train_shape(const vlak_attn_gqa_args* a, int64_t P, float scal
   s.P = static_cast<int>(P);
   s.ds = static_cast<int>(a->dead_start);
   s.de = static_cast<int>(a->dead_end);
-  s.scale = scale;
-  s.scale_log2 = scale * 1.4426950408889634f;
+  // (a positive scale that fp32 rounds to zero: scores of -inf must stay so)
+  s.scale = std::max(scale, 0x1p-126f);
+  s.scale_log2 = s.scale * 1.4426950408889634f;
   s.by_bk = fast_div_by(static_cast<unsigned>(s.n_bk));
   s.by_pair = fast_div_by(static_cast<unsigned>(s.n_pair));
   s.by_hkv = fast_div_by(static_cast<unsigned>(s.Hkv));
@@ -390,6 +403,12 @@ inline cudaError_t launch_pack(const vlak_attn_train_args& a, const TrainShape& 
   pack_mask<<<blocks, 32 * kPackWarps, 0, cs>>>(static_cast<const uint8_t*>(a.mask), a.mask_stride_b,
                                                 a.mask_stride_m, s.B, s.M, s.N, s.row_bits, s.col_bits);
   return cudaGetLastError();
+}
+// Whether a call of `total` steps is fine; P, dead keys: as given or resolved.
+inline bool fine_call(const vlak_attn_gqa_args& a, int64_t total) {
+  const int64_t n_chunks = (a.N + kChunk - 1) / kChunk;
+  const int64_t seen = (a.dead_start + kChunk - 1) / kChunk + n_chunks - a.dead_end / kChunk;
+  return total <= kFineShare * kPlanSms || std::min(n_chunks, seen) <= kFineSteps;
 }
 // Parts of an item of `steps` steps, in a call of `total` steps: none longer
 // than an SM's even share, but no shorter than eight steps (joining costs

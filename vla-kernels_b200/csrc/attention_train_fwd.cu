@@ -17,7 +17,8 @@
 //
 // Long items of few heads are cut into parts, each a call's worth of streams of
 // its own, whose O, m and L a second kernel joins, all in fp32 (the inference
-// kernel's parts are held in bf16). P is rounded to bf16 as the operand of P V.
+// kernel's parts are held in bf16). P is rounded to bf16 as the operand of P V, or
+// to twice that in fine calls (see kFineShare).
 //
 // Bound: by the products' shared-memory reads and issue, 4 SS products of about
 // 49 cycles and 4 TS products of about 43 per 128 x 64 step, then the
@@ -120,7 +121,7 @@ __device__ __forceinline__ void less_registers() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsIssue));
 }
 
-template <int kMode>
+template <int kMode, bool kFine>
 __global__ void __launch_bounds__(kThreads, 1) attn_train_fwd(const __grid_constant__ FwdParams p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = aligned_smem(smem_raw);
@@ -306,6 +307,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_train_fwd(const __grid_const
         const uint64_t v0 = v_desc + s.i * (2 * kSubBytes / 16);
         umma_ts_x2(d, x, v0, id_kn, j > 1);
         umma_ts_x2(d + 64, x + 32, v0 + 256, id_kn, j > 1);
+        if (kFine) {  // the rests of P
+          umma_ts_x2(d, x + 16, v0, id_kn, 1u);
+          umma_ts_x2(d + 64, x + 48, v0 + 256, id_kn, 1u);
+        }
         umma_commit_elect(&bars->pv_done[t & 1]);
         umma_commit_elect(&bars->t_empty[st.i]);
         umma_commit_elect(&bars->b_empty[s.i]);
@@ -376,6 +381,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_train_fwd(const __grid_const
         if (none) {
           const uint32_t zero[16] = {};
           tmem_st16(t0, zero);
+          if (kFine) tmem_st16(t0 + 16, zero);
         } else {
           float sv[32];
           tmem_ld32(t0, sv);
@@ -398,7 +404,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_train_fwd(const __grid_const
           const float nref = m_run == -INFINITY ? 0.f : -m_run;
           const uint64_t nr2 = f2_pack(nref, nref);
           uint64_t acc[2] = {0ull, 0ull};
-          uint32_t pk[16];
+          uint32_t pk[16], rest[4];
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             float x0, x1;
@@ -406,8 +412,15 @@ __global__ void __launch_bounds__(kThreads, 1) attn_train_fwd(const __grid_const
             const float e0 = ex2(x0), e1 = ex2(x1);
             acc[i & 1] = f2_add(acc[i & 1], f2_pack(e0, e1));
             pk[i] = pack_bf16x2(e0, e1);
+            if (kFine) {
+              rest[i % 4] = rest_of_pair(e0, e1, pk[i]);
+              if (i % 4 == 3) {
+                tmem_st4(t0 + i - 3, pk + i - 3);
+                tmem_st4(t0 + 16 + i - 3, rest);
+              }
+            }
           }
-          tmem_st16(t0, pk);
+          if (!kFine) tmem_st16(t0, pk);
           float a0, a1;
           f2_unpack(f2_add(acc[0], acc[1]), a0, a1);
           l_run = l_run * alpha + (a0 + a1);
@@ -660,6 +673,7 @@ struct FwdPlan {
   SubTiling tl;
   int64_t n_bk, n_pair;
   int parts;
+  bool fine;
   int64_t ml, bits, bytes;
 };
 FwdPlan plan_fwd(const vlak_attn_gqa_args* a, bool masked) {
@@ -668,7 +682,9 @@ FwdPlan plan_fwd(const vlak_attn_gqa_args* a, bool masked) {
   w.n_bk = a->B * a->Hkv;
   w.n_pair = (w.tl.n_sub + 1) / 2;
   const int64_t n_chunks = (a->N + kChunk - 1) / kChunk;
-  w.parts = item_parts(n_chunks, w.n_bk * w.n_pair * n_chunks);
+  const int64_t total = w.n_bk * w.n_pair * n_chunks;
+  w.parts = item_parts(n_chunks, total);
+  w.fine = fine_call(*a, total);
   if (w.parts > 1) {
     const int64_t rows = w.parts * w.n_bk * w.tl.n_sub * kSub;
     w.ml = rows * 64 * 4;
@@ -678,16 +694,16 @@ FwdPlan plan_fwd(const vlak_attn_gqa_args* a, bool masked) {
   return w;
 }
 
-template <int kMode>
+template <int kMode, bool kFine>
 cudaError_t launch_fwd(const FwdParams& p, unsigned grid, cudaStream_t cs, int device) {
   static std::atomic<int> ready[64];
   if (ready[device].load() == 0) {
-    const cudaError_t e = cudaFuncSetAttribute(attn_train_fwd<kMode>,
+    const cudaError_t e = cudaFuncSetAttribute(attn_train_fwd<kMode, kFine>,
                                                cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
     if (e != cudaSuccess) return e;
     ready[device].store(1);
   }
-  attn_train_fwd<kMode><<<grid, kThreads, kSmem, cs>>>(p);
+  attn_train_fwd<kMode, kFine><<<grid, kThreads, kSmem, cs>>>(p);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess || p.parts == 1) return e;
   attn_train_fwd_join<<<dim3(p.n_sub * 4, p.n_bk), 256, 0, cs>>>(p);
@@ -771,10 +787,13 @@ int run_fwd(const vlak_attn_train_args* t, void* workspace, int64_t ws_bytes, vo
   if (st != VLAK_OK) return st;
   const unsigned grid = static_cast<unsigned>(std::min(p.n_items, dev.sm_count));
   cudaError_t e = args.mask ? launch_pack(args, p, cs) : cudaSuccess;
-  if (e == cudaSuccess)
-    e = args.lengths ? launch_fwd<kMaskLength>(p, grid, cs, dev.device)
-        : args.mask  ? launch_fwd<kMaskBool>(p, grid, cs, dev.device)
-                     : launch_fwd<kMaskAnalytic>(p, grid, cs, dev.device);
+  auto launch = [&](auto fine) {
+    constexpr bool kFine = decltype(fine)::value;
+    return args.lengths ? launch_fwd<kMaskLength, kFine>(p, grid, cs, dev.device)
+           : args.mask  ? launch_fwd<kMaskBool, kFine>(p, grid, cs, dev.device)
+                        : launch_fwd<kMaskAnalytic, kFine>(p, grid, cs, dev.device);
+  };
+  if (e == cudaSuccess) e = plan.fine ? launch(std::true_type()) : launch(std::false_type());
   return e == cudaSuccess ? VLAK_OK : set_cuda_error("fused_attention_gqa_train launch failed", e);
 }
 

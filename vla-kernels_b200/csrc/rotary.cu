@@ -14,8 +14,8 @@
 // Angles. position * f_i reaches 10^5..10^9 radians in long contexts, where a
 // 32-bit product has lost the fraction of a turn. Whole turns do not matter, so
 // f_i / 2 pi is held as a 64-bit binary fraction of a turn and the product with
-// the position wraps modulo 2^64, exactly: what is left, at 32 bits the
-// fraction of a turn to 2^-32, goes to sincospi in 32 bits. All else is 32-bit
+// the position wraps modulo 2^64, exactly: of what is left the upper 32 bits,
+// the fraction of a turn to 2^-32, go to a 32-bit sine and cosine. All else is 32-bit
 // too: norms, dot products and the weight gradient's sums; outputs are rounded
 // once.
 //

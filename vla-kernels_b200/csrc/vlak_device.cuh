@@ -447,6 +447,11 @@ __device__ __forceinline__ uint64_t sdesc_sw128(uint32_t smem_addr) {
 // lane (row) of the warp's 32-lane quarter and moves consecutive 32-bit
 // columns. The operands bind to array elements directly so the arrays stay
 // in registers.
+__device__ __forceinline__ void tmem_st4(uint32_t taddr, const uint32_t* u) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};"
+               ::"r"(taddr), "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3])
+               : "memory");
+}
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&r)[16]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
