@@ -210,15 +210,18 @@ __global__ void __launch_bounds__(32 * kLaneWarps) rotary_lane(const RotParams p
 }
 
 // ---------------------------------------------------------------------------
-// 16-byte path: a thread holds a unit of two vectors of V entries, the two
-// halves of V pairs (half layout), or 2V neighbouring entries (interleaved, and
-// past rd). A head is D / 2V units on the next power of two of lanes, a slot,
-// so a norm is a few shuffles. A block takes TB tokens at a time with HS slots
+// 16-byte path: a thread holds a unit of two vectors of V entries, one from each
+// half of the rotated part, or of the part past rd, in both layouts: in the half
+// layout they are the halves of V pairs, in the interleaved one V / 2 pairs each.
+// So a head's lanes read neighbouring 16 bytes. A head is D / 2V units on the next
+// power of two of lanes, a slot, so a norm is a few shuffles. A block takes TB tokens at a time with HS slots
 // each; some of the HS serve queries and the others keys, in turn over their
 // heads, so a thread stays with one tensor and its weight-gradient sums stay in
 // registers. The block first computes the tokens' angles into shared memory,
 // once for all heads of queries and keys.
 constexpr int kVecThreads = 128;
+// Blocks per SM, by registers.
+constexpr int vec_blocks(int mode) { return mode == kRotate ? 6 : mode == kNormFwd ? 5 : 4; }
 
 // Arithmetic is on pairs of fp32 (f32x2), which halves its issue slots; the
 // forward norm folds its weights into the angles' factors once per token:
@@ -256,10 +259,28 @@ __device__ __forceinline__ void pack_unit(const uint64_t* f, uint4& v0, uint4& v
   v1 = Elem<T>::pack(t + V);
 }
 
+// Rows come through shared memory, kDepth - 1 ahead of the one being worked on: a
+// thread's own vectors, so without barriers. One row ahead in registers left the
+// kernels waiting for loads: 2 x 8192 tokens of 40 heads of 128 took 60.4 us
+// instead of 53.2, 8191 tokens with norm 36.2 instead of 31.0 forward, 60 instead
+// of 51 backward; the depth (2 to 4) hardly matters. These copies go past L1, so a
+// warp's have to cover whole sectors (see the units above; 76 us with
+// neighbouring vectors per thread).
+__device__ __forceinline__ void copy16_async(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int n>
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(n) : "memory");
+}
+
 template <typename T, int kMode, bool kInter>
-__global__ void __launch_bounds__(kVecThreads, kMode == kRotate ? 6 : kMode == kNormFwd ? 5 : 4)
+__global__ void __launch_bounds__(kVecThreads, vec_blocks(kMode))
     rotary_vec(const RotParams p) {
   constexpr int V = Elem<T>::kVec;
+  constexpr int kDepth = kMode == kNormBwd ? 3 : 4, kVecs = kMode == kNormBwd ? 4 : 2;
+  __shared__ uint4 ring[kDepth][kVecs][kVecThreads];
   // two tables in turn, so one barrier per step is enough: TB * half entries,
   // at most slots * (units * V). Tables lie as [chunk of 16 bytes][unit], so that
   // a warp's units read neighbouring 16 bytes.
@@ -274,12 +295,13 @@ __global__ void __launch_bounds__(kVecThreads, kMode == kRotate ? 6 : kMode == k
   const unsigned stride = gridDim.x * TB;
   const int units = p.D / (2 * V), turned_units = max(1, p.half / V);
   const bool there = u < units, rot = u < p.half / V;
-  // the unit's vectors start at entries e0 and e0 + apart (a spare lane reads
-  // unit 0's)
-  const int e0 = !there ? 0 : rot && !kInter ? u * V : 2 * u * V;
-  const int apart = rot && !kInter ? p.half : V;
+  // the unit's vectors start at entries e0 and e0 + apart
+  const int past = p.D / 2 - p.half;  // half of the entries past rd
+  const int e0 = !there ? 0 : rot ? u * V : p.half + u * V;
+  const int apart = rot || !there ? p.half : past;
   auto entry = [&](int i) {  // of the i-th a (i < V) or b
-    return kInter ? e0 + 2 * (i % V) + i / V : e0 + i % V + (i < V ? 0 : apart);
+    const int k = i % V;
+    return kInter ? e0 + (k < V / 2 ? 2 * k : apart + 2 * k - V) + i / V : e0 + k + (i < V ? 0 : apart);
   };
   const unsigned tokens = static_cast<unsigned>(p.tokens);
   const float inv_D = 1.f / p.D;
@@ -302,36 +324,65 @@ __global__ void __launch_bounds__(kVecThreads, kMode == kRotate ? 6 : kMode == k
     a = f2_pack(w.x, w.y);
     c = f2_pack(w.z, w.w);
   };
+  // the next row to fetch: of tile l_tok0 the head l_h, in the l_trip-th trip. A
+  // thread without one (no token, head or unit) works on what the ring holds; its
+  // results go nowhere.
+  unsigned l_tok0 = blockIdx.x * TB;
+  int l_trip = 0, l_h = h0;
+  bool l_here = false;
+  const T *l_x = nullptr, *l_g = nullptr;
+  auto locate = [&]() {
+    const unsigned tok = l_tok0 + tl;
+    l_here = there && tl < TB && tok < tokens;
+    if (l_here) {
+      const unsigned tb = fast_div(tok, p.by_M);
+      const long long b = tb, m = tok - tb * p.by_M.d;
+      l_x = static_cast<const T*>(t.x) + b * t.x_sb + m * t.x_sm + h0 * t.x_sh + e0;
+      if (kMode == kNormBwd) l_g = static_cast<const T*>(t.g) + b * t.g_sb + m * t.g_sm + h0 * t.g_sh + e0;
+    }
+  };
+  auto fetch = [&](int to) {
+    if (l_here && l_h < H) {
+      copy16_async(&ring[to][0][threadIdx.x], l_x);
+      copy16_async(&ring[to][1][threadIdx.x], l_x + apart);
+      if (kMode == kNormBwd) {
+        copy16_async(&ring[to][2][threadIdx.x], l_g);
+        copy16_async(&ring[to][3][threadIdx.x], l_g + apart);
+      }
+    }
+    copies_commit();
+    l_x += x_step;
+    if (kMode == kNormBwd) l_g += g_step;
+    l_h += h_step;
+    if (++l_trip == p.trips) {
+      l_trip = 0;
+      l_h = h0;
+      l_tok0 += stride;
+      locate();
+    }
+  };
+  locate();
+#pragma unroll
+  for (int i = 0; i < kDepth - 1; ++i) fetch(i);
+  int at_ring = 0;
   bool first = true;
   int buf = 0;
   for (unsigned tok0 = blockIdx.x * TB; tok0 < tokens; tok0 += stride, buf ^= 1) {
     const bool here = there && tl < TB && tok0 + tl < tokens;
-    // a thread without a token reads the block's first (its results go nowhere)
-    const unsigned tok = tl < TB && tok0 + tl < tokens ? tok0 + tl : tok0, tb = fast_div(tok, p.by_M);
-    const long long b = tb, m = tok - tb * p.by_M.d;
-    const T* x = static_cast<const T*>(t.x) + b * t.x_sb + m * t.x_sm + h0 * t.x_sh + e0;
-    const T* g = static_cast<const T*>(t.g) + b * t.g_sb + m * t.g_sm + h0 * t.g_sh + e0;
+    const unsigned tok = tl < TB && tok0 + tl < tokens ? tok0 + tl : tok0;
     T* y = static_cast<T*>(t.y) + (static_cast<long long>(tok) * H + h0) * p.D + e0;
-    uint4 raw[4];
-    auto load = [&]() {
-      raw[0] = ld_stream16(x);
-      raw[1] = ld_stream16(x + apart);
-      if (kMode == kNormBwd) {
-        raw[2] = ld_stream16(g);
-        raw[3] = ld_stream16(g + apart);
-      }
-    };
-    load();  // in flight while the angles are computed
     if (first) {
       first = false;
       fill_turns = turns_of(p.freq[fill_pair]);
       if (kMode != kRotate) {
         for (int e = threadIdx.x; e < p.D; e += kVecThreads) {
-          // entry e as the i-th a or b of its unit
-          const bool halves = !kInter && e < 2 * p.half;
-          const int c = halves ? e % p.half : e;
-          const int eu = halves ? c / V : e / (2 * V), r = halves ? c % V : e % (2 * V);
-          const int i = halves ? r + (e < p.half ? 0 : V) : kInter ? r / 2 + r % 2 * V : r;
+          // entry e as the i-th a or b of its unit: c-th of the first or second
+          // half of its part
+          const bool turns = e < 2 * p.half;
+          const int len = turns ? p.half : past, from = turns ? 0 : 2 * p.half;
+          const int second = e - from >= len, c = e - from - second * len;
+          const int eu = (turns ? 0 : p.half / V) + c / V, r = c % V;
+          const int i = kInter ? second * (V / 2) + r / 2 + r % 2 * V : r + second * V;
           const int at = ((i / 4) * 32 + eu) * 4 + i % 4;
           w_smem[0][at] = weight_at<T>(p, p.t[0].w, e);
           if (p.k_slots) w_smem[1][at] = weight_at<T>(p, p.t[1].w, e);
@@ -343,7 +394,14 @@ __global__ void __launch_bounds__(kVecThreads, kMode == kRotate ? 6 : kMode == k
       if (at < tokens) {
         const unsigned ab = fast_div(at, p.by_M);
         const unsigned long long turns = step_pair == 0 ? fill_turns : turns_of(p.freq[i]);
-        table[buf][((tt * (V / 2) + i % V / 2) * turned_units + i / V) * 2 + i % 2] =
+        // pair i is the j-th of unit `unit`
+        int unit = i / V, j = i % V;
+        if (kInter) {
+          const int vec = i / (V / 2), second = vec >= turned_units;
+          unit = vec - second * turned_units;
+          j = second * (V / 2) + i % (V / 2);
+        }
+        table[buf][((tt * (V / 2) + j / 2) * turned_units + unit) * 2 + j % 2] =
             turn_of<T>(p, position_of(p, ab, at - ab * p.by_M.d), turns);
       }
       tt += step_tok;
@@ -412,13 +470,12 @@ __global__ void __launch_bounds__(kVecThreads, kMode == kRotate ? 6 : kMode == k
     for (int k = 0, h = h0; k < p.trips; ++k, h += h_step) {
       const bool row = here && h < H;
       uint64_t f[V], gr[kMode == kNormBwd ? V : 1];
-      unpack_unit<T, kInter>(raw[0], raw[1], f);
-      if constexpr (kMode == kNormBwd) unpack_unit<T, kInter>(raw[2], raw[3], gr);
-      if (h + h_step < H) {  // else the same row again, for nothing
-        x += x_step;
-        if (kMode == kNormBwd) g += g_step;
-      }
-      load();
+      fetch(at_ring == 0 ? kDepth - 1 : at_ring - 1);
+      copies_wait<kDepth - 1>();
+      unpack_unit<T, kInter>(ring[at_ring][0][threadIdx.x], ring[at_ring][1][threadIdx.x], f);
+      if constexpr (kMode == kNormBwd)
+        unpack_unit<T, kInter>(ring[at_ring][2][threadIdx.x], ring[at_ring][3][threadIdx.x], gr);
+      at_ring = at_ring == kDepth - 1 ? 0 : at_ring + 1;
       if constexpr (kMode == kNormBwd) {
         // with u = w R^T g, both sums in one round of shuffles:
         //   dx = r (u - x r^2 sum(u x) / D),  dw += (R^T g) (x r)
@@ -585,12 +642,12 @@ Launch plan(const vlak_rotary_args* a, int mode, int sm_count) {
     }
     if (!spread || trips >= 16) break;
   }
-  // Blocks: a tile each for the rotation, whose blocks start cheaply; the norm's
-  // lay out weights first, and the backward pass writes a partial weight
-  // gradient per block, so these loop (over resident blocks, twice as many
-  // forward: 37.4 -> 36.2 us for 8191 tokens of 40 heads of 128)
   const int64_t tiles = (tokens + l.block_tokens - 1) / l.block_tokens;
-  l.blocks = static_cast<int>(std::min<int64_t>(tiles, (mode == kRotate ? 64ll : mode == kNormFwd ? 10ll : 4ll) * sm_count));
+  // Blocks: for the norm as many as are resident, which go over their tiles with
+  // rows of the next one in flight, and lay out their weights, and write a partial
+  // weight gradient, once. For the rotation alone a tile each, up to 64 per SM:
+  // 2 x 8192 tokens of 40 heads of 128 in 53 us, against 63 by resident blocks.
+  l.blocks = static_cast<int>(std::min<int64_t>(tiles, (mode == kRotate ? 64ll : vec_blocks(mode)) * sm_count));
   return l;
 }
 
