@@ -93,6 +93,18 @@ def test_c_abi_refuses_workspaces():
     assert n.value == 0
 
 
+@pytest.mark.parametrize("attn", [dict(B=1 << 20, M=1 << 20), dict(B=1 << 30, N=1 << 30),
+                                  dict(B=(1 << 31) - 1, M=(1 << 31) - 1, N=(1 << 31) - 1),
+                                  dict(B=1 << 30, M=1, N=1)])
+def test_c_abi_refuses_what_no_memory_holds(attn):
+    L = lib()
+    t, n = args(dict(attn, prefix_len=-1, dead_start=0, dead_end=0)), ctypes.c_int64(0)
+    assert L.vlak_attn_gqa_train_workspace_size(ctypes.byref(t), ctypes.byref(n)) == 1
+    assert L.vlak_attn_gqa_bwd_workspace_size(ctypes.byref(t), ctypes.byref(n)) == 1
+    assert L.vlak_attn_gqa_train_fwd(ctypes.byref(t), 0x1000, 1 << 60, None) == 1
+    assert L.vlak_attn_gqa_bwd(ctypes.byref(t), 0x1000, 1 << 60, None) == 1
+
+
 def test_ops_have_cuda_kernels_only():
     attention._ensure_registered_train()
     for name in ("train", "fwd_lse", "bwd"):

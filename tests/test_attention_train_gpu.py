@@ -305,6 +305,20 @@ def test_expanded_inputs_and_gradient():
     assert torch.equal(dv, ref[3].sum(0, keepdim=True))
 
 
+def test_one_tensor_as_queries_keys_and_values():
+    x, _, _, do = make(2, 150, 150, 4, 4, seed=5)
+    leaf = x.detach().requires_grad_(True)
+    o = attend(leaf, leaf, leaf, prefix_len=0)
+    (d,) = torch.autograd.grad(o, (leaf,), do)
+    ref = orc.train(x, x, x, do, orc.analytic(150, 150, 0))
+    want = sum(ref[n][0] for n in ("dq", "dk", "dv"))
+    # autograd adds the three in bf16: two more roundings of partial sums
+    size = sum(ref[n][0].abs() for n in ("dq", "dk", "dv"))
+    bound = sum(ref[n][1] for n in ("dq", "dk", "dv")) * (1 + 2 ** -7) + 2 * 2.0 ** -8 * (1 + 2 ** -7) * size
+    assert ((d.double() - want).abs() <= bound + 1e-30).all()
+    check((o.detach(),), {"o": ref["o"]})
+
+
 def test_frozen_inputs():
     q, k, v, do = make(2, 50, 100, 6, 2)
     ref = step(q, k, v, do)

@@ -119,6 +119,15 @@ def test_norm_rotary(shape, inter, dt):
         within(dw, rw, (x.numel() // D + depth) * E * tw)
 
 
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+@pytest.mark.parametrize("inter", [False, True])
+def test_more_tokens_than_resident_blocks(inter, dt):
+    # a block goes over several tiles, fetching rows of the next ones meanwhile
+    test_norm_rotary((1, 5003, 9, 3, 128, 64), inter, dt)
+    test_norm_rotary((2, 2501, 7, 1, 80, 80), inter, dt)
+    test_rotary((1, 40009, 1, 1, 256, 128), inter, dt)
+
+
 @pytest.mark.parametrize("dt", list(DTYPES))
 @pytest.mark.parametrize("inter", [False, True])
 def test_rotary_gradient(inter, dt):

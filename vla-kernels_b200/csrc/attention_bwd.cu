@@ -935,7 +935,7 @@ cudaError_t launch_both(const BwdParams& p, unsigned n_stats, unsigned grid, cud
 
 int bwd_validate(const vlak_attn_train_args* a, int64_t* P, float* scale) {
   if (!a) return set_error(VLAK_ERR_INVALID_ARGUMENT, "fused_attention_gqa_bwd: null arguments");
-  int st = vlak_attn_gqa_check(&a->attn, P, scale);
+  int st = check_train(&a->attn, P, scale, "fused_attention_gqa_bwd");
   if (st != VLAK_OK) return st;
   const void* ptrs[4] = {a->grad_o, a->dq, a->dk, a->dv};
   for (const void* ptr : ptrs)
@@ -1090,7 +1090,7 @@ extern "C" int vlak_attn_gqa_bwd_workspace_size(const vlak_attn_train_args* args
     a.prefix_len = -1;
     a.dead_start = a.dead_end = 0;
   }
-  int st = vlak_attn_gqa_check(&a, nullptr, nullptr);
+  int st = check_train(&a, nullptr, nullptr, "workspace size");
   if (st != VLAK_OK) return st;
   if (a.B > 0 && a.M > 0 && a.N > 0)
     *bytes = plan_bwd(&a, args->dk || args->dv, args->mask != nullptr).bytes;

@@ -374,6 +374,17 @@ inline TrainShape train_shape(const vlak_attn_gqa_args* a, int64_t P, float scal
   s.by_gb = fast_div_by(static_cast<unsigned>(s.Gb));
   return s;
 }
+// The inference entry points' checks, and that counts stay within 64 bits (2^40
+// rows of 128 bytes are more than any memory).
+inline int check_train(const vlak_attn_gqa_args* a, int64_t* P, float* scale, const char* op) {
+  const int st = vlak_attn_gqa_check(a, P, scale);
+  if (st != VLAK_OK) return st;
+  constexpr double kMost = 0x1p40;
+  if (static_cast<double>(a->B) * a->M * a->H > kMost || static_cast<double>(a->B) * a->N * a->Hkv > kMost ||
+      static_cast<double>(a->B) * a->Hkv > INT32_MAX)
+    return set_errorf(VLAK_ERR_INVALID_ARGUMENT, "%s: too many rows or keys", op);
+  return VLAK_OK;
+}
 // The masks of a call beyond the analytic one.
 inline int check_train_masks(const vlak_attn_train_args& a, const char* op) {
   if (a.lengths && a.mask)

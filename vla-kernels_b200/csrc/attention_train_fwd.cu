@@ -723,7 +723,7 @@ int run_fwd(const vlak_attn_train_args* t, void* workspace, int64_t ws_bytes, vo
   const vlak_attn_gqa_args* a = &args.attn;
   int64_t P = 0;
   float scale = 0.f;
-  int st = vlak_attn_gqa_check(a, &P, &scale);
+  int st = check_train(a, &P, &scale, op);
   if (st == VLAK_OK) st = check_train_masks(args, op);
   if (st != VLAK_OK) return st;
   if (reinterpret_cast<uintptr_t>(args.lse) % 4 != 0)
@@ -825,7 +825,7 @@ extern "C" int vlak_attn_gqa_train_workspace_size(const vlak_attn_train_args* ar
     a.prefix_len = -1;
     a.dead_start = a.dead_end = 0;
   }
-  const int st = vlak_attn_gqa_check(&a, nullptr, nullptr);
+  const int st = check_train(&a, nullptr, nullptr, "workspace size");
   if (st != VLAK_OK) return st;
   if (a.B > 0 && a.M > 0 && a.N > 0) *bytes = plan_fwd(&a, args->mask != nullptr).bytes;
   return VLAK_OK;
