@@ -117,7 +117,7 @@ def build_torch_shim(force: bool = False) -> str:
     for libdir in cpp.library_paths():
         cmd += ["-L", libdir, f"-Wl,-rpath,{libdir}"]
     cmd += ["-L", LIB_DIR, "-Wl,-rpath,$ORIGIN", "-lvlak_b200",
-            "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch"]
+            "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch"]
     _run(cmd)
     os.replace(TORCH_LIB + ".tmp", TORCH_LIB)
     return TORCH_LIB

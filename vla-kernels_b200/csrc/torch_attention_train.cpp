@@ -20,6 +20,7 @@ namespace {
 
 using at::Tensor;
 using vlak_torch::check_status;
+using vlak_torch::new_empty;
 using vlak_torch::raise_pending_device_error;
 using OptTensor = std::optional<Tensor>;
 
@@ -97,14 +98,14 @@ std::tuple<Tensor, Tensor, Tensor> forward(const Tensor& q_in, const Tensor& k_i
   const Masks m = check_masks(a, q, lengths, attn_mask, prefix_len, dead_start, dead_end, op);
   c10::cuda::CUDAGuard guard(q.device());
   check_status(vlak_attn_gqa_check(&a, nullptr, nullptr), op);
-  Tensor o = at::empty({a.B, a.M, a.H, 64}, q.options());
-  Tensor lse = at::empty({a.B, a.M, a.H}, q.options().dtype(at::kFloat));
+  Tensor o = new_empty(q, {a.B, a.M, a.H, 64}, q.scalar_type());
+  Tensor lse = new_empty(q, {a.B, a.M, a.H}, at::kFloat);
   Tensor o_low;
   set_o(a, o);
   vlak_attn_train_args t = train_args(a, m);
   t.lse = lse.data_ptr<float>();
   if (for_backward) {
-    o_low = at::empty({a.B, a.M, a.H, 64}, q.options().dtype(at::kChar));
+    o_low = new_empty(q, {a.B, a.M, a.H, 64}, at::kChar);
     t.o_low = o_low.data_ptr();
   }
   // workspaces: from the caching allocator on the current stream, so reused only
@@ -112,7 +113,7 @@ std::tuple<Tensor, Tensor, Tensor> forward(const Tensor& q_in, const Tensor& k_i
   int64_t bytes = 0;
   check_status(vlak_attn_gqa_train_workspace_size(&t, &bytes), op);
   Tensor ws;
-  if (bytes > 0) ws = at::empty({bytes}, q.options().dtype(at::kByte));
+  if (bytes > 0) ws = new_empty(q, {bytes}, at::kByte);
   check_status(vlak_attn_gqa_train_fwd(&t, bytes > 0 ? ws.data_ptr() : nullptr, bytes, stream()), op);
   return {o, lse, o_low};
 }
@@ -157,7 +158,7 @@ std::vector<Tensor> bwd(const Tensor& grad_o_in, const Tensor& q_in, const Tenso
   const Tensor grad_o = tma_ready(grad_o_in), o = tma_ready(o_in);
   set_o(a, o);
   check_status(vlak_attn_gqa_check(&a, nullptr, nullptr), op);
-  std::vector<Tensor> out{at::empty({a.B, a.M, a.H, 64}, q.options())};
+  std::vector<Tensor> out{new_empty(q, {a.B, a.M, a.H, 64}, q.scalar_type())};
   vlak_attn_train_args t = train_args(a, m);
   t.lse = lse.data_ptr<float>();
   t.o_low = o_low.data_ptr();
@@ -165,14 +166,14 @@ std::vector<Tensor> bwd(const Tensor& grad_o_in, const Tensor& q_in, const Tenso
   for (int d = 0; d < 3; ++d) t.grad_o_stride[d] = grad_o.stride(d);
   t.dq = out[0].data_ptr();
   if (with_kv) {
-    out.push_back(at::empty({a.B, a.N, a.Hkv, 64}, q.options()));
-    out.push_back(at::empty({a.B, a.N, a.Hkv, 64}, q.options()));
+    out.push_back(new_empty(q, {a.B, a.N, a.Hkv, 64}, q.scalar_type()));
+    out.push_back(new_empty(q, {a.B, a.N, a.Hkv, 64}, q.scalar_type()));
     t.dk = out[1].data_ptr();
     t.dv = out[2].data_ptr();
   }
   int64_t bytes = 0;
   check_status(vlak_attn_gqa_bwd_workspace_size(&t, &bytes), op);
-  const Tensor ws = at::empty({bytes}, q.options().dtype(at::kByte));
+  const Tensor ws = new_empty(q, {bytes}, at::kByte);
   check_status(vlak_attn_gqa_bwd(&t, ws.data_ptr(), bytes, stream()), op);
   return out;
 }

@@ -20,6 +20,7 @@ namespace {
 using at::Tensor;
 using vlak_torch::check_status;
 using vlak_torch::dtype_code;
+using vlak_torch::new_empty;
 using vlak_torch::raise_pending_device_error;
 using OptTensor = std::optional<Tensor>;
 using Tensors = std::vector<Tensor>;
@@ -55,14 +56,13 @@ vlak_rotary_args rotary_args(const Tensor& q, const OptTensor& k, const Tensor& 
               op, ": positions must be (B, M), (1, M) or (M,)");
   TORCH_CHECK(inv_freq.scalar_type() == at::kDouble && inv_freq.dim() == 1, op,
               ": inv_freq must be a float64 vector");
-  keep.push_back(positions.expand({B, M}));
   keep.push_back(inv_freq.contiguous());
   vlak_rotary_args a{};
-  a.positions = keep[0].data_ptr();
+  a.positions = positions.data_ptr();
   a.pos_dtype = positions.scalar_type() == at::kLong ? VLAK_I64 : VLAK_I32;
-  a.pos_stride[0] = keep[0].stride(0);
-  a.pos_stride[1] = keep[0].stride(1);
-  a.inv_freq = static_cast<const double*>(keep[1].data_ptr());
+  a.pos_stride[0] = positions.dim() == 1 || positions.size(0) != B ? 0 : positions.stride(0);
+  a.pos_stride[1] = positions.stride(-1);
+  a.inv_freq = static_cast<const double*>(keep[0].data_ptr());
   a.B = B;
   a.M = M;
   a.D = D;
@@ -97,7 +97,7 @@ void set_weights(vlak_rotary_args& a, const Tensor& q, const OptTensor& k, const
   a.weight_dtype = dtype_code(q_weight.scalar_type());
 }
 
-Tensor empty_heads(const Tensor& x) { return at::empty(x.sizes(), x.options()); }
+Tensor empty_heads(const Tensor& x) { return new_empty(x, x.sizes(), x.scalar_type()); }
 void* stream() { return c10::cuda::getCurrentCUDAStream().stream(); }
 
 Tensors rotary(const Tensor& q, const OptTensor& k, const Tensor& positions,
@@ -164,14 +164,14 @@ Tensors qk_norm_rotary_bwd(const Tensor& grad_q, const OptTensor& grad_k, const 
     for (int d = 0; d < 3; ++d) a.t[i].grad_stride[d] = keep.back().stride(d);
     out.push_back(empty_heads(x));
     a.t[i].y = out.back().data_ptr();
-    dw.push_back(at::empty({a.D}, q_weight.options()));
+    dw.push_back(new_empty(q, {a.D}, q_weight.scalar_type()));
     a.t[i].grad_weight = dw.back().data_ptr();
   }
   int64_t bytes = 0;
   check_status(vlak_qk_norm_rotary_workspace_size(&a, &bytes), op);
   // from the caching allocator on the current stream: reused only by work
   // queued behind this call there, and a captured graph's own while it lives
-  const Tensor ws = at::empty({bytes}, q.options().dtype(at::kByte));
+  const Tensor ws = new_empty(q, {bytes}, at::kByte);
   check_status(vlak_qk_norm_rotary_bwd(&a, ws.data_ptr(), bytes, stream()), op);
   out.insert(out.end(), dw.begin(), dw.end());
   return out;

@@ -2,6 +2,7 @@
 #pragma once
 
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 
 #include "vlak_b200.h"
 
@@ -32,6 +33,13 @@ inline int dtype_code(at::ScalarType t) {
     case at::kDouble: return VLAK_F64;
     default: return -1;
   }
+}
+
+// A new contiguous tensor on the device of `like`. For implementations under the
+// CUDA key only: it does not go through the dispatcher again, which cost a
+// training call, with its seven or eight tensors, 3 of 80 us.
+inline at::Tensor new_empty(const at::Tensor& like, at::IntArrayRef sizes, at::ScalarType type) {
+  return at::Tensor(at::detail::empty_cuda(sizes, type, like.device(), std::nullopt));
 }
 
 // Checks and arguments of the GQA attention ops (torch_ops.cpp).
