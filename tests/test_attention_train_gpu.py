@@ -290,6 +290,22 @@ def test_layouts_read_in_place():
             assert torch.equal(a, b)
 
 
+def test_strides_past_32_bits():
+    # samples 2^31 + 2^20 entries apart in one buffer, also those of the gradient
+    far = (1 << 31) + (1 << 20)
+    q, k, v, do = make(2, 70, 70, 6, 2, seed=9)
+    buf = torch.empty(far + (1 << 20), device="cuda", dtype=torch.bfloat16)
+    placed, at = [], 0
+    for t in (q, k, v, do):
+        p = buf.as_strided(t.shape, (far, *t.stride()[1:]), at)
+        p.copy_(t)
+        placed.append(p)
+        at += t.stride(0)
+    assert at <= 1 << 20
+    got, same = step(*placed, prefix_len=0), step(q, k, v, do, prefix_len=0)
+    assert all(torch.equal(a, b) for a, b in zip(got, same))
+
+
 def test_expanded_inputs_and_gradient():
     # a batch that shares its keys, and a loss that hands back one expanded number
     B, M, N, H, Hkv = 3, 20, 60, 4, 2

@@ -222,6 +222,30 @@ def test_strides_read_in_place_or_copied():
             within(y, orc.turn(u, th), 34 * E * orc.pair_size(u, th))
 
 
+@pytest.mark.parametrize("inter", [False, True])
+@pytest.mark.parametrize("D", [64, 72])
+def test_strides_past_32_bits(D, inter):
+    # tokens, and in the other tensor heads, 2^31 + 2^20 entries apart
+    far = (1 << 31) + (1 << 20)
+    buf = torch.empty(far + (1 << 16), device="cuda", dtype=torch.bfloat16)
+    q, k = make(1, 2, 3, 2, D, torch.bfloat16, seed=D)
+    fq = buf.as_strided(q.shape, (far * 2, far, D, 1), 0)
+    fk = buf.as_strided(k.shape, (far * 2, D, far, 1), 1 << 12)
+    fq.copy_(q)
+    fk.copy_(k)
+    w = 1 + torch.rand(D, device="cuda", generator=gen(3))
+    f = api().rotary_frequencies(D - 8 if D == 72 else D, device="cuda")
+    pos = torch.tensor([5, 77], device="cuda")
+    for call in (lambda a, b: api().rotary(a, b, pos, f, interleaved=inter),
+                 lambda a, b: api().qk_norm_rotary(a, b, w, w, pos, f, interleaved=inter)):
+        assert all(torch.equal(x, y) for x, y in zip(call(fq, fk), call(q, k)))
+    leaf = [t.detach().requires_grad_(True) for t in (fq, fk)]
+    near = [t.detach().requires_grad_(True) for t in (q, k)]
+    got = torch.autograd.grad(api().qk_norm_rotary(*leaf, w, w, pos, f, interleaved=inter), leaf, (fq, fk))
+    want = torch.autograd.grad(api().qk_norm_rotary(*near, w, w, pos, f, interleaved=inter), near, (q, k))
+    assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
 def test_broadcast_heads_and_gradients():
     # a gradient that is one expanded number, and heads that are one expanded
     # head: their gradient is the sum over the heads
