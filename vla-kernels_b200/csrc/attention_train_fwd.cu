@@ -191,8 +191,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_train_fwd(const __grid_const
       const uint32_t q = n % kQueue;
       if (!__all_sync(kFullMask, bounded_wait(&bars->it_empty[q], ((n / kQueue) & 1) ^ 1, abort_flag)))
         break;
-      // items in turn over the CTAs: the long ones come first
-      const long long id = blockIdx.x + static_cast<long long>(n) * gridDim.x;
+      // items in turn over the CTAs. Under a staircase the long ones come first, so
+      // every other round goes in reverse, else the first CTA had the longest of
+      // each: causal, 2 x 4096 rows, 15 / 5 heads, 125 -> 116 us
+      const bool back = kMode == kMaskAnalytic && (n & 1);
+      const long long id =
+          static_cast<long long>(n) * gridDim.x + (back ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
       Item it{};
       if (id < p.n_items)
         it = decode_item<kMode>(p, static_cast<int>(id));
