@@ -56,8 +56,9 @@ constexpr int kWarpProducer = kComputeWarps, kWarpScores = kComputeWarps + 1,
               kWarpAccum = kComputeWarps + 2;  // (kComputeWarps + 3 has no role)
 constexpr int kWarpOutput = kComputeWarps + 4, kOutputWarps = 4;
 constexpr int kThreads = 32 * (kWarpOutput + kOutputWarps);
-// Registers by warpgroup: compute, issue, output.
-constexpr int kRegsLaunch = 80, kRegsCompute = 88, kRegsIssue = 48, kRegsOutput = 80;
+// Registers by warpgroup: compute, issue, output, whose four accumulators of 16
+// columns are the most.
+constexpr int kRegsLaunch = 80, kRegsCompute = 80, kRegsIssue = 40, kRegsOutput = 112;
 static_assert(32 * kComputeWarps * kRegsCompute + 128 * kRegsIssue + 32 * kOutputWarps * kRegsOutput <=
                   kThreads * kRegsLaunch,
               "the split must fit the launch's registers");
@@ -329,7 +330,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_train_fwd(const __grid_const
     bounded_wait(&bars->drain[1], 0, abort_flag, false);
     __syncwarp();
   } else if (warp < kComputeWarps) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsCompute));
+    static_assert(kRegsCompute == kRegsLaunch, "compute warps keep the launch's registers");
     // Compute warps: a row per lane, 32 of a step's 64 keys; the softmax of one
     // stream.
     const int group = warp >> 3, quarter = warp & 3, gq = (warp >> 2) & 1;
@@ -462,8 +463,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_train_fwd(const __grid_const
       ++live;
     }
   } else if (warp >= kWarpOutput) {
-    // (kRegsOutput is the launch's count: nothing to set)
-    static_assert(kRegsOutput == kRegsLaunch, "output warps keep the launch's registers");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsOutput));
     // Outputs: the streams joined, staged over the item's Q tile in the swizzled
     // layout of the map, then TMA stores; or a part's sums. One lane quarter of
     // TMEM per warp.
@@ -471,6 +471,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_train_fwd(const __grid_const
     const int tl = quarter * 32 + lane;
     const uint32_t tbase = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
     uint32_t t = 0, live = 0;
+    int stored = -1;  // tile that stores are reading (first warp)
     Turn<kTiles> ab;
     for (uint32_t n = 0;; ++n) {
       Item it;
@@ -513,11 +514,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_train_fwd(const __grid_const
       }
       __syncwarp();
       mbar_arrive_elect(&bars->ml_empty[mb]);
-      const float inv = L == 0.f ? 0.f : 1.f / L;
+      const float inv = L == 0.f ? 0.f : __fdividef(1.f, L);
       if (p.parts > 1) {
         if (r.valid) p.ml[part_row] = make_float2(m, L);
       } else {
-        if (r.valid) p.lse[row] = L == 0.f ? -INFINITY : m + log2f(L);
+        if (r.valid) p.lse[row] = L == 0.f ? -INFINITY : m + __log2f(L);
 #pragma unroll
         for (int i = 0; i < 4; ++i) w[i] *= inv;
       }
@@ -525,31 +526,35 @@ __global__ void __launch_bounds__(kThreads, 1) attn_train_fwd(const __grid_const
       tc_fence_after();
       uint8_t* a0 = a_smem + ab.i * kTileBytes;
       float* sums = p.parts > 1 ? p.sums + part_row * 64 : nullptr;
-      // Join and round all 64 columns first, so that the next item may soon
-      // accumulate; then stage them.
-      uint32_t hi[32], lo[16];
+      uint8_t* stage = a0 + tl * kRowBytes;
+      uint4* low = p.parts == 1 && p.o_low != nullptr && r.valid ? reinterpret_cast<uint4*>(p.o_low + row * 64)
+                                                                 : nullptr;
       uint64_t w2[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) w2[i] = f2_pack(w[i], w[i]);
+#pragma unroll 1
+      for (int q = 0; q < 4; ++q) {  // 16 columns of the four streams at a time
+        float x[4][16];
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {  // 16 columns at a time
-        uint64_t o2[8] = {};
-#pragma unroll
-        for (int g = 0; g < 2; ++g) {
-          if (!has[g]) continue;
-          float x[2][16];
-          tmem_ld16(tbase + kAcc + 128 * g + 16 * q, x[0]);
-          tmem_ld16(tbase + kAcc + 128 * g + 64 + 16 * q, x[1]);
-          tmem_wait_ld();
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            o2[i] = f2_fma(f2_pack(x[1][2 * i], x[1][2 * i + 1]), w2[2 * g + 1],
-                           f2_fma(f2_pack(x[0][2 * i], x[0][2 * i + 1]), w2[2 * g], o2[i]));
-        }
+        for (int g = 0; g < 2; ++g)
+          if (has[g]) {
+            tmem_ld16(tbase + kAcc + 128 * g + 16 * q, x[2 * g]);
+            tmem_ld16(tbase + kAcc + 128 * g + 64 + 16 * q, x[2 * g + 1]);
+          }
+        tmem_wait_ld();
         if (q == 3) {  // read: the next item may accumulate
           tc_fence_before();
           mbar_arrive_elect(&bars->acc_empty);
         }
+        uint64_t o2[8] = {};
+#pragma unroll
+        for (int g = 0; g < 2; ++g)
+          if (has[g]) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              o2[i] = f2_fma(f2_pack(x[2 * g + 1][2 * i], x[2 * g + 1][2 * i + 1]), w2[2 * g + 1],
+                             f2_fma(f2_pack(x[2 * g][2 * i], x[2 * g][2 * i + 1]), w2[2 * g], o2[i]));
+          }
         float o[16];
 #pragma unroll
         for (int i = 0; i < 8; ++i) f2_unpack(o2[i], o[2 * i], o[2 * i + 1]);
@@ -561,19 +566,17 @@ __global__ void __launch_bounds__(kThreads, 1) attn_train_fwd(const __grid_const
                   make_float4(o[4 * v], o[4 * v + 1], o[4 * v + 2], o[4 * v + 3]);
           }
         } else {
+          uint32_t hi[8];
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            hi[8 * q + i] = L == 0.f ? 0u : pack_bf16x2(o[2 * i], o[2 * i + 1]);
+          for (int i = 0; i < 8; ++i) hi[i] = L == 0.f ? 0u : pack_bf16x2(o[2 * i], o[2 * i + 1]);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) lo[4 * q + i] = low_bytes(o + 4 * i, hi + 8 * q + 2 * i);
+          for (int v = 0; v < 2; ++v)
+            st_shared_v4(stage + (static_cast<uint32_t>(2 * q + v) ^ static_cast<uint32_t>(tl & 7)) * 16,
+                         hi[4 * v], hi[4 * v + 1], hi[4 * v + 2], hi[4 * v + 3]);
+          if (low != nullptr)
+            low[q] = make_uint4(low_bytes(o, hi), low_bytes(o + 4, hi + 2), low_bytes(o + 8, hi + 4),
+                                low_bytes(o + 12, hi + 6));
         }
-      }
-      if (p.parts == 1) {
-        uint8_t* stage = a0 + tl * kRowBytes;
-#pragma unroll
-        for (int v = 0; v < 8; ++v)
-          st_shared_v4(stage + (static_cast<uint32_t>(v) ^ static_cast<uint32_t>(tl & 7)) * 16, hi[4 * v],
-                       hi[4 * v + 1], hi[4 * v + 2], hi[4 * v + 3]);
       }
       fence_proxy_async_smem();
       __syncwarp();
@@ -581,22 +584,24 @@ __global__ void __launch_bounds__(kThreads, 1) attn_train_fwd(const __grid_const
       if (warp == kWarpOutput) {
         if (!__all_sync(kFullMask, bounded_wait<1>(&bars->staged, live & 1, abort_flag))) break;
         if (lane == 0) {
+          // the tile of the item before, whose stores have read it by now (waiting
+          // for them at once took 1.6K cycles of an item's 7K)
+          if (stored >= 0) {
+            bulk_wait_read0();
+            mbar_arrive(&bars->a_empty[stored]);
+          }
+          stored = p.parts == 1 ? static_cast<int>(ab.i) : -1;
           if (p.parts == 1) {
             for (int i = 0; i < it.n_here; ++i) {
               const int hb = fast_div(it.s0 + i, p.by_mt_count), m0 = (it.s0 + i - hb * p.n_mt) * p.MT;
               tma_store_4d(&p.tm_o, a0 + i * kSubBytes, 0, it.kvh * p.G + hb * p.Gb, m0, it.b);
             }
             bulk_commit_group();
-            bulk_wait_read0();
+          } else {
+            mbar_arrive(&bars->a_empty[ab.i]);
           }
-          mbar_arrive(&bars->a_empty[ab.i]);
         }
         __syncwarp();
-      }
-      if (p.parts == 1 && p.o_low != nullptr && r.valid) {
-        uint4* dst = reinterpret_cast<uint4*>(p.o_low + row * 64);
-#pragma unroll
-        for (int v = 0; v < 4; ++v) dst[v] = make_uint4(lo[4 * v], lo[4 * v + 1], lo[4 * v + 2], lo[4 * v + 3]);
       }
       ab.next();
       t += it.live;
