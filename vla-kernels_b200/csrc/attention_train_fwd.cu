@@ -53,7 +53,7 @@ constexpr int kQueue = 8;                    // items handed out and not yet see
 constexpr int kGroupWarps = 8;               // as in the backward kernel
 constexpr int kComputeWarps = 2 * kGroupWarps;
 constexpr int kWarpProducer = kComputeWarps, kWarpScores = kComputeWarps + 1,
-              kWarpAccum = kComputeWarps + 2;  // (kComputeWarps + 3 has no role)
+              kWarpAccum = kComputeWarps + 2;  // kComputeWarps + 3: stores
 constexpr int kWarpOutput = kComputeWarps + 4, kOutputWarps = 4;
 constexpr int kThreads = 32 * (kWarpOutput + kOutputWarps);
 // Registers by warpgroup: compute, issue, output, whose four accumulators of 16
@@ -90,7 +90,7 @@ struct Barriers {
   uint64_t s_full[kStages], x_full[kStages], t_empty[kStages];
   uint64_t pv_done[2];                       // [group]
   uint64_t ml_full[2], ml_empty[2];          // streams' maxima and sums of an item
-  uint64_t out_full, staged, acc_empty, drain[2];
+  uint64_t out_full, staged[kTiles], acc_empty, drain[2];
   uint64_t it_full[kQueue], it_empty[kQueue];
   Item item[kQueue];
   uint32_t tmem_base;
@@ -137,6 +137,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_train_fwd(const __grid_const
     for (int i = 0; i < kTiles; ++i) {
       mbar_init(&bars->a_full[i], 1);
       mbar_init(&bars->a_empty[i], 1);
+      mbar_init(&bars->staged[i], kOutputWarps);
     }
     for (int i = 0; i < kRing; ++i) {
       mbar_init(&bars->b_full[i], 1);
@@ -155,10 +156,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_train_fwd(const __grid_const
     }
     for (int i = 0; i < kQueue; ++i) {
       mbar_init(&bars->it_full[i], 1);
-      mbar_init(&bars->it_empty[i], kComputeWarps + 2 + kOutputWarps);
+      mbar_init(&bars->it_empty[i], kComputeWarps + 3 + kOutputWarps);
     }
     mbar_init(&bars->out_full, 1);
-    mbar_init(&bars->staged, kOutputWarps);
     mbar_init(&bars->acc_empty, kOutputWarps);
     bars->abort_flag = 0;
     fence_mbar_init();
@@ -465,13 +465,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_train_fwd(const __grid_const
   } else if (warp >= kWarpOutput) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsOutput));
     // Outputs: the streams joined, staged over the item's Q tile in the swizzled
-    // layout of the map, then TMA stores; or a part's sums. One lane quarter of
+    // layout of the map; or a part's sums. One lane quarter of
     // TMEM per warp.
     const int quarter = warp & 3;
     const int tl = quarter * 32 + lane;
     const uint32_t tbase = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
     uint32_t t = 0, live = 0;
-    int stored = -1;  // tile that stores are reading (first warp)
     Turn<kTiles> ab;
     for (uint32_t n = 0;; ++n) {
       Item it;
@@ -580,38 +579,40 @@ __global__ void __launch_bounds__(kThreads, 1) attn_train_fwd(const __grid_const
       }
       fence_proxy_async_smem();
       __syncwarp();
-      mbar_arrive_elect(&bars->staged);
-      if (warp == kWarpOutput) {
-        if (!__all_sync(kFullMask, bounded_wait<1>(&bars->staged, live & 1, abort_flag))) break;
-        if (lane == 0) {
-          // the tile of the item before, whose stores have read it by now (waiting
-          // for them at once took 1.6K cycles of an item's 7K)
-          if (stored >= 0) {
-            bulk_wait_read0();
-            mbar_arrive(&bars->a_empty[stored]);
-          }
-          stored = p.parts == 1 ? static_cast<int>(ab.i) : -1;
-          if (p.parts == 1) {
-            for (int i = 0; i < it.n_here; ++i) {
-              const int hb = fast_div(it.s0 + i, p.by_mt_count), m0 = (it.s0 + i - hb * p.n_mt) * p.MT;
-              tma_store_4d(&p.tm_o, a0 + i * kSubBytes, 0, it.kvh * p.G + hb * p.Gb, m0, it.b);
-            }
-            bulk_commit_group();
-          } else {
-            mbar_arrive(&bars->a_empty[ab.i]);
-          }
-        }
-        __syncwarp();
-      }
+      mbar_arrive_elect(&bars->staged[ab.i]);
       ab.next();
       t += it.live;
       ++live;
     }
-    // the stores complete before the CTA exits
-    if (warp == kWarpOutput && lane == 0) bulk_wait_all0();
-    __syncwarp();
   } else {
     less_registers();
+    // Stores of the staged outputs, which release the items' tiles. (In the output
+    // warps they took 2 to 3K cycles of an item's 7K.) A tile's barrier is not
+    // arrived at again before the tile has been released.
+    Turn<kTiles> ab;
+    for (uint32_t n = 0;; ++n) {
+      Item it;
+      if (!take_item(n, it) || it.live < 0) break;
+      if (it.live == 0) continue;
+      if (!__all_sync(kFullMask, bounded_wait<1>(&bars->staged[ab.i], ab.round, abort_flag))) break;
+      if (lane == 0) {
+        if (p.parts == 1) {
+          for (int i = 0; i < it.n_here; ++i) {
+            const int hb = fast_div(it.s0 + i, p.by_mt_count), m0 = (it.s0 + i - hb * p.n_mt) * p.MT;
+            tma_store_4d(&p.tm_o, a_smem + ab.i * kTileBytes + i * kSubBytes, 0, it.kvh * p.G + hb * p.Gb, m0,
+                         it.b);
+          }
+          bulk_commit_group();
+          bulk_wait_read0();
+        }
+        mbar_arrive(&bars->a_empty[ab.i]);
+      }
+      __syncwarp();
+      ab.next();
+    }
+    // the stores complete before the CTA exits
+    if (lane == 0) bulk_wait_all0();
+    __syncwarp();
   }
 
   tc_fence_before();
