@@ -79,7 +79,7 @@ constexpr int kComputeWarps = 2 * kGroupWarps;
 // group pauses at an item's end (an item of three steps took twice as long
 // when the groups did it in turn).
 constexpr int kWarpProducer = kComputeWarps, kWarpScores = kComputeWarps + 1,
-              kWarpAccum = kComputeWarps + 2;  // (kComputeWarps + 3 has no role)
+              kWarpAccum = kComputeWarps + 2;  // kComputeWarps + 3: stores
 constexpr int kWarpOutput = kComputeWarps + 4, kOutputWarps = 4;
 constexpr int kThreads = 32 * (kWarpOutput + kOutputWarps);
 // Registers: a compute thread wants more than an even share, the others less.
@@ -168,7 +168,7 @@ struct Barriers {
   uint64_t a_full[kTiles], a_empty[kTiles];  // stationary tiles of an item
   uint64_t b_full[kRing], b_empty[kRing];  // streamed pairs
   uint64_t s_full[kStages], x_full[kStages], t_empty[kStages];
-  uint64_t out_full, staged, acc_empty, drain[2];
+  uint64_t out_full, staged[kTiles], acc_empty, drain[2];
   uint64_t it_full[kQueue], it_empty[kQueue];
   Item item[kQueue];
   uint32_t tmem_base;
@@ -242,6 +242,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd(const __grid_constant__ 
     for (int i = 0; i < kTiles; ++i) {
       mbar_init(&bars->a_full[i], 1);
       mbar_init(&bars->a_empty[i], 1);
+      mbar_init(&bars->staged[i], kOutputWarps);
     }
     for (int i = 0; i < kRing; ++i) {
       mbar_init(&bars->b_full[i], 1);
@@ -254,10 +255,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd(const __grid_constant__ 
     }
     for (int i = 0; i < kQueue; ++i) {
       mbar_init(&bars->it_full[i], 1);
-      mbar_init(&bars->it_empty[i], kComputeWarps + 2 + kOutputWarps);
+      mbar_init(&bars->it_empty[i], kComputeWarps + 3 + kOutputWarps);
     }
     mbar_init(&bars->out_full, 1);
-    mbar_init(&bars->staged, kOutputWarps);
     mbar_init(&bars->acc_empty, kOutputWarps);
     mbar_init(&bars->drain[0], 1);
     mbar_init(&bars->drain[1], 1);
@@ -703,7 +703,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd(const __grid_constant__ 
   } else if (warp >= kWarpOutput) {
     less_registers();
     // Outputs: the accumulators, scaled, staged over the item's stationary tiles
-    // in the swizzled layout of the maps, then TMA stores. One lane quarter of
+    // in the swizzled layout of the maps. One lane quarter of
     // TMEM per warp.
     const int quarter = warp & 3;
     const int tl = quarter * 32 + lane;  // key of a dkv item, row of a dq item
@@ -782,12 +782,24 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd(const __grid_constant__ 
       }
       fence_proxy_async_smem();
       __syncwarp();
-      mbar_arrive_elect(&bars->staged);
-      if (warp == kWarpOutput) {
-        if (!__all_sync(kFullMask, bounded_wait<1>(&bars->staged, live & 1, abort_flag))) break;
-        if (lane == 0) {
-          if (parts > 1) {
-          } else if (it.dkv) {
+      mbar_arrive_elect(&bars->staged[ab.i]);
+      ab.next();
+      ++live;
+    }
+  } else {
+    less_registers();
+    // Stores of the staged outputs, which release the items' tiles. A tile's
+    // barrier is not arrived at again before the tile has been released.
+    Turn<kTiles> ab;
+    for (uint32_t n = 0;; ++n) {
+      Item it;
+      if (!take_item(n, it) || it.live < 0) break;
+      if (it.live == 0) continue;
+      if (!__all_sync(kFullMask, bounded_wait<1>(&bars->staged[ab.i], ab.round, abort_flag))) break;
+      if (lane == 0) {
+        if ((it.dkv ? p.kv_parts : p.q_parts) == 1) {
+          uint8_t* a0 = a_smem + ab.i * 4 * kSubBytes;
+          if (it.dkv) {
             tma_store_4d(&p.tm_dk, a0, 0, it.kvh, it.k0, it.b);
             tma_store_4d(&p.tm_dv, a0 + 2 * kSubBytes, 0, it.kvh, it.k0, it.b);
           } else {
@@ -796,22 +808,17 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd(const __grid_constant__ 
               tma_store_4d(&p.tm_dq, a0 + i * kSubBytes, 0, it.kvh * p.G + hb * p.Gb, m0, it.b);
             }
           }
-          if (parts == 1) {
-            bulk_commit_group();
-            bulk_wait_read0();
-          }
-          mbar_arrive(&bars->a_empty[ab.i]);
+          bulk_commit_group();
+          bulk_wait_read0();
         }
-        __syncwarp();
+        mbar_arrive(&bars->a_empty[ab.i]);
       }
+      __syncwarp();
       ab.next();
-      ++live;
     }
     // the stores complete before the CTA exits
-    if (warp == kWarpOutput && lane == 0) bulk_wait_all0();
+    if (lane == 0) bulk_wait_all0();
     __syncwarp();
-  } else {
-    less_registers();
   }
 
   tc_fence_before();
