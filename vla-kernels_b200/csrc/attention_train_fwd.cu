@@ -244,6 +244,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_train_fwd(const __grid_const
   } else if (warp == kWarpScores) {
     less_registers();
     // S = Q K^T of every step, up to kStages steps ahead of the products with V.
+    // Its waits suspend the warp, unlike the others': 4 x 1024 rows, 12 heads 30.4 ->
+    // 29.3 us (all of them suspended 29.7, the backward kernel's 59.5 -> 62).
     const uint32_t id_kk = idesc_bf16_f32(128, 64, false);
     const uint64_t a_desc = sdesc_sw128(smem_u32(a_smem)), b_desc = sdesc_sw128(smem_u32(b_smem));
     // V rows that no query sees meet P = 0 only, and may hold NaN: cleared
@@ -256,14 +258,14 @@ __global__ void __launch_bounds__(kThreads, 1) attn_train_fwd(const __grid_const
       Item it;
       if (!take_item(n, it) || it.live < 0) break;
       if (it.live == 0) continue;
-      if (!__all_sync(kFullMask, bounded_wait<1>(&bars->a_full[ab.i], ab.round, abort_flag))) break;
+      if (!__all_sync(kFullMask, bounded_wait(&bars->a_full[ab.i], ab.round, abort_flag))) break;
       const uint64_t a0 = a_desc + ab.i * (kTileBytes / 16);
       ab.next();
       Steps step;
       step.begin(it);
       for (int j = 0; j < it.live; ++j) {
-        if (!__all_sync(kFullMask, bounded_wait<1>(&bars->t_empty[st.i], st.round ^ 1, abort_flag) &&
-                                       bounded_wait<1>(&bars->b_full[s.i], s.round, abort_flag))) {
+        if (!__all_sync(kFullMask, bounded_wait(&bars->t_empty[st.i], st.round ^ 1, abort_flag) &&
+                                       bounded_wait(&bars->b_full[s.i], s.round, abort_flag))) {
           ok = false;
           break;
         }
