@@ -26,9 +26,9 @@
 // three stages of (T0, T1), so the products of the next steps, also those of the
 // next item, are issued while the current one's elementwise part runs. Sixteen
 // compute warps in two groups take the steps in turn, one warp issues the score
-// products and another the accumulating ones, four carry the outputs away. Items
-// come from a counter, the long ones first; long items of few heads are cut into
-// parts, whose fp32 sums another kernel joins in their order.
+// products and another the accumulating ones, four carry the outputs away and one
+// stores them. Items come from a counter, the long ones first; long items of few
+// heads are cut into parts, whose fp32 sums another kernel joins in their order.
 //
 // Bound: by the products' shared-memory reads and issue. A step (128 x 64) is
 // 8 SS products of about 49 cycles and 4 (dq) or 8 (dkv) TS products of about 43.

@@ -4,7 +4,8 @@
 // Items and pipeline are those of the backward kernel (attention_bwd.cu): a row
 // item is 128 query rows (stationary Q) that walk the keys in chunks of 64, a
 // persistent CTA per SM has all 512 columns of TMEM, one warp issues S = Q K^T of
-// the next steps while the softmax of the current ones runs, another O += P V.
+// the next steps while the softmax of the current ones runs, another O += P V; four
+// join the outputs and one stores them.
 //
 // Four sums per row. Two groups of compute warps take the steps in turn, and in
 // a group two warps share each row, each with half of the chunk's keys. Each of
