@@ -235,6 +235,7 @@ struct TrainFunction : torch::autograd::Function<TrainFunction> {
 Tensor train_autograd(const Tensor& q, const Tensor& k, const Tensor& v, double scale,
                       int64_t prefix_len, int64_t dead_start, int64_t dead_end,
                       const OptTensor& lengths, const OptTensor& attn_mask) {
+  vlak_torch::refuse_tangents({q, k, v}, "fused_attention_gqa_train");
   if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad()))
     return TrainFunction::apply(q, k, v, scale, prefix_len, dead_start, dead_end, lengths, attn_mask);
   static auto op = typed_op<decltype(train)>("vlak::fused_attention_gqa_train");

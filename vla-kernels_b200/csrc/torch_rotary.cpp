@@ -22,6 +22,7 @@ using vlak_torch::check_status;
 using vlak_torch::dtype_code;
 using vlak_torch::new_empty;
 using vlak_torch::raise_pending_device_error;
+using vlak_torch::refuse_tangents;
 using OptTensor = std::optional<Tensor>;
 using Tensors = std::vector<Tensor>;
 
@@ -209,6 +210,7 @@ Tensors call_norm_bwd(const Tensor& gq, const OptTensor& gk, const Tensor& q, co
 }
 
 bool wants_grad(const OptTensor& t) { return present(t) && t->requires_grad(); }
+Tensor or_none(const OptTensor& t) { return t.value_or(Tensor()); }
 
 // Gradient of the rotation: the same op with the turn reversed, on the
 // gradients that arrived (one of the outputs may be unused). It goes through
@@ -247,6 +249,7 @@ struct RotaryFunction : torch::autograd::Function<RotaryFunction> {
 Tensors rotary_autograd(const Tensor& q, const OptTensor& k, const Tensor& positions,
                         const Tensor& inv_freq, bool interleaved, double amplitude,
                         bool inverse) {
+  refuse_tangents({q, or_none(k), inv_freq}, "vlak::rotary");
   if (at::GradMode::is_enabled() && (wants_grad(q) || wants_grad(k)))
     return RotaryFunction::apply(q, k, positions, inv_freq, interleaved, amplitude, inverse);
   at::AutoDispatchBelowADInplaceOrView below;
@@ -299,6 +302,7 @@ Tensors qk_norm_rotary_autograd(const Tensor& q, const OptTensor& k, const Tenso
                                 const OptTensor& kw, const Tensor& positions,
                                 const Tensor& inv_freq, double eps, bool interleaved,
                                 double amplitude) {
+  refuse_tangents({q, or_none(k), qw, or_none(kw), inv_freq}, "vlak::qk_norm_rotary");
   if (at::GradMode::is_enabled() &&
       (wants_grad(q) || wants_grad(k) || wants_grad(qw) || wants_grad(kw)))
     return NormRotaryFunction::apply(q, k, qw, kw, positions, inv_freq, eps, interleaved, amplitude);

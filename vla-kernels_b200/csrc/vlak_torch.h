@@ -4,6 +4,8 @@
 #include <ATen/ATen.h>
 #include <ATen/cuda/EmptyTensor.h>
 
+#include <initializer_list>
+
 #include "vlak_b200.h"
 
 namespace vlak_torch {
@@ -40,6 +42,15 @@ inline int dtype_code(at::ScalarType t) {
 // training call, with its seven or eight tensors, 3 of 80 us.
 inline at::Tensor new_empty(const at::Tensor& like, at::IntArrayRef sizes, at::ScalarType type) {
   return at::Tensor(at::detail::empty_cuda(sizes, type, like.device(), std::nullopt));
+}
+
+// The differentiable ops have no forward-mode derivative. Their autograd kernels
+// go below autograd for inputs that need no gradient, where a tangent would be
+// dropped in silence; so one on any input (they may be undefined) is refused.
+inline void refuse_tangents(std::initializer_list<at::Tensor> inputs, const char* op) {
+  for (const at::Tensor& t : inputs)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(/*level=*/0).defined(), op,
+                                " has no forward-mode derivative");
 }
 
 // Checks and arguments of the GQA attention ops (torch_ops.cpp).

@@ -186,7 +186,7 @@ def fused_attention_gqa_train(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     a fixed order, so gradients repeat bit for bit. A row that sees no key is zeros and has a zero gradient. Values
     that no row may see (a dead band, positions past a sample's length) may be
     anything, NaN included; behind ``attn_mask`` all values must be finite.
-    Differentiable once.
+    Differentiable once, in reverse mode.
 
     To capture a training step into a CUDA graph, let no eager autograd graph
     of the same leaves live meanwhile (drop its loss and outputs first):

@@ -119,7 +119,8 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor,
     shape (B, M), (1, M) or (M,) on the same device; packed q (T, H, D) and
     k (T, H_kv, D) take positions (T,). Pairs are (i, i + rotary_dim / 2), or
     (2i, 2i + 1) when ``interleaved``; both are multiplied by ``amplitude``.
-    Differentiable in q and k, any number of times. Returns new contiguous
+    Differentiable in q and k, any number of times (in reverse mode only: an
+    input with a forward-mode tangent is refused). Returns new contiguous
     tensors (q, k); with k None (keys rotated earlier, as in a cache) just q.
     """
     _ensure_registered()
@@ -140,7 +141,7 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor | None, q_weight: torch.Tens
     over head_dim, in one pass; nothing is rounded between norm and rotation.
 
     q_weight and k_weight are (head_dim,), float32 or of q's dtype.
-    Differentiable once in q, k and the weights (the weights' gradients are
+    Differentiable once, in reverse mode, in q, k and the weights (whose gradients are
     summed in 32 bits in a fixed order, so they repeat bit for bit). Shapes and
     the result are those of ``rotary``; k and k_weight are None together.
     """
