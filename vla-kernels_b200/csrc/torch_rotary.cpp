@@ -211,6 +211,11 @@ Tensors call_norm_bwd(const Tensor& gq, const OptTensor& gk, const Tensor& q, co
 
 bool wants_grad(const OptTensor& t) { return present(t) && t->requires_grad(); }
 Tensor or_none(const OptTensor& t) { return t.value_or(Tensor()); }
+// There is no gradient of the frequencies: where one would be recorded, say so.
+void refuse_frequency_grad(const Tensor& inv_freq, const char* op) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!at::GradMode::is_enabled() || !inv_freq.requires_grad(), op,
+                              " has no gradient of inv_freq; pass inv_freq.detach()");
+}
 
 // Gradient of the rotation: the same op with the turn reversed, on the
 // gradients that arrived (one of the outputs may be unused). It goes through
@@ -250,6 +255,7 @@ Tensors rotary_autograd(const Tensor& q, const OptTensor& k, const Tensor& posit
                         const Tensor& inv_freq, bool interleaved, double amplitude,
                         bool inverse) {
   refuse_tangents({q, or_none(k), inv_freq}, "vlak::rotary");
+  refuse_frequency_grad(inv_freq, "vlak::rotary");
   if (at::GradMode::is_enabled() && (wants_grad(q) || wants_grad(k)))
     return RotaryFunction::apply(q, k, positions, inv_freq, interleaved, amplitude, inverse);
   at::AutoDispatchBelowADInplaceOrView below;
@@ -303,6 +309,7 @@ Tensors qk_norm_rotary_autograd(const Tensor& q, const OptTensor& k, const Tenso
                                 const Tensor& inv_freq, double eps, bool interleaved,
                                 double amplitude) {
   refuse_tangents({q, or_none(k), qw, or_none(kw), inv_freq}, "vlak::qk_norm_rotary");
+  refuse_frequency_grad(inv_freq, "vlak::qk_norm_rotary");
   if (at::GradMode::is_enabled() &&
       (wants_grad(q) || wants_grad(k) || wants_grad(qw) || wants_grad(kw)))
     return NormRotaryFunction::apply(q, k, qw, kw, positions, inv_freq, eps, interleaved, amplitude);

@@ -120,7 +120,8 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor,
     k (T, H_kv, D) take positions (T,). Pairs are (i, i + rotary_dim / 2), or
     (2i, 2i + 1) when ``interleaved``; both are multiplied by ``amplitude``.
     Differentiable in q and k, any number of times (in reverse mode only: an
-    input with a forward-mode tangent is refused). Returns new contiguous
+    input with a forward-mode tangent is refused), not in the frequencies:
+    ``inv_freq`` that requires a gradient is refused. Returns new contiguous
     tensors (q, k); with k None (keys rotated earlier, as in a cache) just q.
     """
     _ensure_registered()
