@@ -301,13 +301,16 @@ struct Turn {
 // rounding of O would weigh as much as that of dS where a row's weight lies on
 // few keys, so the forward pass keeps the next eight bits of each entry of O: the
 // distance of the 32-bit value from its bf16 one, as integers, -2^15 to 2^15,
-// without its low byte (whose middle is taken in its place).
+// rounded to multiples of 2^8, up to 127 of them. So an O that bf16 holds exactly
+// (of a row with one key, whose true dS is 0) stays exact, and bytes of zero stand
+// for no more bits. Such a row's dS comes out as 8e-8 of D, what the 32-bit sums
+// leave; with the upper byte cut off and the lower one's mean added, 1.1e-5.
 __device__ __forceinline__ uint32_t low_bytes(const float* x, const uint32_t* hi) {  // of four entries
   int d[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int top = static_cast<int>(i & 1 ? hi[i >> 1] & 0xffff0000u : hi[i >> 1] << 16);
-    d[i] = min(__float_as_int(x[i]) - top, 0x7fff);  // (a tie may be 2^15)
+    const uint32_t top = i & 1 ? hi[i >> 1] & 0xffff0000u : hi[i >> 1] << 16;
+    d[i] = min(static_cast<int>(__float_as_uint(x[i]) - top + 0x80u), 0x7fff);
   }
   // the second byte of each
   return __byte_perm(__byte_perm(d[0], d[1], 0x0051), __byte_perm(d[2], d[3], 0x0051), 0x5410);
@@ -319,7 +322,7 @@ __device__ __forceinline__ void with_low_bytes(float* x, uint32_t w) {
     // byte i, its sign above it, zero below
     int d;
     asm("prmt.b32 %0, %1, 0, %2;" : "=r"(d) : "r"(w), "r"(0x0004 | i << 4 | (8 + i) << 8 | (8 + i) << 12));
-    x[i] = __int_as_float(__float_as_int(x[i]) + d + 128);
+    x[i] = __int_as_float(__float_as_int(x[i]) + d);
   }
 }
 
