@@ -258,7 +258,8 @@ VLAK_API int vlak_attn_fwd(const void* q, const void* k, const void* v, void* o,
  * Rows that see no key get dq = 0 and add nothing to dk and dv. Keys that no
  * row sees by the analytic mask or the lengths may hold anything (NaN
  * included), and so may rows past their sample's length; those get dk, dv or
- * dq = 0. Behind a bool mask every value must be finite. A NaN or infinity
+ * dq = 0. Where no row of a call sees more than one key (by the analytic mask),
+ * and in samples of length 1, dq and dk are exactly zero. Behind a bool mask every value must be finite. A NaN or infinity
  * that is seen spreads as in the formulas. Results repeat bit for bit.
  *
  * Workspaces: device, 256-byte aligned, owned by the caller and unused by

@@ -113,6 +113,11 @@ struct __align__(64) BwdParams : TrainShape {
   FastDiv by_kblk, by_kv_parts, by_q_parts;
 };
 
+// Softmax over a single key is constant: its score's gradient is exactly zero. So
+// where no row sees more keys, dQ and dK are scaled by zero: in the whole call
+// (out_scale; see run_bwd), or in a sample of length 1.
+__device__ __forceinline__ float scale_of(const BwdParams& p, int L) { return L == 1 ? 0.f : p.out_scale; }
+
 // ---------------------------------------------------------------------------
 // D = rowsum(dO * O), O with its low bytes, and -lse by sub-tile rows: four
 // threads per row, two 16-byte vectors of each tensor per thread. Rows that do not
@@ -767,7 +772,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd(const __grid_constant__ 
                               o[v / 4][v % 4 * 4 + 3]);
           }
         } else {
-          const float scale = dv ? 1.f : p.out_scale;
+          const float scale = dv ? 1.f : scale_of(p, it.L);
           uint8_t* stage = a0 + (dv ? 2 * kSubBytes : 0) + tl * kRowBytes;
 #pragma unroll
           for (int v = 0; v < 4; ++v) {
@@ -857,7 +862,8 @@ __global__ void __launch_bounds__(256) attn_bwd_join_kv(const __grid_constant__ 
   const float4 s = sum_parts(p.kv_sums + (bk * rows + key) * 128 + 4 * v, p.n_bk * rows * 128, p.kv_parts);
   const int b = fast_div(bk, p.by_hkv), kvh = bk - b * p.Hkv;
   const long long at = ((static_cast<long long>(b) * p.N + key) * p.Hkv + kvh) * 64 + 4 * (v & 15);
-  store_4((v < 16 ? p.dk : p.dv) + at, s, v < 16 ? p.out_scale : 1.f);
+  const int L = p.lengths != nullptr ? length_of(p, b) : 0;
+  store_4((v < 16 ? p.dk : p.dv) + at, s, v < 16 ? scale_of(p, L) : 1.f);
 }
 // blockIdx.y: (b, kv head), blockIdx.x: quarter of a sub-tile; 16 threads per row
 __global__ void __launch_bounds__(256) attn_bwd_join_q(const __grid_constant__ BwdParams p) {
@@ -869,8 +875,9 @@ __global__ void __launch_bounds__(256) attn_bwd_join_q(const __grid_constant__ B
   const float4 s = sum_parts(p.q_sums + (bk * rows + st * kSub + row) * 64 + 4 * v, p.n_bk * rows * 64,
                              p.q_parts);
   const int b = fast_div(bk, p.by_hkv), kvh = bk - b * p.Hkv;
+  const int L = p.lengths != nullptr ? length_of(p, b) : 0;
   store_4(p.dq + ((static_cast<long long>(b) * p.M + r.m) * p.H + kvh * p.G + r.g) * 64 + 4 * v, s,
-          p.out_scale);
+          scale_of(p, L));
 }
 
 // ---------------------------------------------------------------------------
@@ -1017,8 +1024,8 @@ int run_bwd(const vlak_attn_train_args* t, void* workspace, int64_t ws_bytes, vo
   p.by_kblk = fast_div_by(static_cast<unsigned>(p.n_kblk));
   p.by_kv_parts = fast_div_by(static_cast<unsigned>(p.kv_parts));
   p.by_q_parts = fast_div_by(static_cast<unsigned>(p.q_parts));
-  // softmax over a single key is constant: its score's gradient is exactly zero
-  p.out_scale = p.N == 1 ? 0.f : p.scale;
+  // the last row sees the most keys: all but the dead ones
+  p.out_scale = p.ds + p.N - p.de <= 1 ? 0.f : p.scale;
   p.host_err = host_error_word(cs);
   p.lse = args.lse;
   p.stats = static_cast<float*>(workspace);
