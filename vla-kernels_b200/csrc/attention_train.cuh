@@ -426,10 +426,14 @@ inline bool fine_call(const vlak_attn_gqa_args& a, int64_t total) {
 }
 // Parts of an item of `steps` steps, in a call of `total` steps: none longer
 // than an SM's even share, but no shorter than eight steps (joining costs
-// about that much), and at most 32.
+// about that much), and at most 32. And whatever the balance, none longer than
+// kMostSteps: some waits last a whole item, a step takes about 0.55 us, and a
+// wait gives up after kWaitLimitNs, seven times what that many take.
+constexpr int64_t kMostSteps = 1 << 18;
 inline int item_parts(int64_t steps, int64_t total) {
   const int64_t most = std::max<int64_t>(8, (total + kPlanSms - 1) / kPlanSms);
-  return static_cast<int>(std::min<int64_t>(32, std::max<int64_t>(1, (steps + most - 1) / most)));
+  const int64_t balanced = std::min<int64_t>(32, (steps + most - 1) / most);
+  return static_cast<int>(std::max<int64_t>({1, balanced, (steps + kMostSteps - 1) / kMostSteps}));
 }
 
 }  // namespace
