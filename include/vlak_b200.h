@@ -261,6 +261,7 @@ VLAK_API int vlak_attn_fwd(const void* q, const void* k, const void* v, void* o,
  * dq = 0. Where no row of a call sees more than one key (by the analytic mask),
  * and in samples of length 1, dq and dk are exactly zero. Behind a bool mask every value must be finite. A NaN or infinity
  * that is seen spreads as in the formulas. Results repeat bit for bit.
+ * At most 2^30 positions and as many keys, and 2^34 rows of q or k in all.
  *
  * Workspaces: device, 256-byte aligned, owned by the caller and unused by
  * anything else until the work on `stream` has finished; sized by the two

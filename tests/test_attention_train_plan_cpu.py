@@ -54,3 +54,25 @@ def test_ordinary_sizes_keep_their_plans():
     # 3 heads of 64 sub-tiles of 64 rows for each kv head (in one box of three
     # heads and 21 positions they would be 196)
     assert sizes(B=2, M=4096, N=4096, H=15, Hkv=5) == [0, 2 * 5 * 3 * 64 * 512 + 256]
+
+
+# 2^30 rows or keys of one head, twice (q and o, k and v), are 275 GB, and 2^34
+# rows in all 2 TB; below them every count of the kernels fits 32 bits
+@pytest.mark.parametrize("attn", [dict(M=(1 << 31) - 1, H=1), dict(M=(1 << 30) + 1, H=1),
+                                  dict(M=1 << 28, H=128), dict(M=1, N=(1 << 31) - 1, H=1),
+                                  dict(M=1, N=(1 << 30) + 1, H=1), dict(M=1, B=1 << 20, N=1 << 15, H=1)])
+def test_sizes_whose_counts_pass_32_bits_are_refused(attn):
+    L, n = lib(), ctypes.c_int64(0)
+    t = args({**dict(B=1, N=64, Hkv=1, prefix_len=-1, dead_start=0, dead_end=0), **attn})
+    for f in (L.vlak_attn_gqa_train_workspace_size, L.vlak_attn_gqa_bwd_workspace_size):
+        assert f(ctypes.byref(t), ctypes.byref(n)) == 1 and n.value == 0
+    assert L.vlak_attn_gqa_train_fwd(ctypes.byref(t), 0x1000, 1 << 60, None) == 1
+    assert L.vlak_attn_gqa_bwd(ctypes.byref(t), 0x1000, 1 << 60, None) == 1
+    assert b"too many rows or keys" in L.vlak_last_error_message()
+
+
+def test_the_largest_sizes_have_plans():
+    for attn in (dict(M=1 << 30, N=64, H=1, Hkv=1), dict(M=1, N=1 << 30, H=1, Hkv=1),
+                 dict(M=1 << 27, N=64, H=128, Hkv=1)):
+        fwd, bwd = sizes(B=1, **attn)
+        assert 0 <= fwd < 1 << 50 and 0 < bwd < 1 << 50

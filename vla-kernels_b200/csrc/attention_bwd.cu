@@ -728,7 +728,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd(const __grid_constant__ 
                               it.k0 + tl) * 128;
         else if ((quarter >> 1) < it.n_here)
           sums = p.q_sums + ((static_cast<long long>(it.part) * p.n_bk + bk) * p.n_sub * kSub +
-                             it.s0 * kSub + tl) * 64;
+                             static_cast<long long>(it.s0) * kSub + tl) * 64;
       }
       if (it.live == 0) {  // nothing seen: zeros
         const int key = it.k0 + tl;
@@ -872,8 +872,8 @@ __global__ void __launch_bounds__(256) attn_bwd_join_q(const __grid_constant__ B
   const SubRow r = sub_row(p, st, row);
   if (!r.valid) return;
   const long long rows = static_cast<long long>(p.n_sub) * kSub;
-  const float4 s = sum_parts(p.q_sums + (bk * rows + st * kSub + row) * 64 + 4 * v, p.n_bk * rows * 64,
-                             p.q_parts);
+  const float4 s = sum_parts(p.q_sums + (bk * rows + static_cast<long long>(st) * kSub + row) * 64 + 4 * v,
+                             p.n_bk * rows * 64, p.q_parts);
   const int b = fast_div(bk, p.by_hkv), kvh = bk - b * p.Hkv;
   const int L = p.lengths != nullptr ? length_of(p, b) : 0;
   store_4(p.dq + ((static_cast<long long>(b) * p.M + r.m) * p.H + kvh * p.G + r.g) * 64 + 4 * v, s,

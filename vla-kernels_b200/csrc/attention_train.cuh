@@ -377,14 +377,15 @@ inline TrainShape train_shape(const vlak_attn_gqa_args* a, int64_t P, float scal
   s.by_gb = fast_div_by(static_cast<unsigned>(s.Gb));
   return s;
 }
-// The inference entry points' checks, and that counts stay within 64 bits (2^40
-// rows of 128 bytes are more than any memory).
+// The inference entry points' checks, and that counts stay within 32 bits: at most
+// 2^30 positions or keys (of one head, twice, 275 GB) and 2^34 rows in all (2 TB).
+// A sub-tile holds 33 rows or more of a long call, so there are under 2^29.
 inline int check_train(const vlak_attn_gqa_args* a, int64_t* P, float* scale, const char* op) {
   const int st = vlak_attn_gqa_check(a, P, scale);
   if (st != VLAK_OK) return st;
-  constexpr double kMost = 0x1p40;
-  if (static_cast<double>(a->B) * a->M * a->H > kMost || static_cast<double>(a->B) * a->N * a->Hkv > kMost ||
-      static_cast<double>(a->B) * a->Hkv > INT32_MAX)
+  constexpr double kMost = 0x1p34;
+  if (a->M > 1 << 30 || a->N > 1 << 30 || static_cast<double>(a->B) * a->M * a->H > kMost ||
+      static_cast<double>(a->B) * a->N * a->Hkv > kMost || static_cast<double>(a->B) * a->Hkv > INT32_MAX)
     return set_errorf(VLAK_ERR_INVALID_ARGUMENT, "%s: too many rows or keys", op);
   return VLAK_OK;
 }

@@ -484,7 +484,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_train_fwd(const __grid_const
       long long part_row = 0;
       if (p.parts > 1)
         part_row = (static_cast<long long>(it.part) * p.n_bk + it.b * p.Hkv + it.kvh) * p.n_sub * kSub +
-                   it.s0 * kSub + tl;
+                   static_cast<long long>(it.s0) * kSub + tl;
       if (it.live == 0) {  // no key seen
         if (p.parts > 1) {
           if (r.valid) p.ml[part_row] = make_float2(-INFINITY, 0.f);
@@ -635,7 +635,7 @@ __global__ void __launch_bounds__(256) attn_train_fwd_join(const __grid_constant
   const SubRow r = sub_row(p, st, row64);
   if (!r.valid) return;
   const long long rows = static_cast<long long>(p.n_sub) * kSub, stride = p.n_bk * rows;
-  const long long at = bk * rows + st * kSub + row64;
+  const long long at = bk * rows + static_cast<long long>(st) * kSub + row64;
   float m = -INFINITY;
   for (int k = 0; k < p.parts; ++k) m = fmaxf(m, p.ml[k * stride + at].x);
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
