@@ -257,10 +257,12 @@ VLAK_API int vlak_attn_fwd(const void* q, const void* k, const void* v, void* o,
  *              of each kv head (backward only); both NULL for dq alone
  * Rows that see no key get dq = 0 and add nothing to dk and dv. Keys that no
  * row sees by the analytic mask or the lengths may hold anything (NaN
- * included), and so may rows past their sample's length; those get dk, dv or
- * dq = 0. Where no row of a call sees more than one key (by the analytic mask),
- * and in samples of length 1, dq and dk are exactly zero. Behind a bool mask every value must be finite. A NaN or infinity
- * that is seen spreads as in the formulas. Results repeat bit for bit.
+ * included), and so may rows that see no key by them (past their sample's
+ * length, or ahead of the staircase); those get dk, dv or dq = 0. Where no row
+ * of a call sees more than one key by the analytic mask, and in samples of
+ * length 1, dq and dk are exactly zero. Behind a bool mask every value must be
+ * finite. A NaN or infinity that is seen spreads as in the formulas. Results
+ * repeat bit for bit.
  * At most 2^30 positions and as many keys, and 2^34 rows of q or k in all.
  *
  * Workspaces: device, 256-byte aligned, owned by the caller and unused by

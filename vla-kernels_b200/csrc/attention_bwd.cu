@@ -393,8 +393,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd(const __grid_constant__ 
     const uint32_t id_kk = idesc_bf16_f32(128, 64, false);
     const uint64_t a_desc = sdesc_sw128(smem_u32(a_smem)), b_desc = sdesc_sw128(smem_u32(b_smem));
     // streamed rows that meet X = 0 only, and may hold NaN, are cleared: keys
-    // that no query sees (dq), query rows past L (dkv)
-    const bool dead = kMode == kMaskLength || (kMode == kMaskAnalytic && p.ds < p.de);
+    // that no query sees (dq), query rows past L or that see no key (dkv): under a
+    // staircase behind nothing but dead keys the first `unseeing` positions
+    const int unseeing = kMode == kMaskAnalytic && p.ds == 0 && p.de == p.P ? max(0, p.P - (p.N - p.M)) : 0;
+    const bool dead = kMode == kMaskLength || (kMode == kMaskAnalytic && (p.ds < p.de || unseeing > 0));
     Turn<kTiles> ab;
     Turn<kRing> s;
     Turn<kStages> st;
@@ -421,10 +423,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd(const __grid_constant__ 
             const int lo = kMode == kMaskLength ? it.L - c0 : p.ds - c0;
             const int hi = kMode == kMaskLength ? kChunk : p.de - c0;
             clear_rows(bp, max(lo, 0), min(hi, kChunk));
-          } else if (kMode == kMaskLength) {
-            const int lo = max(0, it.L - step.pos * p.MT) * p.Gb;
-            clear_rows(bp, lo, kSub);
-            clear_rows(bp + kSubBytes, lo, kSub);
+          } else {
+            // rows of the step's positions before L, or before the first that sees
+            const int n = (kMode == kMaskLength ? it.L : unseeing) - step.pos * p.MT;
+            const int before = min(min(max(n, 0), kSub) * p.Gb, kSub);
+            const int lo = kMode == kMaskLength ? before : 0, hi = kMode == kMaskLength ? kSub : before;
+            clear_rows(bp, lo, hi);
+            clear_rows(bp + kSubBytes, lo, hi);
           }
           step.next(it);
         }

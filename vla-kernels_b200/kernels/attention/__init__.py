@@ -183,8 +183,9 @@ def fused_attention_gqa_train(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     The backward pass (vla-kernels_b200/csrc/attention_bwd.cu) recomputes the
     probabilities; between the passes only q, k, v, the output (with eight
     more bits of each entry) and one float per row are kept. Sums are 32-bit in
-    a fixed order, so gradients repeat bit for bit. A row that sees no key is zeros and has a zero gradient. Values
-    that no row may see (a dead band, positions past a sample's length) may be
+    a fixed order, so gradients repeat bit for bit. A row that sees no key is
+    zeros and has a zero gradient. Values that no row may see (a dead band,
+    positions past a sample's length), and those of rows that see nothing, may be
     anything, NaN included; behind ``attn_mask`` all values must be finite.
     Differentiable once, in reverse mode.
 
