@@ -699,10 +699,11 @@ int validate(const vlak_rotary_args* a, int mode, const char* op) {
     return set_errorf(VLAK_ERR_INVALID_ARGUMENT, "%s: the rotated part must be even, 2 to head_dim", op);
   if (a->n_tensors < 1 || a->n_tensors > 2)
     return set_errorf(VLAK_ERR_INVALID_ARGUMENT, "%s: one or two tensors", op);
-  if (!isfinite(a->amplitude))
+  // (both as the kernels take them, in 32 bits)
+  if (!isfinite(static_cast<float>(a->amplitude)))
     return set_errorf(VLAK_ERR_INVALID_ARGUMENT, "%s: amplitude must be finite", op);
   if (mode != kRotate) {
-    if (!(a->eps >= 0) || !isfinite(a->eps))
+    if (!(a->eps >= 0) || !isfinite(static_cast<float>(a->eps)))
       return set_errorf(VLAK_ERR_INVALID_ARGUMENT, "%s: eps must be finite and not negative", op);
     if (a->weight_dtype != VLAK_F32 && a->weight_dtype != a->dtype)
       return set_errorf(VLAK_ERR_UNSUPPORTED_DTYPE, "%s: weights must be fp32 or of the heads' dtype", op);
