@@ -1087,14 +1087,7 @@ int run_bwd(const vlak_attn_train_args* t, void* workspace, int64_t ws_bytes, vo
 
 }  // namespace
 
-int take_bwd_device_error(int* code) {
-  cudaError_t e = cudaMemcpyFromSymbol(code, g_device_error, sizeof(int));
-  if (e != cudaSuccess) return set_cuda_error("vlak_device_error_read", e);
-  const int zero = 0;
-  e = cudaMemcpyToSymbol(g_device_error, &zero, sizeof(int));
-  if (e != cudaSuccess) return set_cuda_error("vlak_device_error_read", e);
-  return VLAK_OK;
-}
+int take_bwd_device_error(int* code) { return take_device_error(code); }
 
 }  // namespace vlak
 

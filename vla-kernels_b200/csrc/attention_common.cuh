@@ -31,6 +31,15 @@ __device__ __forceinline__ void publish_device_error(int* host_err, int code) {
   }
 }
 
+// Reads and clears the device error word of the including translation unit.
+inline int take_device_error(int* code) {
+  cudaError_t e = cudaMemcpyFromSymbol(code, g_device_error, sizeof(int));
+  if (e != cudaSuccess) return set_cuda_error("vlak_device_error_read", e);
+  const int zero = 0;
+  e = cudaMemcpyToSymbol(g_device_error, &zero, sizeof(int));
+  return e == cudaSuccess ? VLAK_OK : set_cuda_error("vlak_device_error_read", e);
+}
+
 constexpr uint64_t kWaitLimitNs = 1000ull * 1000ull * 1000ull;  // 1 s per wait
 
 // Bounded parity wait; `abort_flag` (shared) short-circuits the other
@@ -77,27 +86,6 @@ __device__ __forceinline__ void clear_rows(uint8_t* tile, int lo, int hi) {
   __syncwarp();
 }
 
-// Bits of keys g0 .. g0+31 of one bool-mask row of N keys; words: the row starts
-// 4-byte aligned (bit i set when key g0 + i is
-// below N and its mask byte is nonzero).
-__device__ __forceinline__ uint32_t mask_bits32(const uint8_t* row, int g0, int N,
-                                                bool words) {
-  uint32_t vm = 0u;
-  if (words && g0 + 32 <= N) {
-    const uint32_t* w = reinterpret_cast<const uint32_t*>(row + g0);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      // one byte per key -> bytes 0x01 / 0x00 -> four bits gathered by a
-      // multiply (the partial products of distinct bytes never overlap)
-      const uint32_t b = __vcmpne4(__ldg(w + i), 0u) & 0x01010101u;
-      vm |= ((b * 0x01020408u) >> 24) << (4 * i);
-    }
-  } else {
-    const int n = min(32, N - g0);
-    for (int i = 0; i < n; ++i) vm |= (__ldg(row + g0 + i) != 0 ? 1u : 0u) << i;
-  }
-  return vm;
-}
 // Tensor map of dims (64, d1, d2, d3) with element strides s1..s3 and box
 // (64, box1, box2, 1), rows in the 128-byte swizzle.
 inline int encode_map(CUtensorMap* map, const void* base, int64_t d1, int64_t d2, int64_t d3,

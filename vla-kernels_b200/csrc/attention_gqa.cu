@@ -275,6 +275,27 @@ __device__ __forceinline__ int live_next(const LiveSet& s, int c) {
   return -1;
 }
 
+// Bits of keys g0 .. g0+31 of one bool-mask row of N keys: bit i is set when key
+// g0 + i is below N and its mask byte is nonzero. words: the row starts 4-byte
+// aligned.
+__device__ __forceinline__ uint32_t mask_bits32(const uint8_t* row, int g0, int N,
+                                                bool words) {
+  uint32_t vm = 0u;
+  if (words && g0 + 32 <= N) {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(row + g0);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      // one byte per key -> bytes 0x01 / 0x00 -> four bits gathered by a
+      // multiply (the partial products of distinct bytes never overlap)
+      const uint32_t b = __vcmpne4(__ldg(w + i), 0u) & 0x01010101u;
+      vm |= ((b * 0x01020408u) >> 24) << (4 * i);
+    }
+  } else {
+    const int n = min(32, N - g0);
+    for (int i = 0; i < n; ++i) vm |= (__ldg(row + g0 + i) != 0 ? 1u : 0u) << i;
+  }
+  return vm;
+}
 __device__ __forceinline__ int chunk_cols(const Params& p, int c) {
   const int width = min(kChunk, p.N - c * kChunk);
   return (width + 15) & ~15;  // MMA N must be a multiple of 16
@@ -1399,13 +1420,9 @@ extern "C" int vlak_attn_gqa_fwd_noalloc(const vlak_attn_gqa_args* args, void* s
 extern "C" int vlak_device_error_read(int* code) {
   vlak::clear_error();
   int v = 0;
-  cudaError_t e = cudaMemcpyFromSymbol(&v, vlak::g_device_error, sizeof(int));
-  if (e != cudaSuccess) return vlak::set_cuda_error("vlak_device_error_read", e);
-  const int zero = 0;
-  e = cudaMemcpyToSymbol(vlak::g_device_error, &zero, sizeof(int));
-  if (e != cudaSuccess) return vlak::set_cuda_error("vlak_device_error_read", e);
-  // the training kernels' words
-  for (int (*take)(int*) : {vlak::take_train_fwd_device_error, vlak::take_bwd_device_error}) {
+  // this kernel's word, and the training kernels'
+  for (int (*take)(int*) : {vlak::take_device_error, vlak::take_train_fwd_device_error,
+                            vlak::take_bwd_device_error}) {
     int more = 0;
     const int st = take(&more);
     if (st != VLAK_OK) return st;
