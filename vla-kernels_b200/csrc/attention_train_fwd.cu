@@ -21,9 +21,12 @@
 // kernel's parts are held in bf16). P is rounded to bf16 as the operand of P V, or
 // to twice that in fine calls (see kFineShare).
 //
-// Bound: by the products' shared-memory reads and issue, 4 SS products of about
-// 49 cycles and 4 TS products of about 43 per 128 x 64 step, then the
-// exponentials, 512 cycles of the special-function units.
+// Bound: no unit alone. A 128 x 64 step needs 512 cycles of the special-function
+// units (its exponentials, 16 per cycle) and 368 of the products (4 SS of about 49
+// and 4 TS of about 43, by their shared-memory reads and issue), and takes about
+// 1000 (causal, 2 x 4096 rows, 15 heads: 214 steps per SM in 112 us): the chain from
+// S in TMEM over the exponentials to P in TMEM, handed over by barriers at both
+// ends, sets the time.
 //
 // Every mbarrier wait is bounded as in the inference kernel.
 

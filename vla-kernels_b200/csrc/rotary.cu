@@ -80,7 +80,9 @@ __device__ __forceinline__ unsigned long long turns_of(double f) {
 // (A cos t, +-A sin t) of the turn position * turns. For 16-bit heads the
 // hardware's sine and cosine: within 2^-21 of the value on half a turn to each
 // side, 2^-10 of half a step of fp16; sincospi, four times the instructions,
-// for 32-bit ones.
+// for 32-bit ones. Either takes the fraction as a float, rounded to 2^-26 of a turn
+// at most: 9e-8 radians, 1.6 roundings of an fp32 result, whose error is 1.3 times
+// that with angles in 64 bits.
 template <typename T>
 __device__ __forceinline__ float2 turn_of(const RotParams& p, unsigned long long pos,
                                           unsigned long long turns) {

@@ -30,8 +30,10 @@ __device__ __forceinline__ float warp_sum(float v) {
 }
 
 // ---------------------------------------------------------------------------
-// n / d for n < 2^31 by a multiplication: m = ceil(2^(32 + l) / d) - 2^32 with
-// l = ceil(log2 d); (n m >> 32) + n is below 2^32 for n < 2^31.
+// n / d for n < 2^31 by a multiplication and a shift (Granlund and Montgomery,
+// "Division by invariant integers using multiplication", 1994):
+// m = ceil(2^(32 + l) / d) - 2^32 with l = ceil(log2 d); (n m >> 32) + n is below
+// 2^32 for n < 2^31.
 struct FastDiv {
   unsigned d, m, l;
 };
