@@ -79,19 +79,27 @@ __device__ __forceinline__ unsigned long long turns_of(double f) {
 }
 // (A cos t, +-A sin t) of the turn position * turns. For 16-bit heads the
 // hardware's sine and cosine: within 2^-21 of the value on half a turn to each
-// side, 2^-10 of half a step of fp16; sincospi, four times the instructions,
-// for 32-bit ones. Either takes the fraction as a float, rounded to 2^-26 of a turn
-// at most: 9e-8 radians, 1.6 roundings of an fp32 result, whose error is 1.3 times
-// that with angles in 64 bits.
+// side, 2^-10 of half a step of fp16, beside which the 2^-26 of a turn that a float
+// of the fraction may be off (9e-8 radians) are nothing. For 32-bit heads sincospi,
+// four times the instructions, and what the float left of the fraction, r, by
+// cos (t + r) = cos t - r sin t, sin (t + r) = sin t + r cos t: without it results
+// were 1.33 times as far off as with angles in 64 bits, with it 0.98 times, in the
+// same time (8191 x 40 heads of 128: 54 us).
 template <typename T>
 __device__ __forceinline__ float2 turn_of(const RotParams& p, unsigned long long pos,
                                           unsigned long long turns) {
   const int part = static_cast<int>((pos * turns) >> 32);  // of a turn, in 2^-32, -1/2 to 1/2
+  constexpr float kRadians = 1.4629180792671596e-9f;       // 2 pi 2^-32
+  const float near = static_cast<float>(part);
   float s, c;
   if constexpr (sizeof(T) == 2) {
-    __sincosf(static_cast<float>(part) * 1.4629180792671596e-9f, &s, &c);  // 2 pi 2^-32
+    __sincosf(near * kRadians, &s, &c);
   } else {
-    sincospif(static_cast<float>(part) * 0x1p-31f, &s, &c);
+    float s0, c0;
+    sincospif(near * 0x1p-31f, &s0, &c0);
+    const float r = static_cast<float>(part - __float2int_rn(near)) * kRadians;
+    c = fmaf(-r, s0, c0);
+    s = fmaf(r, c0, s0);
   }
   return make_float2(p.amp * c, p.amp * p.sign * s);
 }
